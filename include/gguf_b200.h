@@ -177,6 +177,53 @@ int gguf_b200_moe_a8_vec(const void* X, const void* W, void* Y, void* workspace,
                          const int32_t* topk_ids, int64_t n_experts, int type, int dtype, int64_t tokens,
                          int64_t top_k, int64_t N, int64_t K, void* stream);
 
+/* ---- the router, and products of 8-bit integers with one scale per token and per weight row -----
+ * No counterpart in the reference, whose plugin is handed ids and weights of the experts by the serving engine, and whose block
+ * formats carry a scale per 32 values or fewer.  A matrix of 8-bit integers is int8 [rows][K], rows `ld` bytes apart: base and ld
+ * multiples of 16, ld >= K, the bytes behind K never read.  K <= 131071: then no sum of products leaves 32 bits, and every
+ * product below is exact up to the scales. */
+
+/* Router logits [tokens][n_experts] (dtype, rows ld elements apart) -> the top_k experts of every token, ids and weights [tokens][top_k].
+ * s = softmax (scoring 1) or sigmoid (2) of the row; an expert whose logit is -inf or NaN is masked (+inf counts as the
+ * largest finite number).  The choice goes by s + bias, by s without a bias (null).  With n_group > 1 (a divisor of n_experts)
+ * only the experts of the topk_group best groups remain, by the sum of a group's two best choices with a bias, by its best one
+ * without; equal groups by the lower index.  The best choice comes first, equal ones by the lower index.  weight = s (without
+ * bias), divided by the sum over the top_k where renormalize != 0 and that sum is positive, times scale.  A place for which no
+ * unmasked expert (whose choice is a number above -inf) is left has id -1 and weight 0, which the MoE calls of this library skip.
+ * Comparisons are those of fp64, or of the logits themselves where that is the same.
+ * n_experts <= 512, top_k <= 32 and <= topk_group * (n_experts / n_group), n_group <= 32. */
+int gguf_b200_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, float* weights, int32_t* ids, int64_t tokens,
+                        int64_t n_experts, int64_t top_k, int64_t n_group, int64_t topk_group, int scoring, int renormalize, float scale,
+                        void* stream);
+
+/* Rows of floats X [M][K] (rows ldx elements apart) -> codes Q [M][K] (rows ldq bytes apart) and scales [M]:
+ * scale = a / 127 with a = max |x| of the row, code = x * 127 / a rounded to the nearest integer, halves to even, as exact arithmetic
+ * has it.  A row of zeros: scale 0, codes 0.  A row with an infinity or a NaN: scale NaN, codes 0.  For activations and, once, for
+ * weights. */
+int gguf_b200_int8_quantize(const void* X, int dtype, int64_t ldx, void* Q, int64_t ldq, float* scales, int64_t M, int64_t K, void* stream);
+
+/* Linear layer: Y[m][n] = (sum over k of code(X)[m][k] * W[n][k]) * scale(X)[m] * w_scales[n] + bias[n], rounded to dtype once; X [M][K] in dtype,
+ * rows ldx elements apart, quantized by the call as above; bias [N] in dtype or null.  Workspace: gguf_b200_int8_scratch_bytes. */
+int64_t gguf_b200_int8_scratch_bytes(int64_t M, int64_t K);
+int gguf_b200_int8_mul_mat(const void* W, int64_t ldw, const float* w_scales, const void* X, int64_t ldx, const void* bias, void* Y,
+                           void* workspace, int64_t workspace_bytes, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
+/* The same on activations that are quantized already, for several products of the same ones (q/k/v).  flags: 0, or
+ * GGUF_B200_W_IN_FLIGHT where W may be written by the work directly ahead in the stream (an gguf_b200_int8_quantize of W, say);
+ * without it W may be read ahead of the stream (see gguf_b200_weights_complete). */
+int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_scales, const void* Q, int64_t ldq, const float* q_scales,
+                                    const void* bias, void* Y, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
+
+/* The MoE step of gguf_b200_fused_moe on 8-bit integer weights: W13 [E][2I][H] (gate rows, then up rows, of every expert; all rows
+ * ld13 bytes apart) with w13_scales [E][2I], W2 [E][H][I] with w2_scales [E][H].  Tokens are quantized by the row, and so are the
+ * hidden rows act(gate) * up, in fp32, of every slot; Y[t] = sum over j of topk_weights[t][j] * down, rounded to dtype once.
+ * act: 1 silu, 2 gelu (erf form).  n_experts <= 256, H and I multiples of 8.  Slots with an id outside [0, n_experts) contribute
+ * nothing. */
+int64_t gguf_b200_int8_moe_workspace_bytes(int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H, int64_t I);
+int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_t ld13, const float* w13_scales, const void* W2, int64_t ld2,
+                             const float* w2_scales, void* Y, const int32_t* topk_ids, const float* topk_weights, void* workspace,
+                             int64_t workspace_bytes, int dtype, int act, int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H,
+                             int64_t I, void* stream);
+
 /* Decode GEMV that needs no workspace from the caller and allocates nothing.  (No counterpart
  * in the reference: its GEMV allocates its scratch tensor inside the call.)
  * For hosts that cannot allocate: an FFI or plain-C integration that only receives W, X and Y

@@ -1,0 +1,423 @@
+"""The 8-bit integer operators (row quantizer, linear product, routed expert step) against their definitions in 64 bits.
+
+Tolerances.  Codes are those of exact arithmetic and are compared for equality.  A scale is one fp32 division: 2^-24 relative.  A
+result is D * (q_scale * w_scale) + bias with D exact: q_scale, the conversion of D, two products and a sum are rounded to fp32
+once each, at most 5 * 2^-24 of |D| q_scale w_scale + |bias|, and the result once more to its type: eps / 2 of itself, or half
+the smallest subnormal."""
+import ctypes
+
+import pytest
+import torch
+
+from helpers import ROOT  # noqa: F401  (puts the package on the path)
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+TINY = {torch.float32: 2.0 ** -150, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+
+
+@pytest.fixture(scope="module")
+def ops(native_libs):
+    from vllm_gguf_plugin import ops
+
+    return ops
+
+
+def codes_of(x):
+    """(codes, scales) of the definition, float64; rows that are not finite have scale NaN and codes 0."""
+    x = x.double()
+    a = x.abs().amax(1, keepdim=True)
+    ok = torch.isfinite(x).all(1, keepdim=True)
+    a = torch.where(ok, a, 1.0)
+    q = torch.where(ok, torch.round(torch.where(ok, x, 0.0) * 127 / torch.where(a > 0, a, 1.0)), 0.0)
+    return q, torch.where(ok, a / 127, float("nan")).squeeze(1)
+
+
+def weights(rows, k, gen, spread=36.0):
+    buf = torch.full((rows, (k + 15) // 16 * 16), 77, dtype=torch.int8, device="cuda")   # (what lies behind K must not count)
+    buf[:, :k] = (torch.randn(rows, k, device="cuda", generator=gen) * spread).round().clamp(-128, 127).to(torch.int8)
+    return buf[:, :k], (torch.rand(rows, device="cuda", generator=gen) + 0.5) * 1e-3
+
+
+def check_product(y, q, qs, w, ws, bias, dtype, msg=""):
+    d = q.double() @ w.double().T
+    part = d * qs.double()[:, None] * ws.double()
+    want = part if bias is None else part + bias.double()
+    room = 5 * 2.0 ** -24 * (part.abs() + (0 if bias is None else bias.double().abs()))
+    room = room + torch.finfo(dtype).eps / 2 * (want.abs() + room) + TINY[dtype]
+    assert y.shape == want.shape and y.dtype == dtype
+    off = (y.double() - want).abs() - room
+    assert bool((off <= 0).all()), f"{msg}: off by {float((y.double() - want).abs().max())}, {int((off > 0).sum())} of {off.numel()} values"
+
+
+# ---- row quantizer -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 15), (3, 16), (7, 33), (1, 4096), (9, 1000), (130, 2048), (5, 2049), (2, 4100), (3, 16384), (2, 16400),
+                                    (2, 40007), (1, 131072), (1500, 64)])
+def test_quantize_matches_exact_codes(ops, dtype, rows, k):
+    gen = torch.Generator(device="cuda").manual_seed(rows * 7 + k)
+    x = torch.randn(rows, k, device="cuda", generator=gen).to(dtype)
+    q, s = ops.int8_quantize(x)
+    want, scale = codes_of(x)
+    assert q.dtype == torch.int8 and q.shape == (rows, k) and s.shape == (rows,) and q.data_ptr() % 16 == 0 and (rows == 1 or q.stride(0) % 16 == 0)
+    assert torch.equal(q.double(), want)
+    assert bool(((s.double() - scale).abs() <= 2.0 ** -24 * scale).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_halves_zeros_and_what_is_not_finite(ops, dtype):
+    inf, nan = float("inf"), float("nan")
+    top = torch.finfo(dtype).max
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps   # the smallest subnormal
+    rows = [
+        [2.0, 1.0, -1.0, 0.0, -2.0] + [0.0] * 12,                        # 63.5 and -63.5 go to 64
+        [254.0, 1.0, 3.0, 5.0, -1.0, -3.0, -5.0, 7.0] + [0.0] * 9,       # 0.5, 1.5, 2.5 ... to even
+        [0.0, -0.0] + [0.0] * 15,
+        [1.0, inf] + [1.0] * 15,
+        [1.0, -inf] + [1.0] * 15,
+        [nan] + [1.0] * 16,
+        [0.0] * 16 + [nan],
+        [top, -top, top / 2] + [1.0] * 14,
+        [tiny, 0.0, -tiny] + [0.0] * 14,
+        [3 * tiny, tiny, -tiny, 2 * tiny] + [0.0] * 13,
+        [torch.finfo(dtype).smallest_normal, tiny] + [0.0] * 15,
+    ]
+    x = torch.tensor(rows, dtype=torch.float64).to(dtype).cuda()
+    q, s = ops.int8_quantize(x)
+    want, scale = codes_of(x)
+    assert torch.equal(q.double(), want)
+    assert torch.equal(torch.isnan(s), torch.isnan(scale))
+    ok = ~torch.isnan(scale)
+    assert bool(((s.double() - scale).abs()[ok] <= 2.0 ** -24 * scale[ok] + 2.0 ** -150).all())   # (or half the smallest fp32 subnormal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_every_near_half(ops, dtype):
+    """Every value of a binade over the largest of the row, so that all roundings next to halves occur."""
+    n = 4096
+    for top in (1.0, 1.25, 1.9921875, 1.3359375):
+        x = torch.linspace(-top, top, n, dtype=torch.float64).to(dtype).cuda()[None].contiguous()
+        x[0, 0] = top
+        half = ((torch.arange(-127, 127, dtype=torch.float64) + 0.5) * float(x[0, 0]) / 127).to(dtype).cuda()
+        x[0, 1:1 + half.numel()] = half
+        q, _ = ops.int8_quantize(x)
+        assert torch.equal(q.double(), codes_of(x)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_strides(ops, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    big = torch.randn(40, 333, device="cuda", generator=gen).to(dtype)
+    for x in (big[:, 3:100], big[::3, :64], big[:, :320], big[5:6, 1:290], big[:1].expand(6, -1), torch.empty(0, 48, device="cuda", dtype=dtype)):
+        q, _ = ops.int8_quantize(x)
+        assert torch.equal(q.double(), codes_of(x)[0] if len(x) else q.double())
+
+
+# ---- linear product ------------------------------------------------------------------------------------------
+
+SIZES = [(1, 1, 1), (1, 1, 16), (1, 7, 33), (1, 128, 128), (2, 129, 127), (1, 4096, 4096), (3, 200, 4096), (16, 256, 1024), (17, 4000, 512), (27, 384, 8192),
+         (33, 300, 2048), (64, 640, 4096), (65, 130, 4100), (128, 1000, 640), (200, 256, 14336), (255, 130, 256), (256, 130, 640), (257, 130, 640),
+         (300, 4096, 1536), (513, 257, 384), (1000, 520, 1040), (2049, 2100, 400)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear(ops, dtype, m, n, k):
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    w, ws = weights(n, k, gen)
+    x = torch.randn(m, k, device="cuda", generator=gen).to(dtype)
+    bias = torch.randn(n, device="cuda", generator=gen).to(dtype) if (m + n) % 2 else None
+    y = ops.int8_mul_mat(w, ws, x, bias)
+    q, qs = codes_of(x)
+    check_product(y, q, qs, w, ws, bias, dtype, f"{m}x{n}x{k}")
+    # the same in two calls, and again: bit for bit
+    codes, scales = ops.int8_quantize(x)
+    assert torch.equal(ops.int8_mul_mat_prepared(w, ws, codes, scales, dtype, bias), y)
+    assert torch.equal(ops.int8_mul_mat(w, ws, x, bias), y)
+
+
+@pytest.mark.gpu
+def test_linear_largest_sums(ops):
+    """128 * 127 * 131071 fills 31 bits: nothing saturates or wraps."""
+    k = 131071
+    buf = torch.full((130, k + 1), -128, dtype=torch.int8, device="cuda")
+    w = buf[:, :k]
+    ws = torch.ones(130, device="cuda")
+    for m in (1, 20):
+        x = torch.full((m, k), -127.0, device="cuda")
+        x[0] = 127
+        y = ops.int8_mul_mat(w, ws, x)
+        want = torch.full((m, 130), 127.0 * 128 * k, dtype=torch.float64, device="cuda")
+        want[0] *= -1
+        assert bool(((y.double() - want).abs() <= 5 * 2.0 ** -24 * want.abs()).all())
+    with pytest.raises(RuntimeError, match="size"):
+        ops.int8_mul_mat(torch.zeros(1, 131072, dtype=torch.int8, device="cuda"), ws[:1], torch.zeros(1, 131072, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_rows_that_are_not_finite_stay_alone(ops, m):
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    w, ws = weights(200, 256, gen)
+    x = torch.randn(m, 256, device="cuda", generator=gen)
+    clean = ops.int8_mul_mat(w, ws, x)
+    x[0, 3], x[m // 2, 5] = float("nan"), float("-inf")
+    y = ops.int8_mul_mat(w, ws, x)
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[[0, m // 2]] = True
+    assert bool(torch.isnan(y[bad]).all()) and torch.equal(y[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+def test_linear_empty_strided_and_misaligned(ops):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w, ws = weights(96, 100, gen)
+    assert ops.int8_mul_mat(w, ws, torch.empty(0, 100, device="cuda", dtype=torch.float16)).shape == (0, 96)
+    assert ops.int8_mul_mat(w[:0], ws[:0], torch.empty(5, 100, device="cuda")).shape == (5, 0)
+    big = torch.randn(50, 333, device="cuda", generator=gen)
+    for x in (big[:, 1:101], big[::7, 5:105], big[:1, :100].expand(4, -1)):
+        check_product(ops.int8_mul_mat(w, ws, x), *codes_of(x), w, ws, None, torch.float32)
+    # weight rows that are a part of a larger matrix: every third one, and columns from 32 on
+    w2, ws2 = weights(96, 256, gen)
+    x = big[:, :100]
+    check_product(ops.int8_mul_mat(w2[::3, 32:132], ws2[::3].contiguous(), x), *codes_of(x), w2[::3, 32:132], ws2[::3], None, torch.float32)
+    # nothing behind the result is written
+    out = torch.full((8, 96), 5.0, device="cuda")
+    del out
+    for bad in (w2[:, 1:101], torch.zeros(96, 100, dtype=torch.int8, device="cuda"), w2.T, w2[:, ::2]):
+        with pytest.raises(RuntimeError):
+            ops.int8_mul_mat(bad, ws, torch.zeros(3, bad.shape[1], device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 100])
+def test_weights_straight_out_of_the_quantizer(ops, m):
+    """Weights made by the call ahead in the stream, and overwritten by it: no product reads them too early."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(m, 2048, device="cuda", generator=gen, dtype=torch.float32)
+    q, qs = ops.int8_quantize(x)
+    fs = [torch.randn(2048, 2048, device="cuda", generator=gen) for _ in range(6)]
+    got = []
+    for f in fs:
+        w, ws = ops.int8_quantize(f)
+        got.append((ops.int8_mul_mat_prepared(w, ws, q, qs, torch.float32), ops.int8_mul_mat(w, ws, x)))
+    for f, (a, b) in zip(fs, got):
+        w, ws = codes_of(f)
+        check_product(a, *codes_of(x), w, ws, None, torch.float32)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_threads(ops):
+    """Two captured graphs replayed on two streams at once, and eager calls beside them, give what one call alone gives."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    cases = []
+    for m, n, k in ((1, 2048, 2048), (40, 1024, 4096), (300, 512, 1024)):
+        w, ws = weights(n, k, gen)
+        x = torch.randn(m, k, device="cuda", generator=gen).to(torch.bfloat16)
+        cases.append((w, ws, x, ops.int8_mul_mat(w, ws, x)))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+            outs = [ops.int8_mul_mat(w, ws, x) for w, ws, x, _ in cases]
+        graphs.append((g, side, outs))
+    for _ in range(5):
+        for g, side, outs in graphs:
+            for o in outs:
+                o.fill_(-1)
+        torch.cuda.synchronize()
+        for g, side, _ in graphs:
+            with torch.cuda.stream(side):
+                g.replay()
+        eager = [ops.int8_mul_mat(w, ws, x) for w, ws, x, _ in cases]
+        torch.cuda.synchronize()
+        for got in [outs for _, _, outs in graphs] + [eager]:
+            assert all(torch.equal(a, want) for a, (_, _, _, want) in zip(got, cases))
+
+
+# ---- experts -------------------------------------------------------------------------------------------------
+
+
+def moe_want(x, w13, s13, w2, s2, weights_, ids, act):
+    """(result, tolerance before the last rounding) in float64.  fp32 rounds a hidden value h = act(gate) * up by at most 2^-19 of itself
+    (gate and up: 5 * 2^-24 each; the activation's condition number is below 1 + |gate| with |gate| < 100 only where h counts, 2^-19
+    covers |gate| < 30): a code within 127 * 2^-18 of a half may go either way, one step of the row's scale times its weight."""
+    q, qs = codes_of(x)
+    out, room = torch.zeros(x.shape, dtype=torch.float64, device=x.device), torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    half = w13.shape[1] // 2
+    for e in range(w13.shape[0]):
+        for j in range(ids.shape[1]):
+            t = (ids[:, j] == e).nonzero().squeeze(1)
+            if t.numel() == 0:
+                continue
+            both = (q[t] @ w13[e].double().T) * qs[t][:, None] * s13[e].double()
+            gate, up = both[:, :half], both[:, half:]
+            h = (gate * torch.sigmoid(gate) if act == "silu" else gate * torch.special.ndtr(gate)) * up
+            assert float(gate.abs().max()) < 30
+            a = h.abs().amax(1, keepdim=True)
+            unit = h * 127 / torch.where(a > 0, a, 1.0)
+            code = torch.round(unit)
+            close = ((unit - torch.floor(unit) - 0.5).abs() < 127 * 2.0 ** -18).double()
+            f = (a / 127) * s2[e].double() * weights_[t, j].double()[:, None]
+            part = (code @ w2[e].double().T) * f
+            out[t] += part
+            room[t] += (close @ w2[e].double().abs().T) * f.abs() + 2.0 ** -18 * part.abs()
+    return out, room
+
+
+def experts(e, h, i, gen):
+    w13, s13 = weights(e * 2 * i, h, gen)
+    w2, s2 = weights(e * h, i, gen)
+    return w13.unflatten(0, (e, 2 * i)), s13.view(e, 2 * i), w2.unflatten(0, (e, h)), s2.view(e, h)
+
+
+MOE = [(1, 4, 2, 64, 32), (1, 64, 8, 256, 128), (3, 8, 1, 136, 264), (8, 64, 8, 512, 256), (33, 16, 4, 264, 392), (100, 8, 2, 384, 128), (257, 8, 8, 512, 384),
+       (64, 256, 8, 128, 64), (600, 4, 3, 256, 136), (1500, 16, 4, 128, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,i", MOE)
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "silu"), (torch.float16, "gelu"), (torch.float32, "silu")])
+def test_moe(ops, t, e, k, h, i, dtype, act):
+    gen = torch.Generator(device="cuda").manual_seed(t + e + h)
+    w13, s13, w2, s2 = experts(e, h, i, gen)
+    x = torch.randn(t, h, device="cuda", generator=gen).to(dtype)
+    weights_, ids = torch.randn(t, e, device="cuda", generator=gen).softmax(-1).topk(k, dim=-1)
+    ids = ids.to(torch.int32)
+    ids[::5, 0] = -1          # (skipped)
+    if t > 4:
+        ids[3] = e            # a token without any expert
+    y = ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, act)
+    want, room = moe_want(x, w13, s13, w2, s2, weights_, ids, act)
+    room = room + torch.finfo(dtype).eps / 2 * (want.abs() + room) + TINY[dtype] + 2.0 ** -22 * want.abs()
+    assert y.dtype == dtype and bool(((y.double() - want).abs() <= room).all())
+    if t > 4:
+        assert not bool(y[3].any())
+    assert torch.equal(ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, act), y)
+
+
+@pytest.mark.gpu
+def test_moe_all_tokens_to_one_expert_and_the_same_one_twice(ops):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w13, s13, w2, s2 = experts(16, 128, 72, gen)
+    x = torch.randn(700, 128, device="cuda", generator=gen)
+    weights_ = torch.rand(700, 2, device="cuda", generator=gen)
+    ids = torch.full((700, 2), 15, dtype=torch.int32, device="cuda")
+    y = ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, "silu")
+    want, room = moe_want(x, w13, s13, w2, s2, weights_, ids, "silu")
+    assert bool(((y.double() - want).abs() <= room + 2.0 ** -22 * want.abs() + 1e-30).all())
+    ids.fill_(-1)
+    assert not bool(ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, "silu").any())
+    assert ops.int8_fused_moe(x[:0], w13, s13, w2, s2, weights_[:0], ids[:0], "silu").shape == (0, 128)
+
+
+@pytest.mark.gpu
+def test_moe_in_a_graph_with_the_router(ops):
+    """Route and experts captured together; replayed on new logits and activations, padded rows among them."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    w13, s13, w2, s2 = experts(32, 256, 128, gen)
+    x = torch.randn(48, 256, device="cuda", generator=gen).to(torch.bfloat16)
+    logits = torch.randn(48, 32, device="cuda", generator=gen)
+    bias = torch.randn(32, device="cuda", generator=gen) * 0.1
+
+    def step():
+        weights_, ids = ops.moe_route(logits, 4, scoring="sigmoid", bias=bias, n_group=4, topk_group=2, scale=2.0)
+        return ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, "silu"), weights_, ids
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(3):
+        x.copy_(torch.randn(48, 256, device="cuda", generator=gen))
+        logits.copy_(torch.randn(48, 32, device="cuda", generator=gen))
+        logits[40 + i:] = float("-inf")
+        g.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+        assert bool((out[2][40 + i:] == -1).all()) and not bool(out[0][40 + i:].any())
+        want, room = moe_want(x, w13, s13, w2, s2, out[1], out[2], "silu")
+        room = room + 2.0 ** -9 * (want.abs() + room) + 2.0 ** -22 * want.abs() + 1e-30   # (bf16: half of 2^-8)
+        assert bool(((out[0].double() - want).abs() <= 2 * room).all())
+
+
+# ---- refusals ------------------------------------------------------------------------------------------------
+
+
+def test_c_abi_refuses_before_any_launch(native_libs):
+    from gguf_b200 import capi
+
+    lib = capi.lib()
+    p, odd, null = ctypes.c_void_p(4096), ctypes.c_void_p(4104), None
+    q = lib.gguf_b200_int8_quantize
+    assert q(p, 7, 64, p, 64, p, 1, 64, null) == -2
+    assert q(p, 1, 64, p, 64, p, -1, 64, null) == -3 and q(p, 1, 64, p, 64, p, 1, 0, null) == -3
+    assert q(null, 1, 64, p, 64, p, 1, 64, null) == -4 and q(p, 1, 64, odd, 64, p, 1, 64, null) == -4
+    assert q(p, 1, 64, p, 48, p, 1, 64, null) == -4 and q(p, 1, 64, p, 72, p, 1, 64, null) == -4 and q(p, 1, 64, p, 64, null, 1, 64, null) == -4
+    assert q(null, 1, 64, null, 64, null, 0, 64, null) == 0
+    m = lib.gguf_b200_int8_mul_mat
+    assert lib.gguf_b200_int8_scratch_bytes(3, 100) == 512 + 256 and lib.gguf_b200_int8_scratch_bytes(0, 100) == 0
+    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 9, 1, 8, 64, null) == -2
+    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 0, null) == -3
+    assert m(p, 131072, p, p, 131072, null, p, p, 1 << 20, 1, 1, 8, 131072, null) == -7
+    assert m(odd, 64, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4 and m(p, 72, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4
+    assert m(p, 64, null, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4 and m(p, 64, p, p, 64, null, p, null, 0, 1, 1, 8, 64, null) == -4
+    assert m(p, 64, p, p, 64, null, p, p, 16, 1, 1, 8, 64, null) == -5
+    assert m(p, 64, p, p, 64, null, p, p, 0, 1, 0, 8, 64, null) == 0
+    pr = lib.gguf_b200_int8_mul_mat_prepared
+    assert pr(p, 64, p, odd, 64, p, null, p, 0, 1, 1, 8, 64, null) == -4 and pr(p, 64, p, p, 64, null, null, p, 0, 1, 1, 8, 64, null) == -4
+    moe = lib.gguf_b200_int8_fused_moe
+    room = lib.gguf_b200_int8_moe_workspace_bytes(4, 2, 8, 64, 64)
+    assert room > 0 and lib.gguf_b200_int8_moe_workspace_bytes(4, 2, 257, 64, 64) == 0
+
+    def call(w13=p, ld13=64, act=1, dtype=1, top_k=2, e=8, h=64, i=64, ws=room, ids=p, y=p):
+        return moe(p, 64, w13, ld13, p, p, 64, p, y, ids, p, p, ws, dtype, act, 4, top_k, e, h, i, null)
+
+    assert call(act=3) == -3 and call(h=60) == -3 and call(i=36) == -3 and call(top_k=0) == -3 and call(e=0) == -3
+    assert call(dtype=5) == -2 and call(e=257) == -7 and call(w13=odd) == -4 and call(ld13=72) == -4 and call(ids=null) == -4 and call(y=odd) == -4
+    assert call(ws=room - 1) == -5
+
+
+def test_shapes_under_tracing(ops):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        dev = "cuda" if torch.cuda.is_available() else "meta"
+        x = torch.empty(5, 100, device=dev, dtype=torch.bfloat16)
+        q, s = torch.ops._C_gguf.int8_quantize(x)
+        assert q.shape == (5, 100) and q.stride() == (112, 1) and q.dtype == torch.int8 and s.shape == (5,) and s.dtype == torch.float32
+        w = torch.empty(7, 100, device=dev, dtype=torch.int8)
+        assert torch.ops._C_gguf.int8_mul_mat(w, s, x, None).shape == (5, 7)
+        y = torch.ops._C_gguf.int8_mul_mat_prepared(w, s, q, s, None, torch.float16)
+        assert y.shape == (5, 7) and y.dtype == torch.float16
+        assert torch.ops._C_gguf.int8_fused_moe(x, w, s, w, s, s, s, 1).shape == x.shape
+        a, b = torch.ops._C_gguf.moe_route(x, None, 4, 1, 1, 1, True, 1.0)
+        assert a.shape == b.shape == (5, 4) and a.dtype == torch.float32 and b.dtype == torch.int32
+
+
+@pytest.mark.gpu
+def test_refuses_what_it_cannot_take(ops):
+    w, ws = torch.zeros(32, 64, dtype=torch.int8, device="cuda"), torch.ones(32, device="cuda")
+    x = torch.zeros(3, 64, device="cuda")
+    for args in ((w.to(torch.uint8), ws, x), (w, ws[:-1], x), (w, ws.double(), x), (w, ws, x[:, :48]), (w, ws, x.double()), (w, ws, x[0]), (w[0], ws, x),
+                 (w, ws.cpu(), x), (w.cpu(), ws, x), (w, ws, x, torch.ones(31, device="cuda")), (w, ws, x, torch.ones(32, device="cuda", dtype=torch.float16)),
+                 (w, ws, x.T.contiguous().T)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.int8_mul_mat(*args)
+    with pytest.raises(RuntimeError):
+        ops.int8_quantize(torch.zeros(3, 4, 5, device="cuda"))
+    with pytest.raises(RuntimeError):
+        ops.int8_quantize(torch.zeros(3, 4, device="cuda", dtype=torch.int32))
+    with pytest.raises(KeyError):
+        ops.int8_fused_moe(x, w[None], ws[None], w[None], ws[None], ws, ws, "relu")

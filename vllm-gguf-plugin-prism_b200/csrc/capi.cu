@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "int8.cuh"
 #include "kernels.h"
 #include "raw_stream.cuh"
 
@@ -722,7 +723,7 @@ int gguf_b200_fused_moe(const void* X, const void* W13, const void* W2, void* Y,
     if (rc) return rc;
     rc = gemm(base + L.o_y1, 1, act, W2, type2, H, I, base + L.o_y2, topk_weights);
     if (rc) return rc;
-    return launch_moe_sum(base + L.o_y2, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+    return launch_moe_sum(base + L.o_y2, false, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
   }
   const FusedMoeLayout L = fused_moe_layout(type13, type2, dtype, tokens, top_k, n_experts, H, I);
   if (ws_bytes < L.total) return E_WORKSPACE;
@@ -773,7 +774,7 @@ int gguf_b200_fused_moe(const void* X, const void* W13, const void* W2, void* Y,
   rc = gemm(base + L.o_y1, 1, W2, type2, H, I, base + L.o_y2, topk_weights, act, 2 * I);
   if (rc) return rc;
   // 4. sum over the top_k slots of every token
-  return launch_moe_sum(base + L.o_y2, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+  return launch_moe_sum(base + L.o_y2, false, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
 }
 
 int gguf_b200_moe_a8_vec(const void* X, const void* W, void* Y, void* ws, int64_t ws_bytes, const int32_t* topk_ids,
@@ -790,6 +791,168 @@ int gguf_b200_moe_a8_vec(const void* X, const void* W, void* Y, void* ws, int64_
   rc = launch_quantize_q8_1(X, dtype, ws, tokens, K, Q8_MODE_SOA, gemv_sum_mode(type), 0, CORR_NONE, nullptr, 1, 0, s);
   if (rc) return rc;
   return launch_moe_gemv(W, ws, Y, topk_ids, type, dtype, tokens, top_k, N, K, n_experts, st, s);
+}
+
+// ---- 8-bit integer products, router ----
+
+namespace {
+int64_t i8_ld(int64_t k) { return round_up(k, 16); }
+// rows of a matrix of 8-bit integers: where the tensor core's copies can start
+bool i8_rows_ok(const void* p, int64_t ld, int64_t k) { return p && aligned16(p) && ld >= k && ld % 16 == 0; }
+int i8_check(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (!dtype_ok(dtype)) return E_BAD_DTYPE;
+  if (M < 0 || N < 0 || K <= 0) return E_BAD_SHAPE;
+  if (K > I8_MAX_K || N >= (int64_t)1 << 30 || M >= (int64_t)1 << 30) return E_TOO_LARGE;
+  return E_OK;
+}
+struct I8MoeLayout {
+  int64_t pass_rows, passes, o_sorted, o_passes, o_npass, o_q1, o_s1, o_q2, o_s2, o_h, total;
+};
+I8MoeLayout i8_moe_layout(int64_t tokens, int64_t top_k, int64_t E, int64_t H, int64_t I) {
+  I8MoeLayout L{};
+  const int64_t slots = tokens * top_k;
+  L.pass_rows = i8_moe_pass_rows(slots, E);
+  L.passes = moe_plan_passes(slots, (int)E, (int)L.pass_rows);
+  int64_t o = 0;
+  auto take = [&](int64_t bytes) { const int64_t at = o; o += round_up(bytes, 256); return at; };
+  L.o_sorted = take(slots * 4);
+  L.o_passes = take(L.passes * 16);
+  L.o_npass = take(8);
+  L.o_q1 = take(slots * i8_ld(H));
+  L.o_s1 = take(slots * 4);
+  L.o_q2 = take(slots * i8_ld(I));
+  L.o_s2 = take(slots * 4);
+  L.o_h = take(slots * (I > H ? I : H) * 4);   // hidden rows, then -- when they are quantized -- the experts' results
+  L.total = o;
+  return L;
+}
+}  // namespace
+
+int gguf_b200_int8_quantize(const void* X, int dtype, int64_t ldx, void* Q, int64_t ldq, float* scales, int64_t M, int64_t K, void* stream) {
+  if (!dtype_ok(dtype)) return E_BAD_DTYPE;
+  if (M < 0 || K <= 0 || ldx < 0) return E_BAD_SHAPE;
+  if (M >= (int64_t)1 << 31 || K >= (int64_t)1 << 31) return E_TOO_LARGE;
+  if (M == 0) return E_OK;
+  if (!X || !scales || !i8_rows_ok(Q, ldq, K)) return E_BAD_POINTER;
+  I8Quantize a{};
+  a.x = X; a.dtype = dtype; a.ldx = ldx;
+  a.q = static_cast<int8_t*>(Q); a.ldq = ldq; a.scale = scales;
+  a.rows = M; a.k = K;
+  return launch_i8_quantize(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t gguf_b200_int8_scratch_bytes(int64_t M, int64_t K) { return M <= 0 || K <= 0 ? 0 : round_up(M * i8_ld(K), 256) + round_up(M * 4, 256); }
+
+int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_scales, const void* Q, int64_t ldq, const float* q_scales, const void* bias,
+                                    void* Y, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  const int rc = i8_check(dtype, M, N, K);
+  if (rc || M == 0 || N == 0) return rc;
+  if (!i8_rows_ok(W, ldw, K) || !i8_rows_ok(Q, ldq, K) || !w_scales || !q_scales || !Y) return E_BAD_POINTER;
+  int* st = status_ptr();
+  if (!st) return E_CUDA;
+  I8Product a{};
+  a.w = static_cast<const int8_t*>(W); a.ldw = ldw; a.w_scale = w_scales;
+  a.q = static_cast<const int8_t*>(Q); a.ldq = ldq; a.q_scale = q_scales;
+  a.y = Y; a.ldy = N; a.dtype = dtype; a.bias = bias;
+  a.m = M; a.n = N; a.k = K;
+  a.settled = !(flags & GGUF_B200_W_IN_FLIGHT);
+  a.experts = 1;
+  a.status = st;
+  return launch_i8_product(a, static_cast<cudaStream_t>(stream));
+}
+
+int gguf_b200_int8_mul_mat(const void* W, int64_t ldw, const float* w_scales, const void* X, int64_t ldx, const void* bias, void* Y, void* ws,
+                           int64_t ws_bytes, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  int rc = i8_check(dtype, M, N, K);
+  if (rc || M == 0 || N == 0) return rc;
+  if (!X || !i8_rows_ok(W, ldw, K) || !w_scales || !Y || !ws || !aligned16(ws)) return E_BAD_POINTER;
+  if (ws_bytes < gguf_b200_int8_scratch_bytes(M, K)) return E_WORKSPACE;
+  float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(M * i8_ld(K), 256));
+  rc = gguf_b200_int8_quantize(X, dtype, ldx, ws, i8_ld(K), scales, M, K, stream);
+  // (the quantizer releases the product behind its own wait: whatever wrote W ahead of this call is complete by then)
+  return rc ? rc : gguf_b200_int8_mul_mat_prepared(W, ldw, w_scales, ws, i8_ld(K), scales, bias, Y, 0, dtype, M, N, K, stream);
+}
+
+int64_t gguf_b200_int8_moe_workspace_bytes(int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H, int64_t I) {
+  if (tokens <= 0 || top_k <= 0 || n_experts <= 0 || n_experts > 256 || H <= 0 || I <= 0) return 0;
+  return i8_moe_layout(tokens, top_k, n_experts, H, I).total;
+}
+
+int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_t ld13, const float* w13_scales, const void* W2, int64_t ld2,
+                             const float* w2_scales, void* Y, const int32_t* topk_ids, const float* topk_weights, void* ws, int64_t ws_bytes, int dtype,
+                             int act, int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H, int64_t I, void* stream) {
+  if (top_k <= 0 || n_experts <= 0 || I <= 0 || H <= 0 || H % 8 != 0 || I % 8 != 0 || (act != 1 && act != 2)) return E_BAD_SHAPE;
+  if (n_experts > 256 || top_k > 256 || H > I8_MAX_K || I > I8_MAX_K || tokens > 1 << 24 || tokens * top_k > 1 << 24) return E_TOO_LARGE;
+  int rc = i8_check(dtype, tokens, n_experts * 2 * I, H);
+  if (!rc) rc = i8_check(dtype, tokens, n_experts * H, I);
+  if (rc || tokens == 0) return rc;
+  if (!X || !Y || !aligned16(Y) || !i8_rows_ok(W13, ld13, H) || !i8_rows_ok(W2, ld2, I) || !w13_scales || !w2_scales || !topk_ids || !topk_weights || !ws ||
+      !aligned16(ws))
+    return E_BAD_POINTER;
+  const I8MoeLayout L = i8_moe_layout(tokens, top_k, n_experts, H, I);
+  if (ws_bytes < L.total) return E_WORKSPACE;
+  int* st = status_ptr();
+  if (!st) return E_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  const int64_t slots = tokens * top_k;
+  int32_t* sorted = reinterpret_cast<int32_t*>(base + L.o_sorted);
+  int32_t* npass = reinterpret_cast<int32_t*>(base + L.o_npass);
+  // 1. expert-sorted slots and the passes over them; slots without a valid expert are in none, and the sum skips them
+  rc = launch_moe_plan(topk_ids, slots, (int)n_experts, 1, (int)L.pass_rows, sorted, base + L.o_passes, npass, s);
+  if (rc) return rc;
+  // 2. every slot's token, quantized, in the order of the experts
+  I8Quantize q{};
+  q.x = X; q.dtype = dtype; q.ldx = ldx;
+  q.q = reinterpret_cast<int8_t*>(base + L.o_q1); q.ldq = i8_ld(H); q.scale = reinterpret_cast<float*>(base + L.o_s1);
+  q.rows = slots; q.k = H;
+  q.gather = sorted; q.gather_div = top_k; q.n_used = npass + 1;
+  rc = launch_i8_quantize(q, s);
+  if (rc) return rc;
+  // 3. gate and up products and the activation: hidden rows in fp32 (their largest value decides about all codes of a row)
+  I8Product a{};
+  a.w = static_cast<const int8_t*>(W13); a.ldw = ld13; a.w_scale = w13_scales;
+  a.q = q.q; a.ldq = q.ldq; a.q_scale = q.scale;
+  a.y = base + L.o_h; a.ldy = I; a.dtype = DT_F32;
+  a.m = slots; a.n = I; a.k = H;
+  a.passes = base + L.o_passes; a.n_passes = npass;
+  a.experts = n_experts; a.max_passes = L.passes; a.pass_rows = L.pass_rows;
+  a.act = act;
+  a.status = st;
+  rc = launch_i8_product(a, s);
+  if (rc) return rc;
+  // 4. the hidden rows, quantized
+  I8Quantize q2{};
+  q2.x = base + L.o_h; q2.dtype = DT_F32; q2.ldx = I;
+  q2.q = reinterpret_cast<int8_t*>(base + L.o_q2); q2.ldq = i8_ld(I); q2.scale = reinterpret_cast<float*>(base + L.o_s2);
+  q2.rows = slots; q2.k = I;
+  q2.n_used = npass + 1;
+  rc = launch_i8_quantize(q2, s);
+  if (rc) return rc;
+  // 5. down products, weighted, back in the order of the slots; in fp32, so that the sum is rounded once
+  a.w = static_cast<const int8_t*>(W2); a.ldw = ld2; a.w_scale = w2_scales;
+  a.q = q2.q; a.ldq = q2.ldq; a.q_scale = q2.scale;
+  a.ldy = H;
+  a.n = H; a.k = I;
+  a.act = 0;
+  a.sorted = sorted;
+  a.row_scale = topk_weights;
+  rc = launch_i8_product(a, s);
+  if (rc) return rc;
+  // 6. sum over the top_k slots of every token
+  return launch_moe_sum(base + L.o_h, true, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+}
+
+int gguf_b200_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, float* weights, int32_t* ids, int64_t tokens, int64_t n_experts,
+                        int64_t top_k, int64_t n_group, int64_t topk_group, int scoring, int renormalize, float scale, void* stream) {
+  if (!dtype_ok(dtype)) return E_BAD_DTYPE;
+  if (tokens < 0 || ld < 0 || n_experts <= 0 || top_k <= 0 || n_group <= 0 || topk_group <= 0 || (scoring != 1 && scoring != 2)) return E_BAD_SHAPE;
+  if (n_experts > ROUTE_MAX_EXPERTS || top_k > ROUTE_MAX_TOP_K || n_group > 32 || tokens >= (int64_t)1 << 31) return E_TOO_LARGE;
+  if (n_experts % n_group != 0 || topk_group > n_group || top_k > topk_group * (n_experts / n_group)) return E_BAD_SHAPE;
+  if (tokens == 0) return E_OK;
+  if (!logits || !weights || !ids) return E_BAD_POINTER;
+  return launch_moe_route(logits, dtype, ld, bias, weights, ids, tokens, (int)n_experts, (int)top_k, (int)n_group, (int)topk_group, scoring == 2, renormalize,
+                          scale, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

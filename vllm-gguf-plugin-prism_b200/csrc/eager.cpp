@@ -170,7 +170,87 @@ PyObject* py_moe(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* wrap_pair(const std::tuple<Tensor, Tensor>& t) {
+  PyObject* a = THPVariable_Wrap(std::get<0>(t));
+  PyObject* b = a ? THPVariable_Wrap(std::get<1>(t)) : nullptr;
+  PyObject* out = b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return out;
+}
+// The tensors among arguments [0, n), the optional ones among them None or a tensor; false: not an eager call
+template <size_t N> bool plain_args(PyObject* const* a, const bool (&optional)[N], std::optional<Tensor> (&t)[N]) {
+  for (size_t i = 0; i < N; ++i) {
+    if (optional[i] && a[i] == Py_None) continue;
+    const Tensor* p = plain_cuda(a[i]);
+    if (!p) return false;
+    t[i] = *p;
+  }
+  return modes_off();
+}
+
+// moe_route(logits, bias or None, top_k, n_group, topk_group, scoring, renormalize, scale)
+PyObject* py_moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "moe_route takes 8 arguments");
+  std::optional<Tensor> t[2];
+  if (!plain_args(a, {false, true}, t)) Py_RETURN_NONE;
+  int64_t v[4];
+  for (int i = 0; i < 4; ++i) v[i] = PyLong_AsLongLong(a[2 + i]);
+  const int renormalize = PyObject_IsTrue(a[6]);
+  const double scale = PyFloat_AsDouble(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  std::tuple<Tensor, Tensor> out;
+  {
+    const NoGil release;
+    out = Op::moe_route(*t[0], t[1], v[0], v[1], v[2], v[3], renormalize != 0, scale);
+  }
+  return wrap_pair(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_quantize(X)
+PyObject* py_int8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 1, "int8_quantize takes 1 argument");
+  std::optional<Tensor> t[1];
+  if (!plain_args(a, {false}, t)) Py_RETURN_NONE;
+  std::tuple<Tensor, Tensor> out;
+  {
+    const NoGil release;
+    out = Op::int8_quantize(*t[0]);
+  }
+  return wrap_pair(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_mul_mat(W, w_scales, X, bias or None)
+PyObject* py_int8_mul_mat(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 4, "int8_mul_mat takes 4 arguments");
+  std::optional<Tensor> t[4];
+  if (!plain_args(a, {false, false, false, true}, t)) Py_RETURN_NONE;
+  return THPVariable_Wrap(without_gil([&] { return Op::int8_mul_mat(*t[0], *t[1], *t[2], t[3]); }));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_moe(X, W13, w13_scales, W2, w2_scales, topk_weights, topk_ids, act)
+PyObject* py_int8_moe(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "int8_moe takes 8 arguments");
+  std::optional<Tensor> t[7];
+  if (!plain_args(a, {false, false, false, false, false, false, false}, t)) Py_RETURN_NONE;
+  const long act = PyLong_AsLong(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  return THPVariable_Wrap(without_gil([&] { return Op::int8_fused_moe(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], *t[6], act); }));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"moe_route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_moe_route)), METH_FASTCALL, nullptr},
+    {"int8_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_int8_quantize)), METH_FASTCALL, nullptr},
+    {"int8_mul_mat", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_int8_mul_mat)), METH_FASTCALL, nullptr},
+    {"int8_moe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_int8_moe)), METH_FASTCALL, nullptr},
     {"moe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_moe)), METH_FASTCALL, nullptr},
     {"mul_mat", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_mul_mat)), METH_FASTCALL, nullptr},
     {"embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_embed)), METH_FASTCALL, nullptr},

@@ -1,0 +1,150 @@
+// Rows of floats to 8-bit integers with one scale a row:  a = max |x|,  scale = a / 127,  code = x * 127 / a, halves to even.
+// The same kernel serves a token's activations, an expert's hidden rows and, once, a weight matrix.
+//
+// The codes are those of exact arithmetic.  x * (127 / a) in fp32 is off by less than 127 * 2^-22; within 2^-14 of a half the
+// side is settled by the sign of 254 |x| - (2 m + 1) a in fp64, where both products are exact (24 + 8 bits).  16-bit inputs hit
+// halves all the time (x = a / 2 is code 63.5).  A row with an infinity or a NaN has no scale: it gets NaN for one and codes of 0,
+// so that every result it enters is NaN.
+//
+// Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once.
+#include "common.cuh"
+#include "int8.cuh"
+
+namespace gguf_b200 {
+
+constexpr int I8Q_UNIT = 16;   // values a thread handles at a time: one 16-byte store of codes
+constexpr int I8Q_HOLD = 4;    // units it keeps in registers between the maximum and the codes; what is beyond is read again
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void i8q_load(const T* __restrict__ x, int64_t k, int64_t at, T (&v)[I8Q_UNIT]) {
+  if (VEC && at + I8Q_UNIT <= k) {
+#pragma unroll
+    for (int i = 0; i < I8Q_UNIT * (int)sizeof(T) / 16; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(x + at) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < I8Q_UNIT; ++i) v[i] = at + i < k ? x[at + i] : from_float<T>(0.f);
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t i8q_top(const T (&v)[I8Q_UNIT], uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < I8Q_UNIT; ++i) top = max(top, __float_as_uint(to_float<T>(v[i])) & 0x7fffffffu);   // (of bit patterns: infinity and NaN above all numbers)
+  return top;
+}
+__device__ __forceinline__ int i8q_code(float x, float inv, float a) {
+  const float t = x * inv, r = rintf(t);
+  int c = (int)r;
+  if (fabsf(t - r) > 0.5f - 0x1p-14f) {
+    const int m = (int)fabsf(t);
+    const double d = 254.0 * (double)fabsf(x) - (double)(2 * m + 1) * (double)a;
+    const int u = m + (d > 0.0 || (d == 0.0 && (m & 1)));
+    c = x < 0.f ? -u : u;
+  }
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ void i8q_store(const T (&v)[I8Q_UNIT], float lift, float inv, float a, int8_t* __restrict__ q, int64_t k, int64_t at) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)i8q_code(to_float<T>(v[4 * i + j]) * lift, inv, a) & 0xffu) << (8 * j);
+  }
+  if (at + I8Q_UNIT <= k) {
+    *reinterpret_cast<uint4*>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < I8Q_UNIT; ++i)
+      if (at + i < k) q[at + i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+// LANES threads a row, 256 / LANES rows a block
+template <typename T, bool VEC, int LANES>
+__global__ void __launch_bounds__(256) i8_quantize_kernel(const I8Quantize p) {
+  __shared__ uint32_t s_top[8];
+  const int lane = threadIdx.x % LANES;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t rows = p.n_used ? *p.n_used : p.rows;
+  for (int64_t r0 = (int64_t)blockIdx.x * (256 / LANES); r0 < rows; r0 += (int64_t)gridDim.x * (256 / LANES)) {
+    const int64_t r = r0 + threadIdx.x / LANES;
+    const bool live = r < rows;
+    const int64_t from = !live ? 0 : p.gather ? p.gather[r] / p.gather_div : r;
+    const T* x = static_cast<const T*>(p.x) + from * p.ldx;
+    const int64_t k = live ? p.k : 0;
+    T v[I8Q_HOLD][I8Q_UNIT];
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < I8Q_HOLD; ++h) {
+      const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
+      if (at < k) {
+        i8q_load<T, VEC>(x, k, at, v[h]);
+        top = i8q_top<T>(v[h], top);
+      }
+    }
+    for (int64_t at = (int64_t)(I8Q_HOLD * LANES + lane) * I8Q_UNIT; at < k; at += LANES * I8Q_UNIT) {
+      T u[I8Q_UNIT];
+      i8q_load<T, VEC>(x, k, at, u);
+      top = i8q_top<T>(u, top);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (LANES > 32) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+      __syncthreads();
+      top = s_top[0];
+#pragma unroll
+      for (int i = 1; i < LANES / 32; ++i) top = max(top, s_top[i]);
+    }
+    const bool finite = top < 0x7f800000u;
+    const float a0 = __uint_as_float(top), lift = a0 < 0x1p-90f ? 0x1p64f : 1.f;   // (so that 127 / a stays finite; exact)
+    const float a = a0 * lift, inv = finite && top != 0 ? 127.f / a : 0.f;
+    if (live && lane == 0) p.scale[r] = finite ? a0 / 127.f : __uint_as_float(0x7fc00000u);
+    int8_t* q = p.q + r * p.ldq;
+    auto put = [&](const T (&u)[I8Q_UNIT], int64_t at) {
+      if (finite) {
+        i8q_store<T>(u, lift, inv, a, q, k, at);
+      } else {
+        const T zero[I8Q_UNIT] = {};
+        i8q_store<T>(zero, 1.f, 0.f, 1.f, q, k, at);
+      }
+    };
+#pragma unroll
+    for (int h = 0; h < I8Q_HOLD; ++h) {
+      const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
+      if (at < k) put(v[h], at);
+    }
+    for (int64_t at = (int64_t)(I8Q_HOLD * LANES + lane) * I8Q_UNIT; at < k; at += LANES * I8Q_UNIT) {
+      T u[I8Q_UNIT];
+      i8q_load<T, VEC>(x, k, at, u);
+      put(u, at);
+    }
+  }
+}
+
+template <typename T> static int i8_quantize_typed(const I8Quantize& a, cudaStream_t stream) {
+  const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx * (int64_t)sizeof(T) % 16 == 0;
+  const bool warp = a.k <= 32 * I8Q_UNIT * I8Q_HOLD;
+  const int per = warp ? 8 : 1;
+  const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 64;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  cudaError_t e;
+  if (vec)
+    e = warp ? launch_pdl(i8_quantize_kernel<T, true, 32>, grid, dim3(256), 0, stream, a) : launch_pdl(i8_quantize_kernel<T, true, 256>, grid, dim3(256), 0, stream, a);
+  else
+    e = warp ? launch_pdl(i8_quantize_kernel<T, false, 32>, grid, dim3(256), 0, stream, a) : launch_pdl(i8_quantize_kernel<T, false, 256>, grid, dim3(256), 0, stream, a);
+  return e == cudaSuccess ? E_OK : E_CUDA;
+}
+
+int launch_i8_quantize(const I8Quantize& a, cudaStream_t stream) {
+  if (a.rows == 0) return E_OK;
+  switch (a.dtype) {
+    case DT_F32: return i8_quantize_typed<float>(a, stream);
+    case DT_F16: return i8_quantize_typed<__half>(a, stream);
+    case DT_BF16: return i8_quantize_typed<__nv_bfloat16>(a, stream);
+  }
+  return E_BAD_DTYPE;
+}
+
+}  // namespace gguf_b200

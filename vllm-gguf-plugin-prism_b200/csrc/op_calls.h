@@ -9,6 +9,7 @@
 
 #include <optional>
 #include <string>
+#include <tuple>
 
 #include <torch/headeronly/core/ScalarType.h>
 #include <torch/headeronly/util/Exception.h>
@@ -261,6 +262,129 @@ template <class A> struct Calls {
                                  tokens, top_k, E, H, I, A::stream(X)),
              "fused_moe");
     return Y;
+  }
+
+  // ---- 8-bit integer products, router ----
+
+  static void same_device(const Tensor& like, const Tensor& t, const char* op, const char* what) {
+    STD_TORCH_CHECK(A::device(t) == A::device(like), op, ": ", what, " is on another device");
+  }
+  // Elements between the rows of a matrix whose values lie side by side.  (Of one row, any number will do.)
+  static int64_t row_distance(const Tensor& t, const char* op, const char* what) {
+    STD_TORCH_CHECK(t.dim() == 2 && t.size(1) > 0 && (t.size(1) == 1 || t.stride(1) == 1), op, ": ", what, " must be [rows, values] with the values of a row side by side");
+    return t.size(0) > 1 ? t.stride(0) : t.size(1);
+  }
+  // The same of 8-bit integer weights or codes, all matrices of a stack counted as one.
+  static int64_t int8_rows(const Tensor& t, int64_t dim, const char* op, const char* what) {
+    STD_TORCH_CHECK(t.scalar_type() == ScalarType::Char && t.dim() == dim, op, ": ", what, " must be an int8 tensor of ", std::to_string(dim), " dimensions");
+    const int64_t rows = t.size(dim - 2), k = t.size(dim - 1), least = (k + 15) / 16 * 16;
+    STD_TORCH_CHECK(k > 0 && (k == 1 || t.stride(dim - 1) == 1), op, ": the values of a row of ", what, " must lie side by side");
+    int64_t ld = rows > 1 ? t.stride(dim - 2) : dim == 3 && t.size(0) > 1 ? t.stride(0) : least;
+    STD_TORCH_CHECK(dim == 2 || t.size(0) <= 1 || t.stride(0) == rows * ld, op, ": the matrices of ", what, " must follow one another");
+    STD_TORCH_CHECK(t.numel() == 0 || (ld >= k && ld % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0), op, ": the rows of ", what,
+                    " must start at multiples of 16 bytes (int8_quantize lays them out so)");
+    return ld;
+  }
+  static const float* scales_of(const Tensor& s, const Tensor& like, int64_t n, const char* op, const char* what) {
+    same_device(like, s, op, what);
+    STD_TORCH_CHECK(s.scalar_type() == ScalarType::Float && s.is_contiguous() && s.numel() == n, op, ": ", what, " must be contiguous float32, one for every row");
+    return static_cast<const float*>(s.data_ptr());
+  }
+  static const void* bias_of(const std::optional<Tensor>& b, const Tensor& like, int64_t n, ScalarType dt, const char* op) {
+    if (!b) return nullptr;
+    same_device(like, *b, op, "bias");
+    STD_TORCH_CHECK(b->scalar_type() == dt && b->is_contiguous() && b->dim() == 1 && b->numel() == n, op, ": bias must be contiguous, one value per weight row, in the dtype of the result");
+    return b->data_ptr();
+  }
+
+  static std::tuple<Tensor, Tensor> int8_quantize(const Tensor& X) {
+    const char* op = "int8_quantize";
+    const typename A::Guard guard(A::device(X));
+    const int code = dtype_code(X.scalar_type(), op);
+    const int64_t ldx = row_distance(X, op, "X"), M = X.size(0), K = X.size(1), ldq = (K + 15) / 16 * 16;
+    Tensor q = A::empty(X, {M, ldq}, ScalarType::Char), s = A::empty(X, {M}, ScalarType::Float);
+    check_rc(gguf_b200_int8_quantize(X.data_ptr(), code, ldx, q.data_ptr(), ldq, static_cast<float*>(s.data_ptr()), M, K, A::stream(X)), op);
+    return {ldq == K ? q : A::block(q, 0, M, 0, K), s};
+  }
+
+  static Tensor int8_mul_mat(const Tensor& W, const Tensor& w_scales, const Tensor& X, const std::optional<Tensor>& bias) {
+    const char* op = "int8_mul_mat";
+    const typename A::Guard guard(A::device(X));
+    const ScalarType dt = X.scalar_type();
+    const int code = dtype_code(dt, op);
+    same_device(X, W, op, "W");
+    const int64_t ldw = int8_rows(W, 2, op, "W"), ldx = row_distance(X, op, "X"), M = X.size(0), N = W.size(0), K = W.size(1);
+    STD_TORCH_CHECK(X.size(1) == K, op, ": X and W have rows of different lengths");
+    const float* ws = scales_of(w_scales, X, N, op, "w_scales");
+    const void* b = bias_of(bias, X, N, dt, op);
+    Tensor Y = A::empty(X, {M, N}, dt);
+    if (M == 0 || N == 0) return Y;
+    const int64_t bytes = gguf_b200_int8_scratch_bytes(M, K);
+    const typename A::Scratch scratch(X, bytes);
+    check_rc(gguf_b200_int8_mul_mat(W.data_ptr(), ldw, ws, X.data_ptr(), ldx, b, Y.data_ptr(), scratch.get(), bytes, code, M, N, K, A::stream(X)), op);
+    return Y;
+  }
+
+  // (the weights may come straight out of int8_quantize)
+  static Tensor int8_mul_mat_prepared(const Tensor& W, const Tensor& w_scales, const Tensor& Q, const Tensor& q_scales, const std::optional<Tensor>& bias,
+                                      ScalarType dt) {
+    const char* op = "int8_mul_mat_prepared";
+    const typename A::Guard guard(A::device(Q));
+    const int code = dtype_code(dt, op);
+    same_device(Q, W, op, "W");
+    const int64_t ldw = int8_rows(W, 2, op, "W"), ldq = int8_rows(Q, 2, op, "Q"), M = Q.size(0), N = W.size(0), K = W.size(1);
+    STD_TORCH_CHECK(Q.size(1) == K, op, ": Q and W have rows of different lengths");
+    const float *ws = scales_of(w_scales, Q, N, op, "w_scales"), *qs = scales_of(q_scales, Q, M, op, "q_scales");
+    const void* b = bias_of(bias, Q, N, dt, op);
+    Tensor Y = A::empty(Q, {M, N}, dt);
+    if (M == 0 || N == 0) return Y;
+    check_rc(gguf_b200_int8_mul_mat_prepared(W.data_ptr(), ldw, ws, Q.data_ptr(), ldq, qs, b, Y.data_ptr(), GGUF_B200_W_IN_FLIGHT, code, M, N, K, A::stream(Q)), op);
+    return Y;
+  }
+
+  static Tensor int8_fused_moe(const Tensor& X, const Tensor& W13, const Tensor& w13_scales, const Tensor& W2, const Tensor& w2_scales,
+                               const Tensor& topk_weights, const Tensor& topk_ids, int64_t act) {
+    const char* op = "int8_fused_moe";
+    const typename A::Guard guard(A::device(X));
+    const ScalarType dt = X.scalar_type();
+    const int code = dtype_code(dt, op);
+    same_device(X, W13, op, "W13");
+    same_device(X, W2, op, "W2");
+    same_device(X, topk_ids, op, "topk_ids");
+    const int64_t ld13 = int8_rows(W13, 3, op, "W13"), ld2 = int8_rows(W2, 3, op, "W2"), ldx = row_distance(X, op, "X");
+    const int64_t E = W13.size(0), H = W13.size(2), I = W2.size(2), tokens = X.size(0);
+    STD_TORCH_CHECK(W2.size(0) == E && W13.size(1) == 2 * I && W2.size(1) == H && X.size(1) == H, op, ": W13 must be [E, 2I, H], W2 [E, H, I] and X [tokens, H]");
+    STD_TORCH_CHECK(topk_ids.scalar_type() == ScalarType::Int && topk_ids.is_contiguous() && topk_ids.dim() == 2 && topk_ids.size(0) == tokens, op,
+                    ": topk_ids must be contiguous int32 [tokens, top_k]");
+    const int64_t top_k = topk_ids.size(1);
+    const float *s13 = scales_of(w13_scales, X, E * 2 * I, op, "w13_scales"), *s2 = scales_of(w2_scales, X, E * H, op, "w2_scales"),
+                *rw = scales_of(topk_weights, X, tokens * top_k, op, "topk_weights");
+    Tensor Y = A::empty(X, {tokens, H}, dt);
+    const int64_t bytes = gguf_b200_int8_moe_workspace_bytes(tokens, top_k, E, H, I);
+    STD_TORCH_CHECK(bytes > 0 || tokens == 0, op, ": unsupported sizes");
+    const typename A::Scratch scratch(X, bytes);
+    check_rc(gguf_b200_int8_fused_moe(X.data_ptr(), ldx, W13.data_ptr(), ld13, s13, W2.data_ptr(), ld2, s2, Y.data_ptr(), static_cast<const int32_t*>(topk_ids.data_ptr()),
+                                      rw, scratch.get(), bytes, code, (int)act, tokens, top_k, E, H, I, A::stream(X)),
+             op);
+    return Y;
+  }
+
+  // scoring: 1 softmax, 2 sigmoid
+  static std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, const std::optional<Tensor>& bias, int64_t top_k, int64_t n_group, int64_t topk_group,
+                                              int64_t scoring, bool renormalize, double scale) {
+    const char* op = "moe_route";
+    const typename A::Guard guard(A::device(logits));
+    const int code = dtype_code(logits.scalar_type(), op);
+    const int64_t ld = row_distance(logits, op, "logits"), T = logits.size(0), E = logits.size(1);
+    STD_TORCH_CHECK(top_k > 0 && n_group > 0 && E % n_group == 0, op, ": top_k must be positive, n_group a divisor of the experts");
+    STD_TORCH_CHECK(topk_group > 0 && topk_group <= n_group && top_k <= topk_group * (E / n_group), op,
+                    ": topk_group must be between 1 and n_group, and its groups hold at least top_k experts");
+    Tensor w = A::empty(logits, {T, top_k}, ScalarType::Float), ids = A::empty(logits, {T, top_k}, ScalarType::Int);
+    check_rc(gguf_b200_moe_route(logits.data_ptr(), code, ld, bias ? scales_of(*bias, logits, E, op, "bias") : nullptr, static_cast<float*>(w.data_ptr()),
+                                 static_cast<int32_t*>(ids.data_ptr()), T, E, top_k, n_group, topk_group, (int)scoring, renormalize, (float)scale,
+                                 A::stream(logits)),
+             op);
+    return {w, ids};
   }
 };
 

@@ -2,7 +2,7 @@
 // reference's binding file (vllm_gguf_plugin/csrc/torch_bindings.cpp:22-53), registered the same
 // way (stable ABI, ops on the CUDA key, ggml_moe_get_block_size as CompositeExplicitAutograd), so
 // `vllm_gguf_plugin.ops` finds `torch.ops._C_gguf.*` unchanged, plus dequant_matmul (the fused route
-// of the IQ types), dequantize_rows, fused_moe and linear_runs.  The bodies are in op_calls.h.
+// of the IQ types), dequantize_rows, fused_moe, linear_runs, the router and the 8-bit integer products.  The bodies are in op_calls.h.
 //
 // This file uses nothing of torch but its stable ABI and nothing of Python but the module
 // entry: the library runs under every torch that has that ABI, whatever the Python version.
@@ -71,6 +71,18 @@ Tensor fused_moe(Tensor X, Tensor W13, Tensor W2, Tensor topk_weights, Tensor to
 }
 Tensor linear_runs(Tensor X, Tensor W, std::vector<int64_t> runs) { return Op::linear_runs(X, W, runs.data(), runs.size()); }
 void weights_complete(Tensor W) { Op::weights_complete(W); }
+std::tuple<Tensor, Tensor> moe_route(Tensor logits, std::optional<Tensor> bias, int64_t top_k, int64_t n_group, int64_t topk_group, int64_t scoring, bool renormalize,
+                                     double scale) {
+  return Op::moe_route(logits, bias, top_k, n_group, topk_group, scoring, renormalize, scale);
+}
+std::tuple<Tensor, Tensor> int8_quantize(Tensor X) { return Op::int8_quantize(X); }
+Tensor int8_mul_mat(Tensor W, Tensor w_scales, Tensor X, std::optional<Tensor> bias) { return Op::int8_mul_mat(W, w_scales, X, bias); }
+Tensor int8_mul_mat_prepared(Tensor W, Tensor w_scales, Tensor Q, Tensor q_scales, std::optional<Tensor> bias, ScalarType dtype) {
+  return Op::int8_mul_mat_prepared(W, w_scales, Q, q_scales, bias, dtype);
+}
+Tensor int8_fused_moe(Tensor X, Tensor W13, Tensor w13_scales, Tensor W2, Tensor w2_scales, Tensor topk_weights, Tensor topk_ids, int64_t act) {
+  return Op::int8_fused_moe(X, W13, w13_scales, W2, w2_scales, topk_weights, topk_ids, act);
+}
 int64_t ggml_moe_get_block_size(int64_t type) { return gguf_b200_moe_block_size((int)type); }
 
 }  // namespace
@@ -88,6 +100,15 @@ STABLE_TORCH_LIBRARY(_C_gguf, ops) {
   ops.def("dequantize_rows(Tensor W, Tensor ids, int type, ScalarType? dtype) -> Tensor");
   ops.def("weights_complete(Tensor W) -> ()");
   ops.def("linear_runs(Tensor X, Tensor W, int[] runs) -> Tensor");
+  ops.def(
+      "moe_route(Tensor logits, Tensor? bias, int top_k, int n_group, int topk_group, int scoring, bool renormalize, float scale) -> "
+      "(Tensor, Tensor)");
+  ops.def("int8_quantize(Tensor X) -> (Tensor, Tensor)");
+  ops.def("int8_mul_mat(Tensor W, Tensor w_scales, Tensor X, Tensor? bias) -> Tensor");
+  ops.def("int8_mul_mat_prepared(Tensor W, Tensor w_scales, Tensor Q, Tensor q_scales, Tensor? bias, ScalarType dtype) -> Tensor");
+  ops.def(
+      "int8_fused_moe(Tensor X, Tensor W13, Tensor w13_scales, Tensor W2, Tensor w2_scales, Tensor topk_weights, Tensor topk_ids, int act) -> "
+      "Tensor");
   ops.def("fused_moe(Tensor X, Tensor W13, Tensor W2, Tensor topk_weights, Tensor topk_ids, int type13, int type2, int act) -> Tensor");
 }
 
@@ -102,6 +123,11 @@ STABLE_TORCH_LIBRARY_IMPL(_C_gguf, CUDA, ops) {
   ops.impl("weights_complete", TORCH_BOX(&weights_complete));
   ops.impl("linear_runs", TORCH_BOX(&linear_runs));
   ops.impl("fused_moe", TORCH_BOX(&fused_moe));
+  ops.impl("moe_route", TORCH_BOX(&moe_route));
+  ops.impl("int8_quantize", TORCH_BOX(&int8_quantize));
+  ops.impl("int8_mul_mat", TORCH_BOX(&int8_mul_mat));
+  ops.impl("int8_mul_mat_prepared", TORCH_BOX(&int8_mul_mat_prepared));
+  ops.impl("int8_fused_moe", TORCH_BOX(&int8_fused_moe));
 }
 
 STABLE_TORCH_LIBRARY_IMPL(_C_gguf, CompositeExplicitAutograd, ops) { ops.impl("ggml_moe_get_block_size", TORCH_BOX(&ggml_moe_get_block_size)); }

@@ -10,11 +10,11 @@ from __future__ import annotations
 import logging
 
 try:
-    from ._eager import embed, linear, linear_runs, moe, mul_mat
+    from ._eager import embed, int8_moe, int8_mul_mat, int8_quantize, linear, linear_runs, moe, moe_route, mul_mat
 except ImportError as exc:
     logging.getLogger("vllm_gguf_plugin").warning("eager calls go through the operator dispatcher: %s", exc)
 
     def _through_the_operators(*args):
         return None
 
-    embed = linear = linear_runs = moe = mul_mat = _through_the_operators
+    embed = int8_moe = int8_mul_mat = int8_quantize = linear = linear_runs = moe = moe_route = mul_mat = _through_the_operators

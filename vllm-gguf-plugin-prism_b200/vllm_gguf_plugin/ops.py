@@ -21,6 +21,10 @@ Differences from the reference, all deliberate:
 * ``ggml_fused_moe`` is new: the whole MoE step of a layer in one call;
 * ``torch.ops._C_gguf.linear_runs`` is new: the product of a merged layer whose shards are of several types, in place
   (the reference copies every shard and concatenates the products, quantization/linear.py:246-262);
+* ``moe_route`` is new: ids and weights of the experts from the router's logits, which the serving engine computes for the
+  reference;
+* ``int8_quantize``, ``int8_mul_mat``, ``int8_mul_mat_prepared`` and ``int8_fused_moe`` are new: products of 8-bit integers with one
+  scale per token and per weight row, dense and for the experts of a layer;
 * ``ggml_dequant_matmul`` is new: the fused form of "ggml_dequantize then x @ W.T" that the
   reference uses for IQ types above the GEMV batch threshold (quantization/linear.py:50-54).
 """
@@ -166,6 +170,33 @@ def _ggml_moe_a8_vec_fake(X, W, topk_ids, top_k, quant_type, row, tokens):
     return torch.empty((X.size(0) * top_k, row), dtype=X.dtype, device=W.device)
 
 
+@register_fake("_C_gguf::moe_route")
+def _moe_route_fake(logits, bias, top_k, n_group, topk_group, scoring, renormalize, scale):
+    shape = (logits.shape[0], top_k)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+
+@register_fake("_C_gguf::int8_quantize")
+def _int8_quantize_fake(X):
+    m, k = X.shape
+    return X.new_empty((m, (k + 15) // 16 * 16), dtype=torch.int8)[:, :k], X.new_empty((m,), dtype=torch.float32)
+
+
+@register_fake("_C_gguf::int8_mul_mat")
+def _int8_mul_mat_fake(W, w_scales, X, bias):
+    return X.new_empty((X.shape[0], W.shape[0]))
+
+
+@register_fake("_C_gguf::int8_mul_mat_prepared")
+def _int8_mul_mat_prepared_fake(W, w_scales, Q, q_scales, bias, dtype):
+    return Q.new_empty((Q.shape[0], W.shape[0]), dtype=dtype)
+
+
+@register_fake("_C_gguf::int8_fused_moe")
+def _int8_fused_moe_fake(X, W13, w13_scales, W2, w2_scales, topk_weights, topk_ids, act):
+    return X.new_empty(X.shape)
+
+
 # --- public API (reference: ops.py:181-286) ---
 
 
@@ -240,6 +271,63 @@ def ggml_fused_moe(X: torch.Tensor, W13: torch.Tensor, W2: torch.Tensor, topk_we
     act = MOE_ACTIVATIONS[activation]
     y = None if is_compiling() else native.moe(X, W13, W2, topk_weights, topk_ids, quant_type, quant_type2, act)
     return torch.ops._C_gguf.fused_moe(X, W13, W2, topk_weights, topk_ids, quant_type, quant_type2, act) if y is None else y
+
+
+ROUTE_SCORINGS = {"softmax": 1, "sigmoid": 2}
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
+              topk_group: int = 1, renormalize: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Router logits ``[tokens, experts]`` -> ``(weights float32, ids int32)``, both ``[tokens, top_k]``, as the MoE calls take them.
+
+    s = softmax or sigmoid of a row; a logit of -inf or NaN masks its expert.  The choice goes by s + ``bias`` (one value per expert)
+    or, without one, by s.  With ``n_group`` > 1 only experts of the ``topk_group`` best groups remain, by the sum of a group's two
+    best choices with a bias, by its best one without.  The best comes first, equals by the lower index.  A weight is s (without the
+    bias), divided by the sum of the row's weights if ``renormalize``, times ``scale``.  A place for which no unmasked expert is left has
+    id -1 and weight 0; the MoE calls skip it.  Up to 512 experts, 32 groups and a ``top_k`` of 32."""
+    if scoring not in ROUTE_SCORINGS:
+        raise NotImplementedError(f"moe_route: scoring {scoring!r} (supported: {sorted(ROUTE_SCORINGS)})")
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.to(torch.float32).contiguous()
+    args = (logits, bias, top_k, n_group, topk_group, ROUTE_SCORINGS[scoring], renormalize, scale)
+    out = None if is_compiling() else native.moe_route(*args)
+    return torch.ops._C_gguf.moe_route(*args) if out is None else out
+
+
+def int8_quantize(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of floats ``[rows, K]`` -> ``(codes int8 [rows, K], scales float32 [rows])``: scale = max |x| / 127, code = x / scale rounded to
+    the nearest integer as exact arithmetic has it, halves to even.  For weights, once, and for activations that several products share.
+    The rows of the codes start at multiples of 16 bytes, as the products want them.  A row with an infinity or a NaN has a scale of NaN."""
+    out = None if is_compiling() else native.int8_quantize(X)
+    return torch.ops._C_gguf.int8_quantize(X) if out is None else out
+
+
+def int8_mul_mat(W: torch.Tensor, w_scales: torch.Tensor, X: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """A linear layer with 8-bit integer weights ``W [N, K]`` and a scale for each of their rows: ``X [tokens, K]`` (float32, float16 or
+    bfloat16) is quantized by the token as ``int8_quantize`` does it, the product is summed exactly, scaled, and rounded once.
+    -> ``[tokens, N]`` in X's dtype.  The rows of W start at multiples of 16 bytes; K up to 131071."""
+    y = None if is_compiling() else native.int8_mul_mat(W, w_scales, X, bias)
+    return torch.ops._C_gguf.int8_mul_mat(W, w_scales, X, bias) if y is None else y
+
+
+def int8_mul_mat_prepared(W: torch.Tensor, w_scales: torch.Tensor, Q: torch.Tensor, q_scales: torch.Tensor, dtype: torch.dtype,
+                          bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``int8_mul_mat`` on what ``int8_quantize`` made of the activations, for several products of the same ones."""
+    return torch.ops._C_gguf.int8_mul_mat_prepared(W, w_scales, Q, q_scales, bias, dtype)
+
+
+def int8_fused_moe(X: torch.Tensor, W13: torch.Tensor, w13_scales: torch.Tensor, W2: torch.Tensor, w2_scales: torch.Tensor,
+                   topk_weights: torch.Tensor, topk_ids: torch.Tensor, activation: str) -> torch.Tensor:
+    """``ggml_fused_moe`` on 8-bit integer weights: ``W13 [E, 2I, H]`` (gate rows, then up rows) with ``w13_scales [E, 2I]``, ``W2 [E, H, I]``
+    with ``w2_scales [E, H]``.  Tokens, and the hidden rows act(gate) * up in fp32, are quantized by the row; the sum over the experts
+    is rounded once.  X ``[T, H]`` -> ``[T, H]``.  Ids outside [0, E) contribute nothing.  E <= 256; H and I multiples of 8."""
+    if topk_weights.dtype != torch.float32 or not topk_weights.is_contiguous():
+        topk_weights = topk_weights.to(torch.float32).contiguous()
+    if topk_ids.dtype != torch.int32 or not topk_ids.is_contiguous():
+        topk_ids = topk_ids.to(torch.int32).contiguous()
+    args = (X, W13, w13_scales, W2, w2_scales, topk_weights, topk_ids, MOE_ACTIVATIONS[activation])
+    y = None if is_compiling() else native.int8_moe(*args)
+    return torch.ops._C_gguf.int8_fused_moe(*args) if y is None else y
 
 
 def ggml_moe_a8_vec(
