@@ -6,12 +6,12 @@
 // box).  Weight rows sit on the 128-row side of the instruction, tokens on its column side, any multiple of 16 up to 256; so one
 // token costs no more tensor time than sixteen, and what bounds small batches is the weights' way from memory.
 //
-// A CTA: a loader, an MMA issuer, four epilogue warps (thread = weight row = lane of tensor memory), over a ring of stages of 128
+// A CTA: a loader, an MMA issuer, eight epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
 // values.  Three ways to deal out the work:
 //   tiles    a CTA takes items (128 weight rows x up to 256 tokens) a grid apart, two accumulators in turn where they fit
 //   split    fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares the K of one tile.  Each sends its sums of every other's
-//            columns into the other's shared memory, which then adds and stores its columns: no scratch in memory, nothing to clear,
-//            and integer sums do not depend on the order
+//            rows into the other's shared memory, which then adds and stores its rows: no scratch in memory, nothing to clear, and
+//            integer sums do not depend on the order
 //   experts  items are (pass of an expert's tokens, 128 rows); for the gate and up product two boxes of weights, of the same rows of
 //            gate and up, meet the same tokens in two accumulators, so that a thread has both and act(gate) * up never leaves it
 //            but as the result
@@ -28,10 +28,11 @@ namespace gguf_b200 {
 
 constexpr int I8_ROWS = 128, I8_BK = 128;                 // weight rows of a box, values (= bytes) of a stage
 constexpr int I8_A_BYTES = I8_ROWS * I8_BK;
-constexpr int I8_THREADS = 256;                           // warps 0 loader, 1 MMA issuer, 2 tensor memory, 4 to 7 epilogue
+constexpr int I8_EPI = 8;                                 // epilogue warps
+constexpr int I8_THREADS = 128 + 32 * I8_EPI;             // warps 0 loader, 1 MMA issuer, 2 tensor memory, from 4 on epilogue
 constexpr int I8_MAX_STAGES = 16;
 constexpr int I8_SMS = 148;
-constexpr int I8_AUX = 512 + 2 * 256 * 8;                 // barriers; scale and output row of every token, of two items
+constexpr int I8_AUX = 512 + 2 * 256 * 8 + I8_EPI * 1024; // barriers; scale and output row of every token, of two items; 16 tokens x 32 rows a warp
 
 struct I8Params {
   int n, n_up;             // weight rows; distance of the up rows from the gate rows
@@ -92,10 +93,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void st_peer(uint32_t saddr, uint32_t rank, uint32_t v) {   // into CTA `rank` of the cluster, at this CTA's address
-  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.u32 [a], %2;\n\t}" ::"r"(saddr), "r"(rank), "r"(v) : "memory");
-}
-
 __device__ __forceinline__ float i8_act(int act, float g) { return act == 1 ? g / (1.f + expf(-g)) : 0.5f * g * (1.f + erff(g * 0.70710678f)); }
 __device__ __forceinline__ void i8_put(void* y, int dtype, int64_t at, float v) {
   if (dtype == DT_F32) static_cast<float*>(y)[at] = v;
@@ -106,6 +103,35 @@ __device__ __forceinline__ float i8_bias(const I8Params& p, int n) {
   if (!p.bias) return 0.f;
   return p.dtype == DT_F32 ? static_cast<const float*>(p.bias)[n]
          : p.dtype == DT_F16 ? __half2float(static_cast<const __half*>(p.bias)[n]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
+}
+
+// Sixteen tokens (f[0 .. count)) of a warp's 32 rows, a lane's row being n: token j goes to row to[j] of y.  fp32 leaves as it is, 128 bytes
+// an instruction.  16-bit results go through the warp's kilobyte of shared memory, and from there, where all 32 rows count and
+// 16-byte stores are aligned (`wide`), eight tokens an instruction.
+template <typename T>
+__device__ __forceinline__ void i8_store16(T* __restrict__ y, int64_t ldy, const int* to, int count, const float (&f)[16], int n, int lane, int rows, bool wide,
+                                           uint8_t* stage) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < count && lane < rows) y[to[j] * ldy + n] = f[j];
+  } else {
+    T* st = reinterpret_cast<T*>(stage);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) st[j * 32 + lane] = from_float<T>(f[j]);
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = 8 * h + (lane >> 2), part = lane & 3;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + j * 64 + part * 16);
+        if (j < count) *reinterpret_cast<uint4*>(y + to[j] * ldy + (n - lane + 8 * part)) = v;
+      }
+    } else if (lane < rows) {
+      for (int j = 0; j < count; ++j) y[to[j] * ldy + n] = st[j * 32 + lane];
+    }
+    __syncwarp();
+  }
 }
 
 struct I8Item {
@@ -141,6 +167,7 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_scale = reinterpret_cast<float*>(smem + p.aux_off + 512);   // [2][256]
   int* s_row = reinterpret_cast<int*>(s_scale + 512);                  // [2][256]
+  uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_row + 512);          // [I8_EPI][1024]
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -150,7 +177,7 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&accum[s], 1);
-      mbar_init(&drained[s], 4);
+      mbar_init(&drained[s], I8_EPI);
     }
     *gave_up = 0;
     fence_barrier_init();
@@ -244,8 +271,11 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     __syncwarp();
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
-    const int row = (warp - 4) * 32 + lane;
-    const uint32_t t_lane = tmem + ((uint32_t)((warp - 4) * 32) << 16);
+    // (a warp reaches the 32 lanes of tensor memory of its number modulo 4; two warps share them, taking 16 columns in turn)
+    const int quad = (warp & 3) * 32, row = quad + lane, half = (warp - 4) >> 2, tid = threadIdx.x - 128;
+    const uint32_t t_lane = tmem + ((uint32_t)quad << 16);
+    uint8_t* stage = s_stage + (warp - 4) * 1024;
+    const bool wide_y = p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
     int buf = 0, turn = 0;
     uint32_t aph = 0;
     pdl_wait();
@@ -255,43 +285,49 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
       float* xs = s_scale + turn * 256;   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
       int* xr = s_row + turn * 256;
       turn ^= 1;
-      for (int c = row; c < t.rows; c += 128) {
-        const int at = t.x0 + c;
-        float f = p.q_scale[at];
-        int o = at;
-        if (p.passes && NA == 1) {
-          o = p.sorted[at];
-          f *= p.row_scale[o];
+      for (int c = tid; c < p.tn; c += 32 * I8_EPI) {
+        float f = 0.f;
+        int o = t.x0 + c;
+        if (c < t.rows) {
+          f = p.q_scale[o];
+          if (p.passes && NA == 1) {
+            o = p.sorted[o];
+            f *= p.row_scale[o];
+          }
         }
         xs[c] = f;
         xr[c] = o;
       }
-      const int n = t.n0 + row;
-      const bool live = n < p.n;
+      const int n = t.n0 + row, rows = min(32, p.n - (t.n0 + quad));   // (of this warp's 32; not positive: none)
+      const bool live = lane < rows;
       const float ws = live ? p.w_scale[t.a_row + row] : 0.f, wu = NA == 2 && live ? p.w_scale[t.a_row + p.n_up + row] : 0.f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
       __syncwarp();
       tc_fence_after();
-      const uint32_t d = t_lane + (uint32_t)(buf * NA * p.tn);
       if (p.split == 1) {
+        const uint32_t d = t_lane + (uint32_t)(buf * NA * p.tn);
         const float bias = live ? i8_bias(p, n) : 0.f;
-        for (int c0 = 0; c0 < t.rows; c0 += 16) {
+        for (int c0 = 16 * half; c0 < t.rows; c0 += 32) {
           uint32_t v[16], u[16];
           tmem_ld16(d + (uint32_t)c0, v);
           if (NA == 2) tmem_ld16(d + (uint32_t)(p.tn + c0), u);
-          tmem_ld_wait();
-          if (live) {
+          float f[16];
+          float4 x[4];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int c = c0 + j;
-              if (c < t.rows) {
-                float f = (float)(int)v[j] * (xs[c] * ws);
-                if (NA == 2) f = i8_act(p.act, f) * ((float)(int)u[j] * (xs[c] * wu));
-                i8_put(p.y, p.dtype, xr[c] * p.ldy + n, f + bias);
-              }
-            }
+          for (int j = 0; j < 4; ++j) x[j] = reinterpret_cast<const float4*>(xs + c0)[j];
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float xj = reinterpret_cast<const float*>(x)[j];
+            f[j] = (float)(int)v[j] * (xj * ws);
+            if (NA == 2) f[j] = i8_act(p.act, f[j]) * ((float)(int)u[j] * (xj * wu));
+            else f[j] += bias;
           }
+          const int count = min(16, t.rows - c0);
+          if (NA == 2 || p.dtype == DT_F32) i8_store16<float>(static_cast<float*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, false, stage);
+          else if (p.dtype == DT_F16) i8_store16<__half>(static_cast<__half*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, wide_y && rows == 32, stage);
+          else i8_store16<__nv_bfloat16>(static_cast<__nv_bfloat16*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, wide_y && rows == 32, stage);
         }
         tc_fence_before();
         __syncwarp();
@@ -301,34 +337,36 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     }
   }
   __syncwarp();
-  if (p.split > 1) {
-    // ---------------- split: the sums of tokens [c * rank, c * rank + c) are this CTA's to add and store ----------------
+  if (NA == 1 && p.split > 1) {
+    // ---------------- split: the sums of rows [per * rank, per * (rank + 1)) of the tile are this CTA's to add and store ----------------
     cluster_sync();   // every CTA's products are complete, its ring is free: [from][token][row]
     const I8Item t = i8_item(p, first);
-    const int row = (warp - 4) * 32 + lane, c = p.tn / p.split, n = t.n0 + row;
+    const int per = I8_ROWS / p.split, shift = 31 - __clz(per);
     const uint32_t ring = smem_u32(smem);
     if (warp >= 4) {
-      const uint32_t d = tmem + ((uint32_t)((warp - 4) * 32) << 16);
-      for (int c0 = 0; c0 < t.rows; c0 += 16) {
+      const int quad = (warp & 3) * 32, row = quad + lane;
+      const uint32_t d = tmem + ((uint32_t)quad << 16);
+      uint32_t peer;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ring + 4u * (uint32_t)((int)rank * p.tn * per + (row & (per - 1)))), "r"(row >> shift));
+      for (int c0 = 16 * ((warp - 4) >> 2); c0 < t.rows; c0 += 32) {
         uint32_t v[16];
         tmem_ld16(d + (uint32_t)c0, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int to = (c0 + j) / c;
-          st_peer(ring + 4u * (uint32_t)(((int)rank * c + c0 + j - to * c) * I8_ROWS + row), (uint32_t)to, v[j]);
-        }
+        for (int j = 0; j < 16; ++j) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer + 4u * (uint32_t)((c0 + j) * per)), "r"(v[j]) : "memory");
       }
     }
     cluster_sync();
-    if (warp >= 4 && n < p.n) {
-      const float ws = p.w_scale[t.a_row + row], bias = i8_bias(p, n);
-      for (int j = 0; j < c; ++j) {
-        const int tok = (int)rank * c + j;
-        if (tok >= t.rows) break;
-        int sum = 0;
-        for (int from = 0; from < p.split; ++from) sum += (int)lds32(ring + 4u * (uint32_t)((from * c + j) * I8_ROWS + row));
-        i8_put(p.y, p.dtype, (int64_t)(t.x0 + tok) * p.ldy + n, (float)sum * (s_scale[tok] * ws) + bias);
+    if (warp >= 4) {
+      const int tid = threadIdx.x - 128, r = tid & (per - 1), row = (int)rank * per + r, n = t.n0 + row;
+      if (n < p.n) {
+        const float ws = p.w_scale[t.a_row + row], bias = i8_bias(p, n);
+        for (int c = tid >> shift; c < t.rows; c += 32 * I8_EPI >> shift) {
+          int sum = 0;
+#pragma unroll 4
+          for (int from = 0; from < p.split; ++from) sum += (int)lds32(ring + 4u * (uint32_t)((from * p.tn + c) * per + r));
+          i8_put(p.y, p.dtype, (int64_t)(t.x0 + c) * p.ldy + n, (float)sum * (s_scale[c] * ws) + bias);
+        }
       }
     }
   }

@@ -1,9 +1,8 @@
 // Rows of floats to 8-bit integers with one scale a row:  a = max |x|,  scale = a / 127,  code = x * 127 / a, halves to even.
 // The same kernel serves a token's activations, an expert's hidden rows and, once, a weight matrix.
 //
-// The codes are those of exact arithmetic.  x * (127 / a) in fp32 is off by less than 127 * 2^-22; within 2^-14 of a half the
-// side is settled by the sign of 254 |x| - (2 m + 1) a in fp64, where both products are exact (24 + 8 bits).  16-bit inputs hit
-// halves all the time (x = a / 2 is code 63.5).  A row with an infinity or a NaN has no scale: it gets NaN for one and codes of 0,
+// The codes are those of exact arithmetic.  x * (127 / a) with the quotient in fp32 is off by less than 2^-17; within 2^-14 of a half
+// the side is settled exactly (i8q_codes).  16-bit inputs hit halves all the time (x = a / 2 is code 63.5).  A row with an infinity or a NaN has no scale: it gets NaN for one and codes of 0,
 // so that every result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once.
@@ -30,25 +29,41 @@ template <typename T> __device__ __forceinline__ uint32_t i8q_top(const T (&v)[I
   for (int i = 0; i < I8Q_UNIT; ++i) top = max(top, __float_as_uint(to_float<T>(v[i])) & 0x7fffffffu);   // (of bit patterns: infinity and NaN above all numbers)
   return top;
 }
-__device__ __forceinline__ int i8q_code(float x, float inv, float a) {
-  const float t = x * inv, r = rintf(t);
-  int c = (int)r;
-  if (fabsf(t - r) > 0.5f - 0x1p-14f) {
-    const int m = (int)fabsf(t);
-    const double d = 254.0 * (double)fabsf(x) - (double)(2 * m + 1) * (double)a;
-    const int u = m + (d > 0.0 || (d == 0.0 && (m & 1)));
-    c = x < 0.f ? -u : u;
+// Four codes, a byte each.  1.5 * 2^23 added in one fused step rounds x / scale to an integer in the low bits; what was rounded away says
+// whether a half is near, which is settled exactly: the sign of 254 |x| - (2 m + 1) a, m + 1/2 being the half, from two products and
+// their rounding errors (the products are within a few ulp of one another, so their difference is exact).
+__device__ __forceinline__ uint32_t i8q_codes(const float (&x)[4], float inv, float a) {
+  constexpr float MAGIC = 12582912.f;
+  float r[4], off = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = fmaf(x[i], inv, MAGIC);
+    off = fmaxf(off, fabsf(fmaf(x[i], inv, MAGIC - r[i])));
   }
-  return c;
+  if (off > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = fabsf(x[i]), t = u * inv, m = floorf(t);
+      if (fabsf(t - m - 0.5f) < 0x1p-13f) {
+        const float h = 2.f * m + 1.f, p = 254.f * u, q = h * a;
+        const float d = (p - q) + (fmaf(254.f, u, -p) - fmaf(h, a, -q));
+        const float c = d > 0.f || (d == 0.f && ((int)m & 1)) ? m + 1.f : m;
+        r[i] = MAGIC + copysignf(c, x[i]);
+      }
+    }
+  }
+  const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
 template <typename T>
 __device__ __forceinline__ void i8q_store(const T (&v)[I8Q_UNIT], float lift, float inv, float a, int8_t* __restrict__ q, int64_t k, int64_t at) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = 0;
+    float x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)i8q_code(to_float<T>(v[4 * i + j]) * lift, inv, a) & 0xffu) << (8 * j);
+    for (int j = 0; j < 4; ++j) x[j] = to_float<T>(v[4 * i + j]) * lift;
+    w[i] = i8q_codes(x, inv, a);
   }
   if (at + I8Q_UNIT <= k) {
     *reinterpret_cast<uint4*>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -61,7 +76,7 @@ __device__ __forceinline__ void i8q_store(const T (&v)[I8Q_UNIT], float lift, fl
 
 // LANES threads a row, 256 / LANES rows a block
 template <typename T, bool VEC, int LANES>
-__global__ void __launch_bounds__(256) i8_quantize_kernel(const I8Quantize p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : VEC ? 4 : 3) i8_quantize_kernel(const I8Quantize p) {
   __shared__ uint32_t s_top[8];
   const int lane = threadIdx.x % LANES;
   pdl_wait();
@@ -98,7 +113,7 @@ __global__ void __launch_bounds__(256) i8_quantize_kernel(const I8Quantize p) {
       for (int i = 1; i < LANES / 32; ++i) top = max(top, s_top[i]);
     }
     const bool finite = top < 0x7f800000u;
-    const float a0 = __uint_as_float(top), lift = a0 < 0x1p-90f ? 0x1p64f : 1.f;   // (so that 127 / a stays finite; exact)
+    const float a0 = __uint_as_float(top), lift = a0 < 0x1p-90f ? 0x1p64f : a0 > 0x1p100f ? 0x1p-64f : 1.f;   // (so that 127 / a and 254 a stay in range)
     const float a = a0 * lift, inv = finite && top != 0 ? 127.f / a : 0.f;
     if (live && lane == 0) p.scale[r] = finite ? a0 / 127.f : __uint_as_float(0x7fc00000u);
     int8_t* q = p.q + r * p.ldq;
