@@ -248,7 +248,9 @@ def test_streams_graphs_and_threads(ops):
 
 
 def moe_want(x, w13, s13, w2, s2, weights_, ids, act):
-    """(result, tolerance before the last rounding) in float64.  fp32 rounds a hidden value h = act(gate) * up by at most 2^-19 of itself
+    """(result, tolerance before the last rounding) in float64.  For 16-bit tokens an expert's result is rounded to fp16 once on its way to
+    the sum: 2^-11 of itself, or, below fp16's normal numbers, 2^-25 of what it was divided by: powers of two of at most I and at most
+    twice the expert's largest scale.  fp32 rounds a hidden value h = act(gate) * up by at most 2^-19 of itself
     (gate and up: 5 * 2^-24 each; the activation's condition number is below 1 + |gate| with |gate| < 100 only where h counts, 2^-19
     covers |gate| < 30): a code within 127 * 2^-18 of a half may go either way, one step of the row's scale times its weight."""
     q, qs = codes_of(x)
@@ -271,6 +273,8 @@ def moe_want(x, w13, s13, w2, s2, weights_, ids, act):
             part = (code @ w2[e].double().T) * f
             out[t] += part
             room[t] += (close @ w2[e].double().abs().T) * f.abs() + 2.0 ** -18 * part.abs()
+            if x.dtype != torch.float32:
+                room[t] += 2.0 ** -11 * part.abs() + 2.0 ** -25 * half * 2 * float(s2[e].max()) * (a / 127) * weights_[t, j].double().abs()[:, None]
     return out, room
 
 

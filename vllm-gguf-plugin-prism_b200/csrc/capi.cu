@@ -723,7 +723,7 @@ int gguf_b200_fused_moe(const void* X, const void* W13, const void* W2, void* Y,
     if (rc) return rc;
     rc = gemm(base + L.o_y1, 1, act, W2, type2, H, I, base + L.o_y2, topk_weights);
     if (rc) return rc;
-    return launch_moe_sum(base + L.o_y2, false, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+    return launch_moe_sum(base + L.o_y2, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
   }
   const FusedMoeLayout L = fused_moe_layout(type13, type2, dtype, tokens, top_k, n_experts, H, I);
   if (ws_bytes < L.total) return E_WORKSPACE;
@@ -774,7 +774,7 @@ int gguf_b200_fused_moe(const void* X, const void* W13, const void* W2, void* Y,
   rc = gemm(base + L.o_y1, 1, W2, type2, H, I, base + L.o_y2, topk_weights, act, 2 * I);
   if (rc) return rc;
   // 4. sum over the top_k slots of every token
-  return launch_moe_sum(base + L.o_y2, false, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+  return launch_moe_sum(base + L.o_y2, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
 }
 
 int gguf_b200_moe_a8_vec(const void* X, const void* W, void* Y, void* ws, int64_t ws_bytes, const int32_t* topk_ids,
@@ -806,18 +806,20 @@ int i8_check(int dtype, int64_t M, int64_t N, int64_t K) {
   return E_OK;
 }
 struct I8MoeLayout {
-  int64_t pass_rows, passes, o_sorted, o_passes, o_npass, o_q1, o_s1, o_q2, o_s2, o_h, total;
+  int64_t pass_rows, passes, o_sorted, o_place, o_passes, o_npass, o_units, o_q1, o_s1, o_q2, o_s2, o_h, total;
 };
 I8MoeLayout i8_moe_layout(int64_t tokens, int64_t top_k, int64_t E, int64_t H, int64_t I) {
   I8MoeLayout L{};
   const int64_t slots = tokens * top_k;
   L.pass_rows = i8_moe_pass_rows(slots, E);
-  L.passes = moe_plan_passes(slots, (int)E, (int)L.pass_rows);
+  L.passes = i8_moe_passes(slots, E, L.pass_rows);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o += round_up(bytes, 256); return at; };
   L.o_sorted = take(slots * 4);
+  L.o_place = take(slots * 4);
   L.o_passes = take(L.passes * 16);
   L.o_npass = take(8);
+  L.o_units = take(2 * E * 4);
   L.o_q1 = take(slots * i8_ld(H));
   L.o_s1 = take(slots * 4);
   L.o_q2 = take(slots * i8_ld(I));
@@ -896,17 +898,23 @@ int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* base = static_cast<uint8_t*>(ws);
   const int64_t slots = tokens * top_k;
-  int32_t* sorted = reinterpret_cast<int32_t*>(base + L.o_sorted);
-  int32_t* npass = reinterpret_cast<int32_t*>(base + L.o_npass);
+  int32_t *sorted = reinterpret_cast<int32_t*>(base + L.o_sorted), *place = reinterpret_cast<int32_t*>(base + L.o_place),
+          *npass = reinterpret_cast<int32_t*>(base + L.o_npass);
+  float* units = reinterpret_cast<float*>(base + L.o_units);
   // 1. expert-sorted slots and the passes over them; slots without a valid expert are in none, and the sum skips them
-  rc = launch_moe_plan(topk_ids, slots, (int)n_experts, 1, (int)L.pass_rows, sorted, base + L.o_passes, npass, s);
+  I8Plan plan{};
+  plan.topk_ids = topk_ids; plan.slots = slots; plan.experts = (int)n_experts; plan.pass_rows = (int)L.pass_rows;
+  plan.w2_scale = w2_scales; plan.h = H;
+  plan.sorted = sorted; plan.place = place; plan.passes = base + L.o_passes; plan.n_passes = npass;
+  plan.w_unit = units; plan.w_top = units + n_experts;
+  rc = launch_i8_plan(plan, s);
   if (rc) return rc;
-  // 2. every slot's token, quantized, in the order of the experts
+  // 2. the tokens, quantized, a copy in the place of every slot
   I8Quantize q{};
   q.x = X; q.dtype = dtype; q.ldx = ldx;
   q.q = reinterpret_cast<int8_t*>(base + L.o_q1); q.ldq = i8_ld(H); q.scale = reinterpret_cast<float*>(base + L.o_s1);
-  q.rows = slots; q.k = H;
-  q.gather = sorted; q.gather_div = top_k; q.n_used = npass + 1;
+  q.rows = tokens; q.k = H;
+  q.scatter = place; q.copies = (int)top_k;
   rc = launch_i8_quantize(q, s);
   if (rc) return rc;
   // 3. gate and up products and the activation: hidden rows in fp32 (their largest value decides about all codes of a row)
@@ -929,18 +937,24 @@ int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_
   q2.n_used = npass + 1;
   rc = launch_i8_quantize(q2, s);
   if (rc) return rc;
-  // 5. down products, weighted, back in the order of the slots; in fp32, so that the sum is rounded once
+  // 5. down products, back in the order of the slots, divided by powers of two (int8_moe.cu)
+  const float unit = exp2f(ceilf(log2f((float)I)) - 1.f);   // 128 * 128 * I / unit <= 2^15
   a.w = static_cast<const int8_t*>(W2); a.ldw = ld2; a.w_scale = w2_scales;
   a.q = q2.q; a.ldq = q2.ldq; a.q_scale = q2.scale;
+  a.dtype = dtype == DT_F32 ? DT_F32 : DT_F16;
   a.ldy = H;
   a.n = H; a.k = I;
   a.act = 0;
   a.sorted = sorted;
-  a.row_scale = topk_weights;
+  a.w_unit = units;
+  a.unit = 1.f / unit;
   rc = launch_i8_product(a, s);
   if (rc) return rc;
-  // 6. sum over the top_k slots of every token
-  return launch_moe_sum(base + L.o_h, true, Y, topk_ids, (int)n_experts, tokens, top_k, H, dtype, s);
+  // 6. weighted sum over the top_k slots of every token
+  I8Sum y{};
+  y.y = base + L.o_h; y.out = Y; y.place = place; y.topk_ids = topk_ids; y.topk_weights = topk_weights; y.q_scale = q2.scale; y.w_top = units + n_experts;
+  y.unit = unit; y.tokens = tokens; y.top_k = top_k; y.h = H; y.dtype = dtype;
+  return launch_i8_sum(y, s);
 }
 
 int gguf_b200_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, float* weights, int32_t* ids, int64_t tokens, int64_t n_experts,

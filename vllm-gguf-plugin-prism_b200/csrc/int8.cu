@@ -12,12 +12,9 @@
 //   split    fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares the K of one tile.  Each sends its sums of every other's
 //            rows into the other's shared memory, which then adds and stores its rows: no scratch in memory, nothing to clear, and
 //            integer sums do not depend on the order
-//   experts  items are (pass of an expert's tokens, 128 rows); for the gate and up product two boxes of weights, of the same rows of
-//            gate and up, meet the same tokens in two accumulators, so that a thread has both and act(gate) * up never leaves it
-//            but as the result
+//   experts  items are (pass of an expert's tokens, 128 rows).  For the gate and up product a box holds the same 64 rows of both, 16 and
+//            16 in turn: the two meet in one warp, so that act(gate) * up is formed on the way out and nothing else is stored
 #include <cuda.h>
-
-#include <math.h>
 
 #include "int8.cuh"
 #include "kernels.h"
@@ -35,7 +32,7 @@ constexpr int I8_SMS = 148;
 constexpr int I8_AUX = 512 + 2 * 256 * 8 + I8_EPI * 1024; // barriers; scale and output row of every token, of two items; 16 tokens x 32 rows a warp
 
 struct I8Params {
-  int n, n_up;             // weight rows; distance of the up rows from the gate rows
+  int n;                   // results a token
   int w_rows;              // weight rows of an expert
   int k, nk;               // values, stages
   int m, rt, tt, tn, bh;   // tokens; row tiles, token tiles; tokens a tile; rows of a box of tokens
@@ -52,7 +49,8 @@ struct I8Params {
   const int32_t* n_passes;
   int act;
   const int32_t* sorted;
-  const float* row_scale;
+  const float* w_unit;
+  float unit;
   int* status;
 };
 
@@ -82,6 +80,12 @@ __device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int
       ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ void i8_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void i8_box_l2(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
@@ -93,12 +97,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float i8_act(int act, float g) { return act == 1 ? g / (1.f + expf(-g)) : 0.5f * g * (1.f + erff(g * 0.70710678f)); }
-__device__ __forceinline__ void i8_put(void* y, int dtype, int64_t at, float v) {
-  if (dtype == DT_F32) static_cast<float*>(y)[at] = v;
-  else if (dtype == DT_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
-}
+// (the approximate exponential and quotient are off by a few units in the last place, 2^-21 of the result)
+__device__ __forceinline__ float i8_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+__device__ __forceinline__ float i8_gelu(float g) { return 0.5f * g * (1.f + erff(g * 0.70710678f)); }
 __device__ __forceinline__ float i8_bias(const I8Params& p, int n) {
   if (!p.bias) return 0.f;
   return p.dtype == DT_F32 ? static_cast<const float*>(p.bias)[n]
@@ -109,12 +110,12 @@ __device__ __forceinline__ float i8_bias(const I8Params& p, int n) {
 // an instruction.  16-bit results go through the warp's kilobyte of shared memory, and from there, where all 32 rows count and
 // 16-byte stores are aligned (`wide`), eight tokens an instruction.
 template <typename T>
-__device__ __forceinline__ void i8_store16(T* __restrict__ y, int64_t ldy, const int* to, int count, const float (&f)[16], int n, int lane, int rows, bool wide,
+__device__ __forceinline__ void i8_store16(T* __restrict__ y, int64_t ldy, const int* to, int count, const float (&f)[16], int n, int lane, bool live, bool wide,
                                            uint8_t* stage) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (j < count && lane < rows) y[to[j] * ldy + n] = f[j];
+      if (j < count && live) y[to[j] * ldy + n] = f[j];
   } else {
     T* st = reinterpret_cast<T*>(stage);
 #pragma unroll
@@ -127,35 +128,52 @@ __device__ __forceinline__ void i8_store16(T* __restrict__ y, int64_t ldy, const
         const uint4 v = *reinterpret_cast<const uint4*>(stage + j * 64 + part * 16);
         if (j < count) *reinterpret_cast<uint4*>(y + to[j] * ldy + (n - lane + 8 * part)) = v;
       }
-    } else if (lane < rows) {
+    } else if (live) {
       for (int j = 0; j < count; ++j) y[to[j] * ldy + n] = st[j * 32 + lane];
     }
     __syncwarp();
   }
 }
+__device__ __forceinline__ void i8_store16(const I8Params& p, const int* to, int count, const float (&f)[16], int n, int lane, bool live, bool wide, uint8_t* stage) {
+  if (p.dtype == DT_F32) i8_store16<float>(static_cast<float*>(p.y), p.ldy, to, count, f, n, lane, live, wide, stage);
+  else if (p.dtype == DT_F16) i8_store16<__half>(static_cast<__half*>(p.y), p.ldy, to, count, f, n, lane, live, wide, stage);
+  else i8_store16<__nv_bfloat16>(static_cast<__nv_bfloat16*>(p.y), p.ldy, to, count, f, n, lane, live, wide, stage);
+}
 
 struct I8Item {
-  int n0, a_row;           // first row of the tile in its matrix, and in the weights
+  int n0, a_row, e;        // first result, first row in the weights (gate and up: of the gate), expert
   int x0, rows;            // tokens
 };
-__device__ __forceinline__ I8Item i8_item(const I8Params& p, int i) {
+// (waited: behind this thread's pdl_wait)
+template <bool GLU> __device__ __forceinline__ I8Item i8_item(const I8Params& p, int i, bool waited) {
   I8Item t;
   if (p.passes) {
-    const int4 q = p.passes[i / p.rt];
-    t.n0 = i % p.rt * I8_ROWS;
+    const int4 q = waited ? p.passes[i / p.rt] : ld_older(p.passes + i / p.rt);
+    t.e = q.x;
+    t.n0 = i % p.rt * (GLU ? I8_ROWS / 2 : I8_ROWS);
     t.a_row = q.x * p.w_rows + t.n0;
     t.x0 = q.y;
     t.rows = q.z;
   } else {   // the token tiles of a row tile are neighbours
+    t.e = 0;
     t.a_row = t.n0 = i / p.tt * I8_ROWS;
     t.x0 = i % p.tt * p.tn;
     t.rows = min(p.tn, p.m - t.x0);
   }
   return t;
 }
+// The weights of a stage: 128 rows, or four times 16 gate rows and the 16 up rows that go with them
+template <bool GLU> __device__ __forceinline__ void i8_weights(const CUtensorMap* map, uint32_t at, int kb, const I8Item& t, uint32_t bar) {
+  if (GLU) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) i8_box3(at + (uint32_t)(g * 32 * I8_BK), map, kb * I8_BK, t.n0 + 16 * g, 2 * t.e, bar);
+  } else {
+    i8_box(at, map, kb * I8_BK, t.a_row, bar);
+  }
+}
 
-// NA: boxes of weights a stage (2: gate and up)
-template <int NA>
+// GLU: gate and up product of experts
+template <bool GLU>
 __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                                                            const __grid_constant__ I8Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -196,21 +214,23 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
   const uint32_t accum_s = smem_u32(accum), drained_s = smem_u32(drained);
   const int first = p.split > 1 ? (int)blockIdx.x / p.split : (int)blockIdx.x, step = p.split > 1 ? 1 << 30 : (int)gridDim.x;
   const int kb0 = p.split > 1 ? (int)(p.nk * rank) / p.split : 0, kb1 = p.split > 1 ? (int)(p.nk * (rank + 1)) / p.split : p.nk;
-  auto items = [&] { return p.passes ? *p.n_passes * p.rt : p.rt * p.tt; };   // (behind pdl_wait where there are passes)
+  // (the work list is older than the trigger of the kernel ahead: see pdl_wait)
+  const int n_items = p.passes ? __shfl_sync(0xffffffffu, ld_older(p.n_passes), 0) * p.rt : p.rt * p.tt;
 
   if (warp == 0) {
     // ---------------- loader ----------------
     const uint32_t lead = elect_one() ? 1u : 0u, ring = smem_u32(smem);
     int s = 0, ahead = 0;
     uint32_t ph = 0;
-    if (!p.passes) {   // the first weights before the activations are there: into the ring, or, if they may still be written, into L2
-      const I8Item t = i8_item(p, first);
+    if (first < n_items) {   // the first weights before the activations are there: into the ring, or, if they may still be written, into L2
+      const I8Item t = i8_item<GLU>(p, first, false);
+      const uint32_t bytes = (uint32_t)(I8_A_BYTES + (t.rows + p.bh - 1) / p.bh * p.bh * I8_BK);
       ahead = min(p.stages, kb1 - kb0);
       for (int j = 0; j < ahead; ++j)
         if (lead) {
           if (p.settled) {
-            mbar_expect_tx(full_s + 8u * j, (uint32_t)(NA * I8_A_BYTES + (t.rows + p.bh - 1) / p.bh * p.bh * I8_BK));
-            i8_box(ring + (uint32_t)(j * p.stage_bytes), &amap, (kb0 + j) * I8_BK, t.a_row, full_s + 8u * j);
+            mbar_expect_tx(full_s + 8u * j, bytes);
+            i8_weights<GLU>(&amap, ring + (uint32_t)(j * p.stage_bytes), kb0 + j, t, full_s + 8u * j);
           } else {
             i8_box_l2(&amap, (kb0 + j) * I8_BK, t.a_row);
           }
@@ -218,9 +238,8 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
       if (!p.settled) ahead = 0;
     }
     pdl_wait();
-    const int n = items();
-    for (int i = first; i < n; i += step) {
-      const I8Item t = i8_item(p, i);
+    for (int i = first; i < n_items; i += step) {
+      const I8Item t = i8_item<GLU>(p, i, true);
       const int boxes = (t.rows + p.bh - 1) / p.bh;
       for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t fb = full_s + 8u * s, at = ring + (uint32_t)(s * p.stage_bytes);
@@ -229,15 +248,14 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
           if (lds32(gave_up_s) != 0u) goto loaded;   // (no copy into a slot that may be in use)
           __syncwarp();
           if (lead) {
-            mbar_expect_tx(fb, (uint32_t)(NA * I8_A_BYTES + boxes * p.bh * I8_BK));
-            i8_box(at, &amap, kb * I8_BK, t.a_row, fb);
-            if (NA == 2) i8_box(at + I8_A_BYTES, &amap, kb * I8_BK, t.a_row + p.n_up, fb);
+            mbar_expect_tx(fb, (uint32_t)(I8_A_BYTES + boxes * p.bh * I8_BK));
+            i8_weights<GLU>(&amap, at, kb, t, fb);
           }
         } else {
           --ahead;
         }
         if (lead)
-          for (int b = 0; b < boxes; ++b) i8_box(at + (uint32_t)(NA * I8_A_BYTES + b * p.bh * I8_BK), &bmap, kb * I8_BK, t.x0 + b * p.bh, fb);
+          for (int b = 0; b < boxes; ++b) i8_box(at + (uint32_t)(I8_A_BYTES + b * p.bh * I8_BK), &bmap, kb * I8_BK, t.x0 + b * p.bh, fb);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
     }
@@ -249,19 +267,16 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     const uint32_t lo0 = (uint32_t)d0, hi = (uint32_t)(d0 >> 32), stage16 = (uint32_t)p.stage_bytes >> 4;
     int s = 0, buf = 0;
     uint32_t ph = 0, dph = 0;
-    if (p.passes) pdl_wait();
-    const int n = items();
-    for (int i = first; i < n; i += step) {
-      const int cols = (i8_item(p, i).rows + 15) & ~15;
-      const uint32_t idesc = i8_idesc(cols), d = tmem + (uint32_t)(buf * NA * p.tn);
+    for (int i = first; i < n_items; i += step) {
+      const int cols = (__shfl_sync(0xffffffffu, i8_item<GLU>(p, i, false).rows, 0) + 15) & ~15;
+      const uint32_t idesc = i8_idesc(cols), d = tmem + (uint32_t)(buf * p.tn);
       mbar_wait_or(drained_s + 8u * buf, dph ^ 1u, gave_up_s);
       for (int kb = kb0; kb < kb1; ++kb) {
         mbar_wait_or(full_s + 8u * s, ph, gave_up_s);
         __syncwarp();
         tc_fence_after();
-        const uint32_t a = lo0 + (uint32_t)s * stage16, b = a + (NA * I8_A_BYTES >> 4);
-        umma_i8_ss4(d, a, b, hi, idesc, kb > kb0, lead);
-        if (NA == 2) umma_i8_ss4(d + (uint32_t)p.tn, a + (I8_A_BYTES >> 4), b, hi, idesc, kb > kb0, lead);
+        const uint32_t a = lo0 + (uint32_t)s * stage16;
+        umma_i8_ss4(d, a, a + (I8_A_BYTES >> 4), hi, idesc, kb > kb0, lead);
         umma_commit(empty_s + 8u * s, lead);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
@@ -279,55 +294,64 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     int buf = 0, turn = 0;
     uint32_t aph = 0;
     pdl_wait();
-    const int n_items = items();
     for (int i = first; i < n_items; i += step) {
-      const I8Item t = i8_item(p, i);
+      const I8Item t = i8_item<GLU>(p, i, true);
       float* xs = s_scale + turn * 256;   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
       int* xr = s_row + turn * 256;
       turn ^= 1;
+      const bool down = !GLU && p.passes;   // (left to the sum over the experts: scale of the token, routing weight)
       for (int c = tid; c < p.tn; c += 32 * I8_EPI) {
-        float f = 0.f;
-        int o = t.x0 + c;
-        if (c < t.rows) {
-          f = p.q_scale[o];
-          if (p.passes && NA == 1) {
-            o = p.sorted[o];
-            f *= p.row_scale[o];
-          }
-        }
-        xs[c] = f;
-        xr[c] = o;
+        const int at = t.x0 + c;
+        xs[c] = c < t.rows && !down ? p.q_scale[at] : 1.f;
+        xr[c] = c < t.rows && down ? p.sorted[at] : at;
       }
-      const int n = t.n0 + row, rows = min(32, p.n - (t.n0 + quad));   // (of this warp's 32; not positive: none)
-      const bool live = lane < rows;
-      const float ws = live ? p.w_scale[t.a_row + row] : 0.f, wu = NA == 2 && live ? p.w_scale[t.a_row + p.n_up + row] : 0.f;
+      // this lane's row: of 128, or, gate and up, lanes 0 to 15 a gate row and lanes 16 to 31 its up row
+      const int r = GLU ? quad / 2 + (lane & 15) : row, n = t.n0 + r;
+      const bool live = n < p.n, wide = wide_y && t.n0 + quad + 32 <= p.n;
+      float ws = live ? p.w_scale[t.a_row + r + (GLU && lane >= 16 ? p.n : 0)] : 0.f;
+      if (down) ws = ws * p.w_unit[t.e] * p.unit;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
       __syncwarp();
       tc_fence_after();
       if (p.split == 1) {
-        const uint32_t d = t_lane + (uint32_t)(buf * NA * p.tn);
-        const float bias = live ? i8_bias(p, n) : 0.f;
+        const uint32_t d = t_lane + (uint32_t)(buf * p.tn);
+        const float bias = !GLU && live ? i8_bias(p, n) : 0.f;
         for (int c0 = 16 * half; c0 < t.rows; c0 += 32) {
-          uint32_t v[16], u[16];
+          uint32_t v[16];
           tmem_ld16(d + (uint32_t)c0, v);
-          if (NA == 2) tmem_ld16(d + (uint32_t)(p.tn + c0), u);
           float f[16];
           float4 x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = reinterpret_cast<const float4*>(xs + c0)[j];
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float xj = reinterpret_cast<const float*>(x)[j];
-            f[j] = (float)(int)v[j] * (xj * ws);
-            if (NA == 2) f[j] = i8_act(p.act, f[j]) * ((float)(int)u[j] * (xj * wu));
-            else f[j] += bias;
-          }
+          for (int j = 0; j < 16; ++j) f[j] = (float)(int)v[j] * (reinterpret_cast<const float*>(x)[j] * ws) + bias;
           const int count = min(16, t.rows - c0);
-          if (NA == 2 || p.dtype == DT_F32) i8_store16<float>(static_cast<float*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, false, stage);
-          else if (p.dtype == DT_F16) i8_store16<__half>(static_cast<__half*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, wide_y && rows == 32, stage);
-          else i8_store16<__nv_bfloat16>(static_cast<__nv_bfloat16*>(p.y), p.ldy, xr + c0, count, f, n, lane, rows, wide_y && rows == 32, stage);
+          if (GLU) {   // of two tokens, the lanes of the gate take the first and those of up the second
+            const bool up = lane >= 16;
+            float g[8], u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float got = __shfl_xor_sync(0xffffffffu, up ? f[2 * j] : f[2 * j + 1], 16);
+              g[j] = up ? got : f[2 * j];
+              u[j] = up ? f[2 * j + 1] : got;
+            }
+            if (p.act == 1) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) u[j] *= i8_silu(g[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) u[j] *= i8_gelu(g[j]);
+            }
+            float* y = static_cast<float*>(p.y) + (t.x0 + c0 + (up ? 1 : 0)) * p.ldy + n;
+            const int left = live ? count - (up ? 1 : 0) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (2 * j < left) y[2 * j * p.ldy] = u[j];
+          } else {
+            i8_store16(p, xr + c0, count, f, n, lane, live, wide, stage);
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -337,36 +361,56 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     }
   }
   __syncwarp();
-  if (NA == 1 && p.split > 1) {
+  if (!GLU && p.split > 1) {
     // ---------------- split: the sums of rows [per * rank, per * (rank + 1)) of the tile are this CTA's to add and store ----------------
-    cluster_sync();   // every CTA's products are complete, its ring is free: [from][token][row]
-    const I8Item t = i8_item(p, first);
-    const int per = I8_ROWS / p.split, shift = 31 - __clz(per);
-    const uint32_t ring = smem_u32(smem);
-    if (warp >= 4) {
-      const int quad = (warp & 3) * 32, row = quad + lane;
-      const uint32_t d = tmem + ((uint32_t)quad << 16);
+    // The rows of another CTA go into its ring, [sender][row][token], rows 16 bytes more than tn words apart (eight lanes' 16 bytes then
+    // lie in different banks).  A lane keeps its row to the end.
+    cluster_sync();   // every CTA's products are complete, its ring is free
+    const I8Item t = i8_item<false>(p, first, true);
+    const int per = I8_ROWS / p.split, shift = 31 - __clz(per), quad = (warp & 3) * 32, row = quad + lane, owner = row >> shift;
+    const int half = 16 * ((warp - 4) >> 2);
+    const uint32_t d = tmem + ((uint32_t)quad << 16), pitch = 4u * (uint32_t)p.tn + 16u, ring = smem_u32(smem);
+    const bool mine = owner == (int)rank;
+    if (warp >= 4 && !(p.split <= 4 && mine)) {   // (whole warps of a quad, unless 16 rows are a CTA's)
+      const uint32_t slot = rank - (owner < (int)rank ? 1u : 0u);   // (senders in order, without the owner)
       uint32_t peer;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ring + 4u * (uint32_t)((int)rank * p.tn * per + (row & (per - 1)))), "r"(row >> shift));
-      for (int c0 = 16 * ((warp - 4) >> 2); c0 < t.rows; c0 += 32) {
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ring + (slot * (uint32_t)per + (uint32_t)(row & (per - 1))) * pitch), "r"(owner));
+      for (int c0 = half; c0 < t.rows; c0 += 32) {
         uint32_t v[16];
         tmem_ld16(d + (uint32_t)c0, v);
         tmem_ld_wait();
+        if (!mine) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer + 4u * (uint32_t)((c0 + j) * per)), "r"(v[j]) : "memory");
+          for (int j = 0; j < 4; ++j)
+            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(peer + 4u * (uint32_t)(c0 + 4 * j)), "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]),
+                         "r"(v[4 * j + 3]) : "memory");
+        }
       }
     }
     cluster_sync();
-    if (warp >= 4) {
-      const int tid = threadIdx.x - 128, r = tid & (per - 1), row = (int)rank * per + r, n = t.n0 + row;
-      if (n < p.n) {
-        const float ws = p.w_scale[t.a_row + row], bias = i8_bias(p, n);
-        for (int c = tid >> shift; c < t.rows; c += 32 * I8_EPI >> shift) {
-          int sum = 0;
-#pragma unroll 4
-          for (int from = 0; from < p.split; ++from) sum += (int)lds32(ring + 4u * (uint32_t)((from * p.tn + c) * per + r));
-          i8_put(p.y, p.dtype, (int64_t)(t.x0 + c) * p.ldy + n, (float)sum * (s_scale[c] * ws) + bias);
+    if (warp >= 4 && (p.split == 8 ? quad >> 5 == (int)rank >> 1 : mine)) {
+      const int n = t.n0 + row;
+      const bool live = mine && n < p.n, wide = p.split <= 4 && p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && t.n0 + quad + 32 <= p.n;
+      const float ws = live ? p.w_scale[t.a_row + row] : 0.f, bias = live ? i8_bias(p, n) : 0.f;
+      const uint32_t from0 = ring + (uint32_t)(row & (per - 1)) * pitch;
+      for (int c0 = half; c0 < t.rows; c0 += 32) {
+        uint32_t v[16];
+        tmem_ld16(d + (uint32_t)c0, v);
+        tmem_ld_wait();
+        for (int from = 0; from < p.split - 1; ++from) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 w = lds128s(from0 + (uint32_t)(from * per) * pitch + 4u * (uint32_t)(c0 + 4 * j));
+            v[4 * j] += w.x;
+            v[4 * j + 1] += w.y;
+            v[4 * j + 2] += w.z;
+            v[4 * j + 3] += w.w;
+          }
         }
+        float f[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = (float)(int)v[j] * (s_scale[c0 + j] * ws) + bias;
+        i8_store16(p, s_row + c0, min(16, t.rows - c0), f, n, lane, live, wide, s_stage + (warp - 4) * 1024);
       }
     }
   }
@@ -390,43 +434,38 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
   if (warp == 2) tmem_dealloc(tmem, p.tmem_cols);
 }
 
-static bool i8_map(CUtensorMap& map, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows) {
+// rows of k bytes; planes > 0: as [planes][rows / planes], boxes of box_rows rows of two planes
+static bool i8_map(CUtensorMap& map, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows, int64_t planes = 0) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (!enc) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {I8_BK, (cuuint32_t)box_rows}, one[2] = {1, 1};
-  return enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const int64_t per = planes ? rows / planes : rows;
+  const cuuint64_t dims[3] = {(cuuint64_t)k, (cuuint64_t)per, (cuuint64_t)planes}, strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(per * pitch)};
+  const cuuint32_t box[3] = {I8_BK, (cuuint32_t)box_rows, 2}, one[3] = {1, 1, 1};
+  return enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NA> static int i8_launch(const CUtensorMap& amap, const CUtensorMap& bmap, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
+template <bool GLU> static int i8_launch(const CUtensorMap& amap, const CUtensorMap& bmap, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return E_CUDA;
   if (!configured[dev & 63]) {
-    if (cudaFuncSetAttribute(i8_kernel<NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
+    if (cudaFuncSetAttribute(i8_kernel<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
     configured[dev & 63] = true;
   }
-  return launch_pdl_cluster(i8_kernel<NA>, dim3((unsigned)grid), dim3(I8_THREADS), (unsigned)p.split, smem, stream, amap, bmap, p) == cudaSuccess ? E_OK : E_CUDA;
-}
-
-// Tokens of an expert's pass: its average share of the slots and three standard deviations, up to 128
-int64_t i8_moe_pass_rows(int64_t slots, int64_t experts) {
-  const double mean = (double)slots / (double)experts;
-  const int64_t rows = round_up((int64_t)(mean + 3.0 * sqrt(mean)) + 1, 16);
-  return rows <= 64 ? rows : 128;
+  return launch_pdl_cluster(i8_kernel<GLU>, dim3((unsigned)grid), dim3(I8_THREADS), (unsigned)p.split, smem, stream, amap, bmap, p) == cudaSuccess ? E_OK : E_CUDA;
 }
 
 int launch_i8_product(const I8Product& a, cudaStream_t stream) {
-  const int na = a.act ? 2 : 1;
+  const bool glu = a.act != 0;
+  const int per_tile = glu ? I8_ROWS / 2 : I8_ROWS;   // results a row tile
   I8Params p{};
   p.n = (int)a.n;
-  p.n_up = (int)a.n;
-  p.w_rows = (int)(a.n * na);
+  p.w_rows = (int)(a.n * (glu ? 2 : 1));
   p.k = (int)a.k;
   p.nk = (int)((a.k + I8_BK - 1) / I8_BK);
   p.m = (int)a.m;
-  p.rt = (int)((a.n + I8_ROWS - 1) / I8_ROWS);
+  p.rt = (int)((a.n + per_tile - 1) / per_tile);
   if (a.passes) {
     p.tn = (int)a.pass_rows;
     p.tt = 1;
@@ -435,7 +474,7 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
     p.tn = (int)round_up((a.m + p.tt - 1) / p.tt, 16);
   }
   p.bh = !a.passes || p.tn <= 64 ? p.tn : 64;
-  p.stage_bytes = na * I8_A_BYTES + p.tn * I8_BK;
+  p.stage_bytes = I8_A_BYTES + (int)round_up(p.tn, p.bh) * I8_BK;
   const int per_sm = p.tn <= 64 ? 2 : 1;
   const int64_t tiles = a.passes ? a.max_passes * p.rt : (int64_t)p.rt * p.tt;
   if (tiles > 1 << 29) return E_TOO_LARGE;
@@ -446,28 +485,28 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.stages = room / p.stage_bytes;
   if (p.stages > I8_MAX_STAGES) p.stages = I8_MAX_STAGES;
   p.aux_off = p.stages * p.stage_bytes;
-  const int cols = na * p.tn, most = 512 / per_sm;
-  p.nbuf = p.split == 1 && 2 * cols <= most ? 2 : 1;
+  p.nbuf = p.split == 1 && 2 * p.tn <= 512 / per_sm ? 2 : 1;
   p.tmem_cols = 32;
-  while ((int)p.tmem_cols < p.nbuf * cols) p.tmem_cols *= 2;
+  while ((int)p.tmem_cols < p.nbuf * p.tn) p.tmem_cols *= 2;
   p.y = a.y;
   p.ldy = a.ldy;
   p.dtype = a.dtype;
   p.w_scale = a.w_scale;
   p.q_scale = a.q_scale;
   p.bias = a.bias;
-  p.settled = a.settled;
+  p.settled = a.settled || a.passes;
   p.passes = static_cast<const int4*>(a.passes);
   p.n_passes = a.n_passes;
   p.act = a.act;
   p.sorted = a.sorted;
-  p.row_scale = a.row_scale;
+  p.w_unit = a.w_unit;
+  p.unit = a.unit;
   p.status = a.status;
   const int64_t slots = I8_SMS * per_sm, grid = p.split > 1 ? tiles * p.split : tiles < slots ? tiles : slots;
   CUtensorMap amap, bmap;
-  if (!i8_map(amap, a.w, a.k, a.experts * p.w_rows, a.ldw, I8_ROWS) || !i8_map(bmap, a.q, a.k, a.m, a.ldq, p.bh)) return E_CUDA;
+  if (!i8_map(amap, a.w, a.k, a.experts * p.w_rows, a.ldw, glu ? 16 : I8_ROWS, glu ? 2 * a.experts : 0) || !i8_map(bmap, a.q, a.k, a.m, a.ldq, p.bh)) return E_CUDA;
   const size_t smem = 1024 + (size_t)p.aux_off + I8_AUX;
-  return na == 2 ? i8_launch<2>(amap, bmap, p, (int)grid, smem, stream) : i8_launch<1>(amap, bmap, p, (int)grid, smem, stream);
+  return glu ? i8_launch<true>(amap, bmap, p, (int)grid, smem, stream) : i8_launch<false>(amap, bmap, p, (int)grid, smem, stream);
 }
 
 }  // namespace gguf_b200

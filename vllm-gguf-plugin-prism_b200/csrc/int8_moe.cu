@@ -1,0 +1,214 @@
+// The routed expert step around its products of 8-bit integers: the order of the slots, and the sum over a token's experts.
+//
+//   i8_plan_kernel  slots (token * top_k + j) sorted by expert, in their order; every expert's rows in passes of like size.  Blocks take
+//                   equal runs of slots; each counts all slots for itself (16 k of them are 64 KB, from L2), those ahead of its run apart,
+//                   and places its own: no block waits for another.  More blocks, one an expert, look for the expert's largest scale.
+//   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * factor, in fp32, rounded once
+//
+// The experts' results y = D * w_scale travel from the down product to the sum in fp16 for 16-bit tokens (fp32 for fp32): half the bytes of
+// the step's largest buffer.  They are divided by powers of two first, one above the expert's largest scale and one that brings the
+// largest |D| there can be (128 * 127 * I) to 2^15 at most, so that nothing overflows whatever the scales.  It is one rounding of at most 2^-11
+// of a result, an eighth of the sum's own for bf16, the same as the sum's own for fp16; of results below fp16's normal numbers, at
+// most I * 2^-25 of one unit of D (at the expert's largest scale).
+#include <math.h>
+
+#include "common.cuh"
+#include "int8.cuh"
+
+namespace gguf_b200 {
+
+constexpr int I8_MAX_EXPERTS = 256, I8_PLAN_BLOCKS = 32;
+
+// An expert's c rows in passes of like size: whole groups of 16 tokens but for the last, at most pass_rows
+__device__ __forceinline__ int i8_pass_size(int c, int pass_rows) {
+  const int np = (c + pass_rows - 1) / pass_rows;
+  return np > 0 ? ((c + np - 1) / np + 15) / 16 * 16 : 16;
+}
+__device__ __forceinline__ int i8_pass_count(int c, int pass_rows) {
+  const int per = i8_pass_size(c, pass_rows);
+  return (c + per - 1) / per;
+}
+
+__global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int blocks, int run) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int32_t s_cnt[32][I8_MAX_EXPERTS + 1];   // first: counts of all slots, by warp modulo 8; then a warp's slots of a step, and its first place
+  __shared__ int32_t s_before[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS];
+  __shared__ float s_top[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.experts;
+  if ((int)blockIdx.x >= blocks) {   // largest scale of an expert (a scale that is not finite: as if it were not there)
+    const int e = blockIdx.x - blocks;
+    float top = 0.f;
+    for (int64_t i = threadIdx.x; i < p.h; i += 1024) {
+      const float v = fabsf(p.w2_scale[e * p.h + i]);
+      if (v <= 3.402823466e+38f) top = fmaxf(top, v);
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    if (warp == 0) {
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s_top[lane])));
+      if (lane == 0) {
+        int x = 0;
+        frexpf(top, &x);
+        x = max(-126, min(127, x));
+        p.w_top[e] = exp2f((float)x);
+        p.w_unit[e] = exp2f((float)-x);
+      }
+    }
+    return;
+  }
+  const int slots = (int)p.slots, s0 = min(slots, (int)blockIdx.x * run), s1 = min(slots, s0 + run);
+  for (int i = threadIdx.x; i < 16 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < slots; s += 1024) {
+    const int e = p.topk_ids[s];
+    if (e >= 0 && e < E) atomicAdd(&s_cnt[(warp & 7) + (s < s0 ? 0 : 8)][e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += 1024) {
+    int before = 0, rest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      before += s_cnt[i][e];
+      rest += s_cnt[8 + i][e];
+    }
+    s_before[e] = before;
+    s_total[e] = before + rest;
+  }
+  __syncthreads();
+  if (warp == 0) {   // prefix sums over the experts: rows and passes
+    int rows = 0, ps = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane, c = e < E ? s_total[e] : 0, np = i8_pass_count(c, p.pass_rows);
+      int a = c, b = np;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, a, m), v = __shfl_up_sync(0xffffffffu, b, m);
+        if (lane >= m) { a += u; b += v; }
+      }
+      if (e < E) {
+        s_next[e] = rows + a - c + s_before[e];
+        s_pass[e] = ps + b - np;
+      }
+      rows += __shfl_sync(0xffffffffu, a, 31);
+      ps += __shfl_sync(0xffffffffu, b, 31);
+    }
+    if (lane == 0 && blockIdx.x == 0) {
+      p.n_passes[0] = ps;
+      p.n_passes[1] = rows;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = warp; e < E; e += 32) {
+      const int c = s_total[e], per = i8_pass_size(c, p.pass_rows);
+      for (int i = lane; i * per < c; i += 32) static_cast<int4*>(p.passes)[s_pass[e] + i] = make_int4(e, s_next[e] + i * per, min(per, c - i * per), 0);
+    }
+  __syncthreads();   // (s_next moves on below)
+  for (int b = s0; b < s1; b += 1024) {
+    for (int i = threadIdx.x; i < 32 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
+    __syncthreads();
+    const int s = b + threadIdx.x, e = s < s1 ? p.topk_ids[s] : -1;
+    const bool valid = e >= 0 && e < E;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (valid && lane == __ffs(same) - 1) s_cnt[warp][e] = __popc(same);
+    __syncthreads();
+    if ((int)threadIdx.x < E) {   // per expert: first place of every warp
+      int at = s_next[threadIdx.x];
+      for (int w0 = 0; w0 < 32; w0 += 8) {   // (eight loads in flight)
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = s_cnt[w0 + i][threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s_cnt[w0 + i][threadIdx.x] = at;
+          at += v[i];
+        }
+      }
+      s_next[threadIdx.x] = at;
+    }
+    __syncthreads();
+    if (s < s1) {
+      const int at = valid ? s_cnt[warp][e] + __popc(same & ((1u << lane) - 1u)) : -1;
+      if (valid) p.sorted[at] = s;
+      p.place[s] = at;
+    }
+    __syncthreads();
+  }
+}
+
+// Tokens of an expert's pass, at most 256: its average share of the slots and three standard deviations
+int64_t i8_moe_pass_rows(int64_t slots, int64_t experts) {
+  const double mean = (double)slots / (double)experts;
+  const int64_t rows = round_up((int64_t)(mean + 3.0 * sqrt(mean)) + 1, 16);
+  return rows <= 64 ? rows : rows <= 256 ? round_up(rows, 64) : 256;
+}
+int64_t i8_moe_passes(int64_t slots, int64_t experts, int64_t pass_rows) {
+  const int64_t worst = slots / pass_rows + experts;
+  return slots < worst ? slots : worst;
+}
+int launch_i8_plan(const I8Plan& a, cudaStream_t stream) {
+  if (a.experts < 1 || a.experts > I8_MAX_EXPERTS || a.slots > 1 << 24) return E_BAD_SHAPE;
+  const int64_t steps = (a.slots + 1023) / 1024, per = (steps + I8_PLAN_BLOCKS - 1) / I8_PLAN_BLOCKS;
+  const int run = (int)per * 1024, blocks = (int)((a.slots + run - 1) / run);
+  return launch_pdl(i8_plan_kernel, dim3((unsigned)(blocks + a.experts)), dim3(1024), 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
+}
+
+// Eight columns a thread.
+template <typename Y, typename T> __global__ void __launch_bounds__(256) i8_sum_kernel(const I8Sum p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int WI = sizeof(Y) / 2, WO = sizeof(T) / 2;   // 16-byte words of eight values
+  const unsigned per_row = (unsigned)(p.h / 8), top_k = (unsigned)p.top_k;
+  const unsigned total = (unsigned)p.tokens * per_row;
+  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+    const unsigned t = i / per_row, c = 8 * (i - t * per_row), slot0 = t * top_k;
+    const Y* in = static_cast<const Y*>(p.y) + (int64_t)slot0 * p.h + c;
+    float s[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = 0.f;
+    for (unsigned j0 = 0; j0 < top_k; j0 += 4, in += 4 * p.h) {   // four experts' rows in flight
+      uint4 v[4][WI];
+      float f[4];
+#pragma unroll
+      for (unsigned j = 0; j < 4; ++j) {
+        const int at = j0 + j < top_k ? __ldg(p.place + slot0 + j0 + j) : -1;
+        f[j] = 0.f;
+        if (at >= 0) {     // (a slot without a valid expert contributes nothing)
+#pragma unroll
+          for (int k = 0; k < WI; ++k) v[j][k] = reinterpret_cast<const uint4*>(in + j * p.h)[k];
+          f[j] = __ldg(p.topk_weights + slot0 + j0 + j) * __ldg(p.q_scale + at) * (__ldg(p.w_top + __ldg(p.topk_ids + slot0 + j0 + j)) * p.unit);
+        } else {
+#pragma unroll
+          for (int k = 0; k < WI; ++k) v[j][k] = make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = fmaf(to_float<Y>(reinterpret_cast<const Y*>(v[j])[k]), f[j], s[k]);
+    }
+    uint4 o[WO];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(o)[k] = from_float<T>(s[k]);
+#pragma unroll
+    for (int k = 0; k < WO; ++k) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)t * p.h + c)[k] = o[k];
+  }
+}
+
+int launch_i8_sum(const I8Sum& a, cudaStream_t stream) {
+  const int64_t total = a.tokens * (a.h / 8);
+  if (a.h % 8 != 0 || total >= (int64_t)1 << 31) return E_TOO_LARGE;
+  const dim3 grid((unsigned)((total + 255) / 256 > 148 * 8 ? 148 * 8 : (total + 255) / 256));
+  cudaError_t e;
+  switch (a.dtype) {
+    case DT_F32: e = launch_pdl(i8_sum_kernel<float, float>, grid, dim3(256), 0, stream, a); break;
+    case DT_F16: e = launch_pdl(i8_sum_kernel<__half, __half>, grid, dim3(256), 0, stream, a); break;
+    case DT_BF16: e = launch_pdl(i8_sum_kernel<__half, __nv_bfloat16>, grid, dim3(256), 0, stream, a); break;
+    default: return E_BAD_DTYPE;
+  }
+  return e == cudaSuccess ? E_OK : E_CUDA;
+}
+
+}  // namespace gguf_b200

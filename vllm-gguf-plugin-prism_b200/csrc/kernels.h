@@ -186,8 +186,7 @@ int launch_moe_plan(const int32_t* topk_ids, int64_t slots, int n_experts, int a
 // passes of `block` rows from a caller's block-aligned lists (expert ids outside [0, n_experts) and blocks beyond n_post_pad left out)
 int launch_moe_blocks(const int32_t* expert_ids, const int32_t* n_post_pad, int64_t n_sorted, int n_experts, int block, void* passes,
                       int32_t* n_passes, cudaStream_t stream);
-// (y in fp32, or in dtype)
-int launch_moe_sum(const void* y, bool y_f32, void* out, const int32_t* topk_ids, int n_experts, int64_t tokens, int64_t top_k, int64_t h,
+int launch_moe_sum(const void* y, void* out, const int32_t* topk_ids, int n_experts, int64_t tokens, int64_t top_k, int64_t h,
                    int dtype, cudaStream_t stream);
 // the router ahead of it (moe_route.cu); sizes are checked by the caller: at most ROUTE_MAX_EXPERTS, ROUTE_MAX_TOP_K, as many groups
 constexpr int ROUTE_MAX_EXPERTS = 512, ROUTE_MAX_TOP_K = 32;

@@ -151,19 +151,19 @@ int launch_moe_blocks(const int32_t* expert_ids, const int32_t* n_post_pad, int6
 
 // Eight columns per thread.  (One column per thread, with a 64-bit division for it, took 10.4 us for 256 tokens of 2048
 // columns and eight experts, 278 instructions a column; the traffic is worth 1.5 us.)
-template <typename Y, typename T>
-__global__ void __launch_bounds__(256) moe_sum_kernel(const Y* __restrict__ y, T* __restrict__ out, const int32_t* __restrict__ topk_ids,
+template <typename T>
+__global__ void __launch_bounds__(256) moe_sum_kernel(const T* __restrict__ y, T* __restrict__ out, const int32_t* __restrict__ topk_ids,
                                                       int n_experts, int64_t tokens, int top_k, int64_t h) {
   pdl_trigger();
   pdl_wait();
-  constexpr int W = sizeof(Y) / 2, WO = sizeof(T) / 2;   // 16-byte words of eight values
+  constexpr int W = sizeof(T) / 2;               // 16-byte words of eight values
   const unsigned per_row = (unsigned)(h / 8);
   const int64_t total = tokens * per_row;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const unsigned t = (unsigned)i / per_row;
     const int64_t c = 8 * (int64_t)((unsigned)i - t * per_row);
     const int32_t* ids = topk_ids + (int64_t)t * top_k;
-    const Y* in = y + (int64_t)t * top_k * h + c;
+    const T* in = y + (int64_t)t * top_k * h + c;
     float s[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[k] = 0.f;
@@ -175,41 +175,33 @@ __global__ void __launch_bounds__(256) moe_sum_kernel(const Y* __restrict__ y, T
 #pragma unroll
       for (int k = 0; k < W; ++k) v[k] = reinterpret_cast<const uint4*>(in)[k];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] += to_float<Y>(reinterpret_cast<const Y*>(v)[k]);
+      for (int k = 0; k < 8; ++k) s[k] += to_float<T>(reinterpret_cast<const T*>(v)[k]);
     }
-    uint4 o[WO];
+    uint4 o[W];
 #pragma unroll
     for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(o)[k] = from_float<T>(s[k]);
 #pragma unroll
-    for (int k = 0; k < WO; ++k) reinterpret_cast<uint4*>(out + (int64_t)t * h + c)[k] = o[k];
+    for (int k = 0; k < W; ++k) reinterpret_cast<uint4*>(out + (int64_t)t * h + c)[k] = o[k];
   }
 }
 
-template <typename Y, typename T>
-static cudaError_t moe_sum_launch(const void* y, void* out, const int32_t* topk_ids, int n_experts, int64_t tokens, int64_t top_k, int64_t h,
-                                  cudaStream_t stream) {
-  const int64_t total = tokens * (h / 8);
-  const unsigned grid = (unsigned)((total + 255) / 256 > 148 * 8 ? 148 * 8 : (total + 255) / 256);
-  return launch_pdl(moe_sum_kernel<Y, T>, dim3(grid), dim3(256), 0, stream, static_cast<const Y*>(y), static_cast<T*>(out), topk_ids, n_experts, tokens,
-                    (int)top_k, h);
-}
-int launch_moe_sum(const void* y, bool y_f32, void* out, const int32_t* topk_ids, int n_experts, int64_t tokens, int64_t top_k, int64_t h,
+int launch_moe_sum(const void* y, void* out, const int32_t* topk_ids, int n_experts, int64_t tokens, int64_t top_k, int64_t h,
                    int dtype, cudaStream_t stream) {
   if (h % 8 != 0) return E_BAD_SHAPE;
-  if (tokens * (h / 8) == 0) return E_OK;
-  if (tokens * (h / 8) >= (int64_t)1 << 32) return E_TOO_LARGE;
+  const int64_t total = tokens * (h / 8);
+  if (total == 0) return E_OK;
+  if (total >= (int64_t)1 << 32) return E_TOO_LARGE;
+  const unsigned grid = (unsigned)((total + 255) / 256 > 148 * 8 ? 148 * 8 : (total + 255) / 256);
   cudaError_t e;
   switch (dtype) {
     case DT_F32:
-      e = moe_sum_launch<float, float>(y, out, topk_ids, n_experts, tokens, top_k, h, stream);
+      e = launch_pdl(moe_sum_kernel<float>, dim3(grid), dim3(256), 0, stream, (const float*)y, (float*)out, topk_ids, n_experts, tokens, (int)top_k, h);
       break;
     case DT_F16:
-      e = y_f32 ? moe_sum_launch<float, __half>(y, out, topk_ids, n_experts, tokens, top_k, h, stream)
-                : moe_sum_launch<__half, __half>(y, out, topk_ids, n_experts, tokens, top_k, h, stream);
+      e = launch_pdl(moe_sum_kernel<__half>, dim3(grid), dim3(256), 0, stream, (const __half*)y, (__half*)out, topk_ids, n_experts, tokens, (int)top_k, h);
       break;
     case DT_BF16:
-      e = y_f32 ? moe_sum_launch<float, __nv_bfloat16>(y, out, topk_ids, n_experts, tokens, top_k, h, stream)
-                : moe_sum_launch<__nv_bfloat16, __nv_bfloat16>(y, out, topk_ids, n_experts, tokens, top_k, h, stream);
+      e = launch_pdl(moe_sum_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, stream, (const __nv_bfloat16*)y, (__nv_bfloat16*)out, topk_ids, n_experts, tokens, (int)top_k, h);
       break;
     default:
       return E_BAD_DTYPE;
