@@ -1,5 +1,7 @@
 """The expert router against its definition in 64 bits.  Ids are compared for equality; a weight is computed in fp64 and rounded to
-fp32 once (2^-24 of itself; 2^-23 is asked, for the fp64 steps before it)."""
+fp32 once (2^-24 of itself; 2^-23 is asked, for the fp64 steps before it).  The sum of a softmax that the weights are not divided
+by again is one of fp32 exponentials: an argument x - max rounded to 2^-24 of itself (at most 2^-24 * |d| e^-|d| of the sum, below
+2^-25) and 2 units in the last place of the function, 2^-22: 2^-21 more is asked."""
 import ctypes
 
 import pytest
@@ -47,11 +49,11 @@ def route(logits, top_k, scoring="softmax", bias=None, n_group=1, topk_group=1, 
     return torch.tensor(weights, dtype=torch.float64), torch.tensor(ids, dtype=torch.int32)
 
 
-def check(got, want):
+def check(got, want, summed=False):
     w, ids = got
     assert w.dtype == torch.float32 and ids.dtype == torch.int32 and w.is_contiguous() and ids.is_contiguous()
     assert torch.equal(ids.cpu(), want[1])
-    assert bool(((w.cpu().double() - want[0]).abs() <= 2.0 ** -23 * want[0].abs() + 2.0 ** -149).all())
+    assert bool(((w.cpu().double() - want[0]).abs() <= (2.0 ** -23 + (2.0 ** -21 if summed else 0)) * want[0].abs() + 2.0 ** -149).all())
 
 
 @pytest.mark.gpu
@@ -66,7 +68,7 @@ def test_route(ops, dtype, t, e, k, groups, topk_group, scoring, with_bias):
     bias = torch.randn(e, device="cuda", generator=gen) * 0.2 if with_bias else None
     for renormalize, scale in ((True, 1.0), (False, 2.5)):
         kw = dict(scoring=scoring, bias=bias, n_group=groups, topk_group=topk_group, renormalize=renormalize, scale=scale)
-        check(ops.moe_route(logits, k, **kw), route(logits, k, **kw))
+        check(ops.moe_route(logits, k, **kw), route(logits, k, **kw), scoring == "softmax" and not renormalize)
 
 
 @pytest.mark.gpu
@@ -96,7 +98,7 @@ def test_route_ties_masks_and_extremes(ops, scoring, with_bias, groups):
     for topk_group in range(max(1, -(-k * groups // e)), groups + 1):
         for renormalize in (True, False):
             kw = dict(scoring=scoring, bias=bias, n_group=groups, topk_group=topk_group, renormalize=renormalize)
-            check(ops.moe_route(logits, k, **kw), route(logits, k, **kw))
+            check(ops.moe_route(logits, k, **kw), route(logits, k, **kw), scoring == "softmax" and not renormalize)
 
 
 @pytest.mark.gpu

@@ -162,7 +162,7 @@ template <typename Y, typename T> __global__ void __launch_bounds__(256) i8_sum_
   constexpr int WI = sizeof(Y) / 2, WO = sizeof(T) / 2;   // 16-byte words of eight values
   const unsigned per_row = (unsigned)(p.h / 8), top_k = (unsigned)p.top_k;
   const unsigned total = (unsigned)p.tokens * per_row;
-  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+  if (const unsigned i = blockIdx.x * 256 + threadIdx.x; i < total) {
     const unsigned t = i / per_row, c = 8 * (i - t * per_row), slot0 = t * top_k;
     const Y* in = static_cast<const Y*>(p.y) + (int64_t)slot0 * p.h + c;
     float s[8];
@@ -200,7 +200,7 @@ template <typename Y, typename T> __global__ void __launch_bounds__(256) i8_sum_
 int launch_i8_sum(const I8Sum& a, cudaStream_t stream) {
   const int64_t total = a.tokens * (a.h / 8);
   if (a.h % 8 != 0 || total >= (int64_t)1 << 31) return E_TOO_LARGE;
-  const dim3 grid((unsigned)((total + 255) / 256 > 148 * 8 ? 148 * 8 : (total + 255) / 256));
+  const dim3 grid((unsigned)((total + 255) / 256));
   cudaError_t e;
   switch (a.dtype) {
     case DT_F32: e = launch_pdl(i8_sum_kernel<float, float>, grid, dim3(256), 0, stream, a); break;

@@ -168,6 +168,7 @@ template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quant
 }
 template <typename T, bool VEC> static cudaError_t i8_quantize_rows(const I8Quantize& a, cudaStream_t stream) {
   if (a.k <= 32 * I8Q_UNIT) return i8_quantize_form<T, VEC, 32, 1>(a, stream);
+  if (a.k <= 64 * I8Q_UNIT) return i8_quantize_form<T, VEC, 64, 1>(a, stream);
   if (a.k <= 128 * I8Q_UNIT) return i8_quantize_form<T, VEC, 128, 1>(a, stream);
   if (a.k <= 256 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 1>(a, stream);
   if (a.k <= 512 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 2>(a, stream);
