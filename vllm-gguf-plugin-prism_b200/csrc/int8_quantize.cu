@@ -1,9 +1,11 @@
 // Rows of floats to 8-bit integers with one scale a row:  a = max |x|,  scale = a / 127,  code = x * 127 / a, halves to even.
 // The same kernel serves a token's activations, an expert's hidden rows and, once, a weight matrix.
 //
-// The codes are those of exact arithmetic.  x * (127 / a) with the quotient in fp32 is off by less than 2^-17; within 2^-14 of a half
-// the side is settled exactly (i8q_codes).  16-bit inputs hit halves all the time (x = a / 2 is code 63.5).  A row with an infinity or a NaN has no scale: it gets NaN for one and codes of 0,
-// so that every result it enters is NaN.
+// The codes are those of exact arithmetic.  16-bit values: y = 127 x is exact in fp32, and a quotient y / a that is not a half is off by 2^-19 of
+// itself at least (y has 18 bits, a 11), so the quotient with one correction step, right to 2^-23 and exact where it is a half, settles
+// it; halves are common (x = a / 2 is code 63.5; of bf16 values one in three hundred).  fp32 values: within 2^-14 of a half the side is
+// settled by exact products (i8q_exact).  A row with an infinity or a NaN has no scale: it gets NaN for one and codes of 0, so that every
+// result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once (copies of it as often as asked).
 #include "common.cuh"
@@ -37,46 +39,62 @@ template <typename T> __device__ __forceinline__ uint32_t i8q_top_bits(uint32_t 
   const unsigned short b = (unsigned short)max(top & 0xffffu, top >> 16);
   return __float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&b))) & 0x7fffffffu;
 }
-// Four codes, a byte each.  1.5 * 2^23 added in one fused step rounds x / scale to an integer in the low bits; what was rounded away says
-// whether a half is near, which is settled exactly: the sign of 254 |x| - (2 m + 1) a, m + 1/2 being the half, from two products and
-// their rounding errors (the products are within a few ulp of one another, so their difference is exact).
-__device__ __forceinline__ uint32_t i8q_codes(const float (&x)[4], float inv, float a) {
-  constexpr float MAGIC = 12582912.f;
-  float r[4], off = 0.f;
+__device__ __forceinline__ uint32_t i8q_pack(float r0, float r1, float r2, float r3) {   // the lowest bytes
+  return __byte_perm(__byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x0040), __byte_perm(__float_as_uint(r2), __float_as_uint(r3), 0x0040), 0x5410);
+}
+constexpr float I8Q_MAGIC = 12582912.f;   // 1.5 * 2^23: added to a small number, it leaves its integer in the low bits
+// The code of u = |x| (a lifted into fp32's middle): m or m + 1 by the sign of 254 u - (2 m + 1) a, from two products and their rounding
+// errors (the products are within a few ulp of one another where it matters, so their difference is exact).
+__device__ __forceinline__ float i8q_exact(float x, float inv, float a) {
+  const float u = fabsf(x), t = u * inv, m = floorf(t);
+  float c = rintf(t);
+  if (fabsf(t - m - 0.5f) < 0x1p-13f) {
+    const float h = 2.f * m + 1.f, p = 254.f * u, q = h * a;
+    const float d = (p - q) + (fmaf(254.f, u, -p) - fmaf(h, a, -q));
+    c = d > 0.f || (d == 0.f && ((int)m & 1)) ? m + 1.f : m;
+  }
+  return I8Q_MAGIC + copysignf(c, x);
+}
+// (one copy of the code that is hardly ever run: unrolled into every group of four, fetching it cost more than running it)
+__device__ __noinline__ uint32_t i8q_exact4(float x0, float x1, float x2, float x3, float lift, float inv, float a) {
+  return i8q_pack(i8q_exact(x0 * lift, inv, a), i8q_exact(x1 * lift, inv, a), i8q_exact(x2 * lift, inv, a), i8q_exact(x3 * lift, inv, a));
+}
+// What the codes of a row go by; a is lifted (by a power of two, exactly) so that 127 / a and 254 a stay in range
+struct I8Row {
+  float a, inv, r, lift, y;   // 127 / a, 1 / a, 127 * lift
+};
+__device__ __forceinline__ I8Row i8q_row(float a) {
+  I8Row w;
+  w.lift = a < 0x1p-90f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
+  w.a = a * w.lift;
+  w.inv = 127.f / w.a;
+  w.r = 1.f / w.a;
+  w.y = 127.f * w.lift;
+  return w;
+}
+// Sixteen codes, a byte each.  The number 1.5 * 2^23 added to a quotient rounds it to an integer; for fp32 in one fused step with the
+// product, and what was rounded away says whether a half is near.
+template <typename T> __device__ __forceinline__ uint4 i8q_unit(const T (&v)[I8Q_UNIT], const I8Row& p) {
+  uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    r[i] = fmaf(x[i], inv, MAGIC);
-    off = fmaxf(off, fabsf(fmaf(x[i], inv, MAGIC - r[i])));
-  }
-  if (off > 0.5f - 0x1p-14f) {
+    float x[4], r[4];
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = fabsf(x[i]), t = u * inv, m = floorf(t);
-      if (fabsf(t - m - 0.5f) < 0x1p-13f) {
-        const float h = 2.f * m + 1.f, p = 254.f * u, q = h * a;
-        const float d = (p - q) + (fmaf(254.f, u, -p) - fmaf(h, a, -q));
-        const float c = d > 0.f || (d == 0.f && ((int)m & 1)) ? m + 1.f : m;
-        r[i] = MAGIC + copysignf(c, x[i]);
+      for (int j = 0; j < 4; ++j) {
+        const float y = to_float<T>(v[4 * i + j]) * p.y, q = y * p.r;
+        r[j] = fmaf(fmaf(-q, p.a, y), p.r, q) + I8Q_MAGIC;
       }
-    }
-  }
-  const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);
-  return __byte_perm(lo, hi, 0x5410);
-}
-// Sixteen codes; lift is 1 but for rows whose largest value is near the ends of fp32's range
-template <typename T> __device__ __forceinline__ uint4 i8q_unit(const T (&v)[I8Q_UNIT], float lift, float inv, float a) {
-  uint32_t w[4];
-  if (lift == 1.f) {
+      w[i] = i8q_pack(r[0], r[1], r[2], r[3]);
+    } else {
+      float off = p.lift == 1.f ? 0.f : 1.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x[4] = {to_float<T>(v[4 * i]), to_float<T>(v[4 * i + 1]), to_float<T>(v[4 * i + 2]), to_float<T>(v[4 * i + 3])};
-      w[i] = i8q_codes(x, inv, a);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x[4] = {to_float<T>(v[4 * i]) * lift, to_float<T>(v[4 * i + 1]) * lift, to_float<T>(v[4 * i + 2]) * lift, to_float<T>(v[4 * i + 3]) * lift};
-      w[i] = i8q_codes(x, inv, a);
+      for (int j = 0; j < 4; ++j) {
+        x[j] = to_float<T>(v[4 * i + j]);
+        r[j] = fmaf(x[j], p.inv, I8Q_MAGIC);
+        off = fmaxf(off, fabsf(fmaf(x[j], p.inv, I8Q_MAGIC - r[j])));
+      }
+      w[i] = off > 0.5f - 0x1p-14f ? i8q_exact4(x[0], x[1], x[2], x[3], p.lift, p.inv, p.a) : i8q_pack(r[0], r[1], r[2], r[3]);
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -96,7 +114,8 @@ __device__ __forceinline__ void i8q_store(uint4 c, int8_t* __restrict__ q, int64
 // beyond is read again
 template <typename T, bool VEC, int LANES, int HOLD>
 __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD * sizeof(T) <= 8 ? 4 : 2) : 2) i8_quantize_kernel(const I8Quantize p) {
-  __shared__ uint32_t s_top[8];
+  __shared__ uint32_t s_top[2][8];
+  int turn = 0;
   const int lane = threadIdx.x % LANES;
   pdl_wait();
   pdl_trigger();
@@ -123,21 +142,22 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD *
     }
     top = __reduce_max_sync(0xffffffffu, i8q_top_bits<T>(top));
     if (LANES > 32) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+      uint32_t* st = s_top[turn];   // (in turn: whoever has passed this barrier is done with the last row's)
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) st[threadIdx.x >> 5] = top;
       __syncthreads();
       const int w0 = (int)threadIdx.x / LANES * (LANES / 32);
-      top = s_top[w0];
+      top = st[w0];
 #pragma unroll
-      for (int i = 1; i < LANES / 32; ++i) top = max(top, s_top[w0 + i]);
+      for (int i = 1; i < LANES / 32; ++i) top = max(top, st[w0 + i]);
     }
-    const bool finite = top < 0x7f800000u;
-    const float a0 = __uint_as_float(top), lift = a0 < 0x1p-90f ? 0x1p64f : a0 > 0x1p100f ? 0x1p-64f : 1.f;   // (so that 127 / a and 254 a stay in range)
-    const float a = a0 * lift, inv = finite && top != 0 ? 127.f / a : 0.f, scale = finite ? a0 / 127.f : __uint_as_float(0x7fc00000u);
+    const bool finite = top < 0x7f800000u, zero = !finite || top == 0;
+    const float a = __uint_as_float(top), scale = finite ? a / 127.f : __uint_as_float(0x7fc00000u);
+    const I8Row w = i8q_row(zero ? 1.f : a);
     const int copies = p.scatter ? p.copies : 1;
     uint4 c[HOLD];
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) c[h] = finite ? i8q_unit<T>(v[h], lift, inv, a) : make_uint4(0, 0, 0, 0);
+    for (int h = 0; h < HOLD; ++h) c[h] = zero ? make_uint4(0, 0, 0, 0) : i8q_unit<T>(v[h], w);
 #pragma unroll 4
     for (int j = 0; j < copies; ++j) {
       const int64_t o = !live ? -1 : p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
@@ -152,10 +172,10 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD *
     for (int64_t at = (int64_t)(HOLD * LANES + lane) * I8Q_UNIT; at < k; at += LANES * I8Q_UNIT) {
       T u[I8Q_UNIT];
       i8q_load<T, VEC>(x, k, at, u);
-      const uint4 w = finite ? i8q_unit<T>(u, lift, inv, a) : make_uint4(0, 0, 0, 0);
+      const uint4 c = zero ? make_uint4(0, 0, 0, 0) : i8q_unit<T>(u, w);
       for (int j = 0; j < copies; ++j) {
         const int64_t o = p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
-        if (o >= 0) i8q_store(w, p.q + o * p.ldq, k, at);
+        if (o >= 0) i8q_store(c, p.q + o * p.ldq, k, at);
       }
     }
   }
@@ -166,13 +186,14 @@ template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quant
   const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 64;
   return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
 }
+// Two units a thread where there are rows enough to fill the GPU; a block a row where there are not.
 template <typename T, bool VEC> static cudaError_t i8_quantize_rows(const I8Quantize& a, cudaStream_t stream) {
-  if (a.k <= 32 * I8Q_UNIT) return i8_quantize_form<T, VEC, 32, 1>(a, stream);
-  if (a.k <= 64 * I8Q_UNIT) return i8_quantize_form<T, VEC, 64, 1>(a, stream);
-  if (a.k <= 128 * I8Q_UNIT) return i8_quantize_form<T, VEC, 128, 1>(a, stream);
-  if (a.k <= 256 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 1>(a, stream);
-  if (a.k <= 512 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 2>(a, stream);
-  return i8_quantize_form<T, VEC, 256, 4>(a, stream);
+  if (a.k > 512 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 4>(a, stream);
+  if (a.k > 256 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 2>(a, stream);
+  if (a.rows < 148 * 4) return i8_quantize_form<T, VEC, 256, 1>(a, stream);
+  if (a.k > 128 * I8Q_UNIT) return i8_quantize_form<T, VEC, 128, 2>(a, stream);
+  if (a.k > 64 * I8Q_UNIT) return i8_quantize_form<T, VEC, 64, 2>(a, stream);
+  return i8_quantize_form<T, VEC, 32, 2>(a, stream);
 }
 template <typename T> static int i8_quantize_typed(const I8Quantize& a, cudaStream_t stream) {
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx * (int64_t)sizeof(T) % 16 == 0;

@@ -1,16 +1,19 @@
 // The router of a mixture of experts: logits -> ids and weights of the top_k experts of every token.
 //
-//   s = softmax or sigmoid of the row's logits (fp64 where a choice hangs on it); an expert whose logit is -inf or NaN is masked
+//   s = softmax or sigmoid of the row's logits (fp64 where a choice hangs on it, fp32 in the weights); an expert whose logit is -inf or NaN is masked
 //   choice = s + bias; without a bias the order of s is the order of the logits, which are compared as they are
 //   groups: only the experts of the topk_group best groups remain, by the sum of a group's two best choices (with a bias) or by
 //   its best one (without)
 //   the top_k best remaining, the best first, equals by the lower index; weight = s, divided by their sum, times scale
 //   a place for which nothing is left: id -1, weight 0
 //
-// One warp a token, expert 32 j + l in lane l.  A choice becomes an unsigned key of the same order, 0 for "out", and the maximum
-// over the warp is a hardware reduction.  Choices by scores are made in fp32 first, with an error bound: where two of them that decide
-// about something are nearer than that (one row in a thousand), the row is done again in fp64.  (8192 tokens, 256 experts in eight
-// groups: 45 us with all scores in fp64.)
+// One warp a token, expert 32 j + l in lane l.  A choice becomes an unsigned key of the same order, and the maximum over the warp is a
+// hardware reduction.  In the first pass a key is 32 bits, the lowest of which say which of a lane's experts it is; where what is left of the
+// numbers (in fp32, scores with an error bound) does not settle an order that matters, the row is done again with 64-bit keys: of
+// scores about one row in a thousand, of fp32 logits those with equals.
+//
+// Bound by the integer pipe, which runs at half the issue rate: 8192 tokens, 256 experts in eight groups with a bias, took 45 us with
+// 64-bit keys throughout and 24 with keys that kept 0 for "out", exact maxima for every row and fp64 in the weights.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -25,21 +28,23 @@ struct RouteParams {
   int64_t tokens;
   int experts, top_k, groups, topk_group, sigmoid, renormalize;
   float scale;
+  int per, group_of;   // experts a group; (e * group_of) >> 20 is e's group (e < 512: off by less than 2^-11 from e / per)
 };
 
-// keys of the same order as the numbers they come from; 0 is below all of them
+// Keys of the same order as the numbers they come from (no NaN).  Those of -infinity, and 0, are below ROUTE_LEAST: "out".
+constexpr uint32_t ROUTE_LEAST = 0x00800000u;
 __device__ __forceinline__ uint32_t route_key(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return v == -INFINITY || v != v ? 0u : v == 0.f ? 0x80000000u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  const uint32_t b = __float_as_uint(v + 0.f);   // (zeros of both signs are equal)
+  return b ^ (uint32_t)((int)b >> 31 | (int)0x80000000);
 }
-__device__ __forceinline__ uint64_t route_key(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
-  return v == -INFINITY || v != v ? 0ull : v == 0.0 ? 1ull << 63 : (b >> 63) ? ~b : b | (1ull << 63);
+__device__ __forceinline__ uint64_t route_key(double v) {   // (and 0 for -infinity and NaN)
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+  return v > -INFINITY ? b ^ (uint64_t)((long long)b >> 63 | (long long)(1ull << 63)) : 0ull;
 }
-__device__ __forceinline__ float route_value(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
-__device__ __forceinline__ double route_value(uint64_t key) {
-  return __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key));
-}
+__device__ __forceinline__ float route_value(uint32_t key) { return __uint_as_float(key ^ (uint32_t)(~((int)key >> 31) | (int)0x80000000)); }
+__device__ __forceinline__ double route_value(uint64_t key) { return __longlong_as_double((long long)(key ^ (uint64_t)(~((long long)key >> 63) | (long long)(1ull << 63)))); }
+__device__ __forceinline__ bool route_out(uint32_t key) { return key < ROUTE_LEAST; }
+__device__ __forceinline__ bool route_out(uint64_t key) { return key == 0; }
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
   const uint32_t hi = warp_max((uint32_t)(v >> 32));
@@ -50,106 +55,124 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
-// Whether a choice `a` is above another, `b`, for certain.  An fp32 score (at most 1) is off by less than 2^-19: the approximate
-// exponential by (|x| + 2) 2^-23 of itself, which the score's derivative brings below 2^-22; a softmax' sum of up to 512 terms by 21 roundings of
-// 2^-24; the quotient by 2^-22.  The sum with the bias adds 2^-24 of itself, a sum of two choices twice all that.  (NaN: not certain.)
-__device__ __forceinline__ bool route_above(float a, float b, float times) { return a - b > times * (0x1p-18f + 0x1p-22f * (fabsf(a) + fabsf(b))); }
+__device__ __forceinline__ float route_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+  return r;
+}
+__device__ __forceinline__ float route_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Whether a choice `a` is above another, `b`, for certain.  off: what two scores can be off by together.  e^x above is off by (|x| + 2) 2^-23 of
+// itself; a sigmoid by s (1 - s) times that, at most 2^-23, and 2^-24 + 2^-23 for the sum and the reciprocal: two of them by less than 2^-20.
+// A softmax' sum of up to 512 terms adds 21 roundings of 2^-24: two by less than 2^-18.  The sum with the bias is rounded by 2^-24 of
+// itself, and a key leaves out less than V 2^-23 of it; a sum of two choices is off by twice all that.  (NaN: not certain.)
+template <int V> __device__ __forceinline__ bool route_above(float a, float b, float off) {
+  return a - b > off * (1.f + (float)(V + 1) * 0x1p-3f * (fabsf(a) + fabsf(b)));   // ((V + 1) 2^-23 (|a| + |b|), off being 2^-20 at least)
+}
 
-// Keys of a token's experts -> lane i's id is the i-th choice, -1 where there is none.  False: the fp32 choices do not settle it.
+// The groups that remain, a bit each.  sure: false where the order of two groups that decides is not certain.
 template <typename Key, int V, bool SCORES>
-__device__ __forceinline__ bool route_choose(const RouteParams& p, Key (&key)[V], int lane, int& id) {
-  constexpr bool CHECK = SCORES && sizeof(Key) == 4;
-  bool sure = true;
-  if (p.groups > 1) {
-    const int per = p.experts / p.groups;
-    const float inv_per = 1.f / (float)per;
-    int group[V];
+__device__ __forceinline__ uint32_t route_groups(const RouteParams& p, const Key (&key)[V], int lane, float off, bool& sure) {
+  Key mine = 0;   // lane g: score of group g
+  auto close = [&](int g, Key a, Key b) {   // a, b: this lane's two best of group g
+    const Key best = warp_max(a);
+    Key score = best;
+    if constexpr (SCORES) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
+      const Key second = warp_max(lane == owner ? b : a);
+      if (!route_out(second)) score = route_key(route_value(best) + route_value(second));
+    }
+    if (lane == g) mine = route_out(best) ? 0 : score;
+  };
+  if (p.per % 32 == 0) {   // a group is whole registers
+    const int n = p.per / 32;
+    Key a = 0, b = 0;
+    int left = n, g = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) group[j] = (int)(((float)(32 * j + lane) + 0.5f) * inv_per);
-    Key mine = 0;   // lane g: score of group g
-    auto close = [&](int g, Key a, Key b) {   // a, b: this lane's two best of group g
-      const Key best = warp_max(a);
-      Key score = best;
-      if constexpr (SCORES) {
-        const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
-        const Key second = warp_max(lane == owner ? b : a);
-        if (second != 0) score = route_key(route_value(best) + route_value(second));
+    for (int j = 0; j < V; ++j) {
+      b = max(b, min(a, key[j]));
+      a = max(a, key[j]);
+      if (--left == 0) {
+        if (g < p.groups) close(g, a, b);
+        a = b = 0;
+        left = n;
+        ++g;
       }
-      if (lane == g) mine = score;
-    };
-    if (per % 32 == 0) {   // a group is whole registers
+    }
+  } else {
+#pragma unroll 1
+    for (int g = 0; g < p.groups; ++g) {
       Key a = 0, b = 0;
-      int left = per / 32, g = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        b = max(b, min(a, key[j]));
-        a = max(a, key[j]);
-        if (--left == 0) {
-          if (g < p.groups) close(g, a, b);
-          a = b = 0;
-          left = per / 32;
-          ++g;
-        }
+        const Key x = (32 * j + lane) * p.group_of >> 20 == g ? key[j] : Key(0);
+        b = max(b, min(a, x));
+        a = max(a, x);
       }
-    } else {
-      for (int g = 0; g < p.groups; ++g) {
-        Key a = 0, b = 0;
+      close(g, a, b);
+    }
+  }
+  // (a group without an expert is picked when nothing else is left, which changes nothing)
+  uint32_t taken = 0;
+  Key last = 0;
+#pragma unroll 1
+  for (int i = 0; i < p.topk_group; ++i) {
+    last = warp_max(mine);
+    const int g = __ffs(__ballot_sync(0xffffffffu, mine == last && lane < p.groups && !(taken >> lane & 1u))) - 1;
+    taken |= 1u << g;
+    if (lane == g) mine = 0;
+  }
+  if constexpr (sizeof(Key) == 4) {
+    const Key next = warp_max(mine);
+    sure = next == 0 || (SCORES ? route_above<V>(route_value(last), route_value(next), 2.f * off) : (last / V) > (next / V));   // (equal up to the index)
+  }
+  return taken;
+}
+template <typename Key, int V> __device__ __forceinline__ void route_keep(const RouteParams& p, Key (&key)[V], int lane, uint32_t taken) {
+  if (p.per % 32 == 0) {
+    const int n = p.per / 32;
+    int left = n;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const Key x = group[j] == g ? key[j] : Key(0);
-          b = max(b, min(a, x));
-          a = max(a, x);
-        }
-        close(g, a, b);
+    for (int j = 0; j < V; ++j) {
+      if (!(taken & 1u)) key[j] = 0;
+      if (--left == 0) {
+        left = n;
+        taken >>= 1;
       }
     }
-    // (a group without an expert is picked when nothing else is left, which changes nothing)
-    uint32_t taken = 0;
-    Key last = 0;
-    for (int i = 0; i < p.topk_group; ++i) {
-      last = warp_max(mine);
-      const int g = __ffs(__ballot_sync(0xffffffffu, mine == last && lane < p.groups && !(taken >> lane & 1u))) - 1;
-      taken |= 1u << g;
-      if (lane == g) mine = 0;
-    }
-    if (CHECK) {
-      const Key next = warp_max(mine);
-      sure = next == 0 || route_above((float)route_value(last), (float)route_value(next), 2.f);
-    }
+  } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (!(taken >> (group[j] & 31) & 1u)) key[j] = 0;   // (places behind the last expert are out already)
+      if (!(taken >> ((32 * j + lane) * p.group_of >> 20 & 31) & 1u)) key[j] = 0;   // (places behind the last expert are out already)
   }
-  Key a = 0;
-  int at = 0;
-  auto nearest = [&] {
-    a = 0;
+}
+
+// 64-bit keys (exact, equals by the lower index) -> lane i's id is the i-th choice, -1 where there is none
+template <int V, bool SCORES> __device__ __forceinline__ int route_exact(const RouteParams& p, uint64_t (&key)[V], int lane) {
+  if (p.groups > 1) {
+    bool sure;
+    route_keep<uint64_t, V>(p, key, lane, route_groups<uint64_t, V, SCORES>(p, key, lane, 0.f, sure));
+  }
+  int id = -1;
+#pragma unroll 1
+  for (int i = 0; i < p.top_k; ++i) {
+    uint64_t a = 0;
+    int at = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (key[j] > a) { a = key[j]; at = j; }
-  };
-  nearest();
-  id = -1;
-  Key before = 0;
-  for (int i = 0; i < p.top_k + (CHECK ? 1 : 0); ++i) {
-    const Key best = warp_max(a);
+    const uint64_t best = warp_max(a);
     if (best == 0) break;
-    if (CHECK) {
-      if (i > 0) sure = sure && route_above((float)route_value(before), (float)route_value(best), 1.f);
-      before = best;
-      if (i == p.top_k) break;
-    }
     const int e = (int)__reduce_min_sync(0xffffffffu, a == best ? (unsigned)(32 * at + lane) : 0xffffffffu);
     if (lane == i) id = e;
-    if (lane == (e & 31)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (32 * j + lane == e) key[j] = 0;
-      nearest();
-    }
-    __syncwarp();
+    for (int j = 0; j < V; ++j)
+      if (32 * j + lane == e) key[j] = 0;
   }
-  return sure;
+  return id;
 }
 
 // SCORES: choices are scores and a bias; without, the logits themselves are compared
@@ -160,83 +183,140 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
   for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); t < p.tokens; t += (int64_t)gridDim.x * 4) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    auto logit = [&](int e) {
-      const float v = to_float<T>(row[e]);
-      return v != v ? -INFINITY : fminf(v, 3.402823466e+38f);
-    };
+    auto least = [](float v) { return fmaxf(v, -INFINITY); };              // (a NaN becomes -infinity)
+    auto most = [](float v) { return fminf(v, 3.402823466e+38f); };
     float x[V];
-    uint32_t key[V];
+    uint32_t key[V];   // V is a power of two: the lowest bits hold V - 1 - j
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int e = 32 * j + lane;
-      x[j] = e < p.experts ? logit(e) : -INFINITY;
+      x[j] = e < p.experts ? least(to_float<T>(row[e])) : -INFINITY;
     }
-    float high = 0.f;
-    if (!p.sigmoid) {
+    // A softmax: the largest logit and the sum, where they are needed.  (Weights that are divided by their own sum, of experts chosen by
+    // their logits, go by the first choice.)
+    float high = 0.f, total = 0.f;
+    if (!p.sigmoid && (SCORES || !p.renormalize)) {
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) top = max(top, route_key(x[j]));
+      for (int j = 0; j < V; ++j) {
+        x[j] = most(x[j]);
+        top = max(top, route_key(x[j]));
+      }
       top = warp_max(top);
-      if (top != 0) high = route_value(top);
-    }
-    double total = 0.0;   // of a softmax; 0 where the weights are divided by their own sum
-    if (!p.sigmoid && !p.renormalize) {   // (terms off by 2^-21 of themselves at most)
+      if (!route_out(top)) high = route_value(top);
+      if (!p.renormalize) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) total += (double)expf(x[j] - high);
-      total = warp_sum(total);
+        for (int j = 0; j < V; ++j) total += expf(x[j] - high);
+        total = warp_sum(total);
+      }
     }
-    int id;
-    bool sure;
     if constexpr (SCORES) {
-      float e[V], sum = 1.f;
-      if (!p.sigmoid) {
-        sum = 0.f;
+      float s[V];
+      if (p.sigmoid) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          e[j] = __expf(x[j] - high);
-          sum += e[j];
+          x[j] = most(x[j]);
+          s[j] = route_rcp(1.f + route_exp(-x[j]));
         }
-        sum = __frcp_rn(fmaxf(warp_sum(sum), 1e-30f));
+      } else {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s[j] = route_exp(x[j] - high);
+          sum += s[j];
+        }
+        sum = route_rcp(fmaxf(warp_sum(sum), 1e-30f));
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] *= sum;
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float s = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-x[j])) : e[j] * sum;
-        key[j] = x[j] == -INFINITY ? 0u : route_key(s + p.bias[32 * j + lane]);
+      for (int j = 0; j < V; ++j) {   // (0 * x: a masked expert's choice is a NaN, and out, like that of a bias which is one)
+        const float bias = 32 * j + lane < p.experts ? p.bias[32 * j + lane] : 0.f;
+        key[j] = route_key(least(s[j] + fmaf(0.f, x[j], bias)));
       }
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) key[j] = route_key(x[j]);
     }
-    sure = route_choose<uint32_t, V, SCORES>(p, key, lane, id);
-    auto score = [&](float v) {   // of an unmasked expert; softmax without `total`: up to a factor
-      if (p.sigmoid) return 1.0 / (1.0 + exp(-(double)v));
-      const double e = exp((double)v - (double)high);
-      return total > 0.0 ? e / total : e;
-    };
-    if constexpr (SCORES) {
-      if (!p.sigmoid && !sure) {
-        total = 0.0;
-#pragma unroll 1
-        for (int e = lane; e < p.experts; e += 32) {
-          const float v = logit(e);
-          total += v == -INFINITY ? 0.0 : exp((double)v - (double)high);
-        }
-        total = warp_sum(total);
-      }
-      if (!sure) {
-        uint64_t wide[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) wide[j] = x[j] == -INFINITY ? 0 : route_key(score(x[j]) + (double)p.bias[32 * j + lane]);
-        route_choose<uint64_t, V, true>(p, wide, lane, id);
+    for (int j = 0; j < V; ++j) key[j] = (key[j] & ~(uint32_t)(V - 1)) | (uint32_t)(V - 1 - j);
+    bool sure = true;
+    const float off = p.sigmoid ? 0x1p-20f : 0x1p-18f;
+    if (p.groups > 1) {
+      const uint32_t taken = route_groups<uint32_t, V, SCORES>(p, key, lane, off, sure);
+      route_keep<uint32_t, V>(p, key, lane, taken);
+    }
+    // A lane's keys in descending order (odd-even merge sort), so that taking one is a shift.
+#pragma unroll
+    for (int n = 1; n < V; n *= 2)
+#pragma unroll
+      for (int d = n; d > 0; d /= 2)
+#pragma unroll
+        for (int j = d % n; j + d < V; j += 2 * d)
+#pragma unroll
+          for (int i = 0; i < d; ++i)
+            if (i + j + d < V && (i + j) / (2 * n) == (i + j + d) / (2 * n)) {
+              const uint32_t u = key[i + j], v = key[i + j + d];
+              key[i + j] = max(u, v);
+              key[i + j + d] = min(u, v);
+            }
+    // Of equal keys the one in the lowest lane is taken: the same j, so the lowest expert.  16-bit logits lose nothing in their keys.
+    constexpr bool CHECK = SCORES || sizeof(T) == 4;
+    int id = -1;
+    uint32_t before = 0;
+#pragma unroll 1
+    for (int i = 0; i < p.top_k + (CHECK ? 1 : 0); ++i) {
+      const uint32_t best = warp_max(key[0]);
+      if (route_out(best)) break;
+      if (CHECK && i > 0) sure = sure && (SCORES ? route_above<V>(route_value(before), route_value(best), off) : (before / V) > (best / V));
+      before = best;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+      if (lane == i && i < p.top_k) id = 32 * (V - 1 - (int)(best & (V - 1))) + owner;
+      if (lane == owner) {
+#pragma unroll
+        for (int j = 0; j + 1 < V; ++j) key[j] = key[j + 1];
+        key[V - 1] = 0;
       }
     }
-    double w = id >= 0 ? score(logit(id)) : 0.0;
+    if (CHECK && !sure) {
+      uint64_t wide[V];
+      if constexpr (SCORES) {
+        double s[V], all = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s[j] = x[j] == -INFINITY ? 0.0 : exp(p.sigmoid ? -(double)x[j] : (double)x[j] - (double)high);
+          all += s[j];
+        }
+        if (!p.sigmoid) all = warp_sum(all);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          wide[j] = x[j] == -INFINITY ? 0 : route_key((p.sigmoid ? 1.0 / (1.0 + s[j]) : s[j] / all) + (double)p.bias[32 * j + lane]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) wide[j] = route_key((double)x[j]);
+      }
+      id = route_exact<V, SCORES>(p, wide, lane);
+    }
+    const float v = id >= 0 ? most(to_float<T>(row[id])) : 0.f;
+    if (!SCORES && p.renormalize && !p.sigmoid) high = __shfl_sync(0xffffffffu, v, 0);
+    float w = 0.f;
+    if (id >= 0) {
+      const float d = p.sigmoid ? -fabsf(v) : v - high, b = d - v;
+      float z = expf(d);
+      if (!p.sigmoid && d > -200.f) z += z * ((v - (d - b)) - (high + b));   // (what the difference lost: |d| 2^-25 of z)
+      w = p.sigmoid ? (v >= 0.f ? 1.f : z) / (1.f + z) : total > 0.f ? z / total : z;
+    }
     if (p.renormalize) {
-      const double sum = warp_sum(w);
-      w = sum > 0.0 ? w / sum : 0.0;
+      const float sum = warp_sum(w);
+      if (sum >= 1e-30f) {
+        w = w / sum;
+      } else {   // (sigmoids of logits around -70 and less)
+        const double d = id >= 0 && p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : 0.0, all = warp_sum(d);
+        w = all > 0.0 ? (float)(d / all) : 0.f;
+      }
     }
     if (lane < p.top_k) {
-      p.weights[t * p.top_k + lane] = (float)(w * (double)p.scale);
+      p.weights[t * p.top_k + lane] = w * p.scale;
       p.ids[t * p.top_k + lane] = id;
     }
   }
@@ -256,7 +336,8 @@ template <typename T> static cudaError_t route_typed(const RouteParams& p, cudaS
 
 int launch_moe_route(const void* logits, int dtype, int64_t ld, const float* bias, float* weights, int32_t* ids, int64_t tokens, int experts, int top_k,
                      int groups, int topk_group, int sigmoid, int renormalize, float scale, cudaStream_t stream) {
-  const RouteParams p{logits, ld, bias, weights, ids, tokens, experts, top_k, groups, topk_group, sigmoid, renormalize, scale};
+  const RouteParams p{logits, ld, bias, weights, ids, tokens, experts, top_k, groups, topk_group, sigmoid, renormalize, scale, experts / groups,
+                      ((1 << 20) + experts / groups - 1) / (experts / groups)};
   if (tokens == 0) return E_OK;
   cudaError_t e;
   switch (dtype) {
