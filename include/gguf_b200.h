@@ -203,13 +203,13 @@ int gguf_b200_moe_route(const void* logits, int dtype, int64_t ld, const float* 
 int gguf_b200_int8_quantize(const void* X, int dtype, int64_t ldx, void* Q, int64_t ldq, float* scales, int64_t M, int64_t K, void* stream);
 
 /* Linear layer: Y[m][n] = (sum over k of code(X)[m][k] * W[n][k]) * scale(X)[m] * w_scales[n] + bias[n], rounded to dtype once; X [M][K] in dtype,
- * rows ldx elements apart, quantized by the call as above; bias [N] in dtype or null.  Workspace: gguf_b200_int8_scratch_bytes. */
+ * rows ldx elements apart, quantized by the call as above; bias [N] in dtype or null.  flags: 0, or GGUF_B200_W_IN_FLIGHT where W may be
+ * written by the work directly ahead in the stream (a gguf_b200_int8_quantize of W, say); without it W may be read ahead of the
+ * stream (see gguf_b200_weights_complete).  Workspace: gguf_b200_int8_scratch_bytes. */
 int64_t gguf_b200_int8_scratch_bytes(int64_t M, int64_t K);
 int gguf_b200_int8_mul_mat(const void* W, int64_t ldw, const float* w_scales, const void* X, int64_t ldx, const void* bias, void* Y,
-                           void* workspace, int64_t workspace_bytes, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
-/* The same on activations that are quantized already, for several products of the same ones (q/k/v).  flags: 0, or
- * GGUF_B200_W_IN_FLIGHT where W may be written by the work directly ahead in the stream (an gguf_b200_int8_quantize of W, say);
- * without it W may be read ahead of the stream (see gguf_b200_weights_complete). */
+                           void* workspace, int64_t workspace_bytes, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
+/* The same on activations that are quantized already, for several products of the same ones (q/k/v). */
 int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_scales, const void* Q, int64_t ldq, const float* q_scales,
                                     const void* bias, void* Y, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream);
 

@@ -120,7 +120,8 @@ def test_quantize_strides(ops, dtype):
 
 # ---- linear product ------------------------------------------------------------------------------------------
 
-SIZES = [(1, 1, 1), (1, 1, 16), (1, 7, 33), (1, 128, 128), (2, 129, 127), (1, 4096, 4096), (3, 200, 4096), (16, 256, 1024), (17, 4000, 512), (27, 384, 8192),
+SIZES = [(1, 1, 1), (1, 1, 16), (1, 7, 33), (1, 128, 128), (2, 129, 127), (1, 4096, 4096), (2, 1000, 2064), (3, 200, 4096), (5, 300, 1040), (7, 128, 14336),
+         (8, 513, 5000), (1, 19072, 6144), (4, 19072, 6160), (9, 130, 4096), (16, 256, 1024), (17, 4000, 512), (27, 384, 8192),
          (33, 300, 2048), (64, 640, 4096), (65, 130, 4100), (128, 1000, 640), (200, 256, 14336), (255, 130, 256), (256, 130, 640), (257, 130, 640),
          (300, 4096, 1536), (513, 257, 384), (1000, 520, 1040), (2049, 2100, 400)]
 
@@ -372,13 +373,13 @@ def test_c_abi_refuses_before_any_launch(native_libs):
     assert q(null, 1, 64, null, 64, null, 0, 64, null) == 0
     m = lib.gguf_b200_int8_mul_mat
     assert lib.gguf_b200_int8_scratch_bytes(3, 100) == 512 + 256 and lib.gguf_b200_int8_scratch_bytes(0, 100) == 0
-    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 9, 1, 8, 64, null) == -2
-    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 0, null) == -3
-    assert m(p, 131072, p, p, 131072, null, p, p, 1 << 20, 1, 1, 8, 131072, null) == -7
-    assert m(odd, 64, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4 and m(p, 72, p, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4
-    assert m(p, 64, null, p, 64, null, p, p, 1 << 20, 1, 1, 8, 64, null) == -4 and m(p, 64, p, p, 64, null, p, null, 0, 1, 1, 8, 64, null) == -4
-    assert m(p, 64, p, p, 64, null, p, p, 16, 1, 1, 8, 64, null) == -5
-    assert m(p, 64, p, p, 64, null, p, p, 0, 1, 0, 8, 64, null) == 0
+    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 0, 9, 1, 8, 64, null) == -2
+    assert m(p, 64, p, p, 64, null, p, p, 1 << 20, 0, 1, 1, 8, 0, null) == -3
+    assert m(p, 131072, p, p, 131072, null, p, p, 1 << 20, 0, 1, 1, 8, 131072, null) == -7
+    assert m(odd, 64, p, p, 64, null, p, p, 1 << 20, 0, 1, 1, 8, 64, null) == -4 and m(p, 72, p, p, 64, null, p, p, 1 << 20, 0, 1, 1, 8, 64, null) == -4
+    assert m(p, 64, null, p, 64, null, p, p, 1 << 20, 0, 1, 1, 8, 64, null) == -4 and m(p, 64, p, p, 64, null, p, null, 0, 0, 1, 1, 8, 64, null) == -4
+    assert m(p, 64, p, p, 64, null, p, p, 16, 0, 1, 1, 8, 64, null) == -5
+    assert m(p, 64, p, p, 64, null, p, p, 0, 0, 1, 0, 8, 64, null) == 0
     pr = lib.gguf_b200_int8_mul_mat_prepared
     assert pr(p, 64, p, odd, 64, p, null, p, 0, 1, 1, 8, 64, null) == -4 and pr(p, 64, p, p, 64, null, null, p, 0, 1, 1, 8, 64, null) == -4
     moe = lib.gguf_b200_int8_fused_moe

@@ -864,11 +864,25 @@ int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_s
 }
 
 int gguf_b200_int8_mul_mat(const void* W, int64_t ldw, const float* w_scales, const void* X, int64_t ldx, const void* bias, void* Y, void* ws,
-                           int64_t ws_bytes, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+                           int64_t ws_bytes, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
   int rc = i8_check(dtype, M, N, K);
   if (rc || M == 0 || N == 0) return rc;
+  if (ldx < 0) return E_BAD_SHAPE;
   if (!X || !i8_rows_ok(W, ldw, K) || !w_scales || !Y || !ws || !aligned16(ws)) return E_BAD_POINTER;
   if (ws_bytes < gguf_b200_int8_scratch_bytes(M, K)) return E_WORKSPACE;
+  if (i8_few(X, dtype, ldx, M, N, K)) {
+    int* st = status_ptr();
+    if (!st) return E_CUDA;
+    I8Product a{};
+    a.w = static_cast<const int8_t*>(W); a.ldw = ldw; a.w_scale = w_scales;
+    a.x = X; a.ldx = ldx;
+    a.y = Y; a.ldy = N; a.dtype = dtype; a.bias = bias;
+    a.m = M; a.n = N; a.k = K;
+    a.settled = !(flags & GGUF_B200_W_IN_FLIGHT);
+    a.experts = 1;
+    a.status = st;
+    return launch_i8_product(a, static_cast<cudaStream_t>(stream));
+  }
   float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(M * i8_ld(K), 256));
   rc = gguf_b200_int8_quantize(X, dtype, ldx, ws, i8_ld(K), scales, M, K, stream);
   // (the quantizer releases the product behind its own wait: whatever wrote W ahead of this call is complete by then)

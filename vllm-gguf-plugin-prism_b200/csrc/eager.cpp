@@ -224,13 +224,15 @@ PyObject* py_int8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// int8_mul_mat(W, w_scales, X, bias or None)
+// int8_mul_mat(W, w_scales, X, bias or None, settled)
 PyObject* py_int8_mul_mat(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 4, "int8_mul_mat takes 4 arguments");
+  TORCH_CHECK(n == 5, "int8_mul_mat takes 5 arguments");
   std::optional<Tensor> t[4];
   if (!plain_args(a, {false, false, false, true}, t)) Py_RETURN_NONE;
-  return THPVariable_Wrap(without_gil([&] { return Op::int8_mul_mat(*t[0], *t[1], *t[2], t[3]); }));
+  const int settled = PyObject_IsTrue(a[4]);
+  if (settled < 0) return nullptr;
+  return THPVariable_Wrap(without_gil([&] { return Op::int8_mul_mat(*t[0], *t[1], *t[2], t[3], settled != 0); }));
   END_HANDLE_TH_ERRORS
 }
 

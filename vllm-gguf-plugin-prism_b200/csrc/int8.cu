@@ -6,7 +6,7 @@
 // box).  Weight rows sit on the 128-row side of the instruction, tokens on its column side, any multiple of 16 up to 256; so one
 // token costs no more tensor time than sixteen, and what bounds small batches is the weights' way from memory.
 //
-// A CTA: a loader, an MMA issuer, eight epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
+// A CTA: a loader, an MMA issuer, sixteen epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
 // values.  Three ways to deal out the work:
 //   tiles    a CTA takes items (128 weight rows x up to 256 tokens) a grid apart, two accumulators in turn where they fit
 //   split    fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares the K of one tile.  Each sends its sums of every other's
@@ -14,9 +14,12 @@
 //            integer sums do not depend on the order
 //   experts  items are (pass of an expert's tokens, 128 rows).  For the gate and up product a box holds the same 64 rows of both, 16 and
 //            16 in turn: the two meet in one warp, so that act(gate) * up is formed on the way out and nothing else is stored
+//
+// A few tokens come as they are (FEW): the epilogue warps make their codes, and each CTA the ones of its K, in shared memory while the
+// weights arrive.  One launch instead of two; every CTA repeats the search for a token's largest value.
 #include <cuda.h>
 
-#include "int8.cuh"
+#include "int8_codes.cuh"
 #include "kernels.h"
 #include "raw_stream.cuh"
 #include "tcgen05.cuh"
@@ -25,7 +28,7 @@ namespace gguf_b200 {
 
 constexpr int I8_ROWS = 128, I8_BK = 128;                 // weight rows of a box, values (= bytes) of a stage
 constexpr int I8_A_BYTES = I8_ROWS * I8_BK;
-constexpr int I8_EPI = 8;                                 // epilogue warps
+constexpr int I8_EPI = 16;                                // epilogue warps
 constexpr int I8_THREADS = 128 + 32 * I8_EPI;             // warps 0 loader, 1 MMA issuer, 2 tensor memory, from 4 on epilogue
 constexpr int I8_MAX_STAGES = 16;
 constexpr int I8_SMS = 148;
@@ -51,6 +54,9 @@ struct I8Params {
   const int32_t* sorted;
   const float* w_unit;
   float unit;
+  const void* x;           // FEW: [m][ldx], behind the ring the codes of this CTA's K (2 KB a stage)
+  int64_t ldx;
+  int codes_off, recv_off; // recv_off: room for other CTAs' sums, 0: in the ring
   int* status;
 };
 
@@ -89,16 +95,19 @@ __device__ __forceinline__ void i8_box3(uint32_t dst, const CUtensorMap* map, in
 __device__ __forceinline__ void i8_box_l2(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
 // (the approximate exponential and quotient are off by a few units in the last place, 2^-21 of the result)
-__device__ __forceinline__ float i8_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+__device__ __forceinline__ float i8_silu(float g) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
+  return g * r;
+}
 __device__ __forceinline__ float i8_gelu(float g) { return 0.5f * g * (1.f + erff(g * 0.70710678f)); }
 __device__ __forceinline__ float i8_bias(const I8Params& p, int n) {
   if (!p.bias) return 0.f;
@@ -172,23 +181,59 @@ template <bool GLU> __device__ __forceinline__ void i8_weights(const CUtensorMap
   }
 }
 
-// GLU: gate and up product of experts
-template <bool GLU>
-__global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+// Codes of the tokens and their scales, by the 512 threads of the epilogue: a token's threads (all of them for one token, two warps each for
+// five to eight) read its row once for the largest value, and the part [k0, k1) again for the codes, which go where a TMA box of 16 rows
+// with the 128-byte swizzle would have put them.
+template <typename T> __device__ __forceinline__ void i8_few_codes(const I8Params& p, int k0, int k1, uint32_t codes, float* scale, uint32_t* top_of, int tid) {
+  const int lanes = 32 * I8_EPI / (p.m <= 2 ? p.m : p.m <= 4 ? 4 : 8), tok = tid / lanes, lane = tid % lanes;
+  const bool live = tok < p.m;
+  const T* x = static_cast<const T*>(p.x) + (live ? tok : 0) * p.ldx;
+  uint32_t top = 0;
+  for (int at = lane * I8Q_UNIT; at < (live ? p.k : 0); at += lanes * I8Q_UNIT) {
+    T v[I8Q_UNIT];
+    i8q_load<T, true>(x, p.k, at, v);
+    top = i8q_top<T>(v, top);
+  }
+  top = __reduce_max_sync(0xffffffffu, i8q_top_bits<T>(top));
+  if ((tid & 31) == 0) top_of[tid >> 5] = top;
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
+  for (int i = 0; i < lanes / 32; ++i) top = max(top, top_of[tok * (lanes / 32) + i]);
+  const bool finite = top < 0x7f800000u, zero = !finite || top == 0;
+  const float a = __uint_as_float(top);
+  const I8Row w = i8q_row(zero ? 1.f : a);
+  if (live && lane == 0) scale[tok] = finite ? a / 127.f : __uint_as_float(0x7fc00000u);
+  for (int at = k0 + lane * I8Q_UNIT; at < (live ? k1 : 0); at += lanes * I8Q_UNIT) {
+    uint4 c = make_uint4(0, 0, 0, 0);
+    if (at < p.k && !zero) {
+      T v[I8Q_UNIT];
+      i8q_load<T, true>(x, p.k, at, v);
+      c = i8q_unit<T>(v, w);
+    }
+    const uint32_t to = codes + (uint32_t)((at - k0) / I8_BK * 2048 + tok * 128 + ((at / 16 ^ tok) & 7) * 16);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w) : "memory");
+  }
+}
+
+// GLU: gate and up product of experts.  FEW: float (or void: not so), __half, __nv_bfloat16: up to eight tokens of that type
+template <bool GLU, typename FewT = void>
+__global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                                                            const __grid_constant__ I8Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // (from the shared-window address, so that the CTAs of a cluster agree about offsets)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.aux_off);
   uint64_t *full = bars, *empty = bars + I8_MAX_STAGES, *accum = bars + 2 * I8_MAX_STAGES, *drained = accum + 2, *last = accum + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 7);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_scale = reinterpret_cast<float*>(smem + p.aux_off + 512);   // [2][256]
   int* s_row = reinterpret_cast<int*>(s_scale + 512);                  // [2][256]
   uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_row + 512);          // [I8_EPI][1024]
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr bool FEW = !std::is_void<FewT>::value;
+  uint64_t* coded = accum + 6;   // FEW: the codes are there
 
   if (threadIdx.x == 0) {
+    mbar_init(coded, I8_EPI);
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -200,6 +245,7 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     *gave_up = 0;
     fence_barrier_init();
   }
+  if (p.split > 1) cluster_arrive();   // (waited for before anything is sent)
   if (warp == 2) {
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
@@ -207,10 +253,11 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t rank = p.split > 1 ? cluster_rank() : 0u;
-  if (p.split > 1) cluster_sync();
+  // (From lane 0 to all: the compiler then knows that a warp's lanes agree, and keeps what follows from it in uniform registers.  With a
+  // loop that it takes for divergent, an MMA takes 115 clocks however few its tokens are.)
+  const uint32_t rank = p.split > 1 ? __shfl_sync(0xffffffffu, cluster_rank(), 0) : 0u;
   pdl_trigger();
-  const uint32_t tmem = *tmem_slot, gave_up_s = smem_u32(const_cast<const int*>(gave_up)), full_s = smem_u32(full), empty_s = smem_u32(empty);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), gave_up_s = smem_u32(const_cast<const int*>(gave_up)), full_s = smem_u32(full), empty_s = smem_u32(empty);
   const uint32_t accum_s = smem_u32(accum), drained_s = smem_u32(drained);
   const int first = p.split > 1 ? (int)blockIdx.x / p.split : (int)blockIdx.x, step = p.split > 1 ? 1 << 30 : (int)gridDim.x;
   const int kb0 = p.split > 1 ? (int)(p.nk * rank) / p.split : 0, kb1 = p.split > 1 ? (int)(p.nk * (rank + 1)) / p.split : p.nk;
@@ -224,8 +271,8 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     uint32_t ph = 0;
     if (first < n_items) {   // the first weights before the activations are there: into the ring, or, if they may still be written, into L2
       const I8Item t = i8_item<GLU>(p, first, false);
-      const uint32_t bytes = (uint32_t)(I8_A_BYTES + (t.rows + p.bh - 1) / p.bh * p.bh * I8_BK);
-      ahead = min(p.stages, kb1 - kb0);
+      const uint32_t bytes = (uint32_t)(I8_A_BYTES + (FEW ? 0 : (t.rows + p.bh - 1) / p.bh * p.bh * I8_BK));
+      ahead = FEW && !p.settled ? kb1 - kb0 : min(p.stages, kb1 - kb0);
       for (int j = 0; j < ahead; ++j)
         if (lead) {
           if (p.settled) {
@@ -240,7 +287,7 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     pdl_wait();
     for (int i = first; i < n_items; i += step) {
       const I8Item t = i8_item<GLU>(p, i, true);
-      const int boxes = (t.rows + p.bh - 1) / p.bh;
+      const int boxes = FEW ? 0 : (t.rows + p.bh - 1) / p.bh;
       for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t fb = full_s + 8u * s, at = ring + (uint32_t)(s * p.stage_bytes);
         if (ahead == 0) {
@@ -270,13 +317,15 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     for (int i = first; i < n_items; i += step) {
       const int cols = (__shfl_sync(0xffffffffu, i8_item<GLU>(p, i, false).rows, 0) + 15) & ~15;
       const uint32_t idesc = i8_idesc(cols), d = tmem + (uint32_t)(buf * p.tn);
+      const uint32_t codes0 = (uint32_t)umma_desc_sw128(smem_u32(smem + p.codes_off));
+      if (FEW) mbar_wait_or(smem_u32(coded), 0u, gave_up_s);
       mbar_wait_or(drained_s + 8u * buf, dph ^ 1u, gave_up_s);
       for (int kb = kb0; kb < kb1; ++kb) {
         mbar_wait_or(full_s + 8u * s, ph, gave_up_s);
         __syncwarp();
         tc_fence_after();
         const uint32_t a = lo0 + (uint32_t)s * stage16;
-        umma_i8_ss4(d, a, a + (I8_A_BYTES >> 4), hi, idesc, kb > kb0, lead);
+        umma_i8_ss4(d, a, FEW ? codes0 + (uint32_t)(kb - kb0) * (2048 >> 4) : a + (I8_A_BYTES >> 4), hi, idesc, kb > kb0, lead);
         umma_commit(empty_s + 8u * s, lead);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
@@ -286,8 +335,8 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     __syncwarp();
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
-    // (a warp reaches the 32 lanes of tensor memory of its number modulo 4; two warps share them, taking 16 columns in turn)
-    const int quad = (warp & 3) * 32, row = quad + lane, half = (warp - 4) >> 2, tid = threadIdx.x - 128;
+    // (a warp reaches the 32 lanes of tensor memory of its number modulo 4; four warps share them, taking 16 columns in turn)
+    const int quad = (warp & 3) * 32, row = quad + lane, turn16 = 16 * ((warp - 4) >> 2), tid = threadIdx.x - 128;
     const uint32_t t_lane = tmem + ((uint32_t)quad << 16);
     uint8_t* stage = s_stage + (warp - 4) * 1024;
     const bool wide_y = p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
@@ -296,14 +345,20 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
     pdl_wait();
     for (int i = first; i < n_items; i += step) {
       const I8Item t = i8_item<GLU>(p, i, true);
-      float* xs = s_scale + turn * 256;   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
+      float* xs = s_scale + (FEW ? 0 : turn * 256);   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
       int* xr = s_row + turn * 256;
       turn ^= 1;
       const bool down = !GLU && p.passes;   // (left to the sum over the experts: scale of the token, routing weight)
       for (int c = tid; c < p.tn; c += 32 * I8_EPI) {
         const int at = t.x0 + c;
-        xs[c] = c < t.rows && !down ? p.q_scale[at] : 1.f;
+        if (!FEW) xs[c] = c < t.rows && !down ? p.q_scale[at] : 1.f;
         xr[c] = c < t.rows && down ? p.sorted[at] : at;
+      }
+      if constexpr (FEW) if (i == first) {   // (the same for all of a CTA's items)
+        i8_few_codes<FewT>(p, kb0 * I8_BK, kb1 * I8_BK, smem_u32(smem + p.codes_off), xs, reinterpret_cast<uint32_t*>(s_stage), tid);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(coded);
       }
       // this lane's row: of 128, or, gate and up, lanes 0 to 15 a gate row and lanes 16 to 31 its up row
       const int r = GLU ? quad / 2 + (lane & 15) : row, n = t.n0 + r;
@@ -317,7 +372,7 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
       if (p.split == 1) {
         const uint32_t d = t_lane + (uint32_t)(buf * p.tn);
         const float bias = !GLU && live ? i8_bias(p, n) : 0.f;
-        for (int c0 = 16 * half; c0 < t.rows; c0 += 32) {
+        for (int c0 = turn16; c0 < t.rows; c0 += 4 * I8_EPI) {
           uint32_t v[16];
           tmem_ld16(d + (uint32_t)c0, v);
           float f[16];
@@ -363,19 +418,23 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
   __syncwarp();
   if (!GLU && p.split > 1) {
     // ---------------- split: the sums of rows [per * rank, per * (rank + 1)) of the tile are this CTA's to add and store ----------------
-    // The rows of another CTA go into its ring, [sender][row][token], rows 16 bytes more than tn words apart (eight lanes' 16 bytes then
+    // The rows of another CTA go into its shared memory, [sender][row][token], rows 16 bytes more than tn words apart (eight lanes' 16 bytes then
     // lie in different banks).  A lane keeps its row to the end.
-    cluster_sync();   // every CTA's products are complete, its ring is free
+    cluster_wait();
+    if (p.recv_off == 0) {   // every CTA's products have to be complete, so that its ring is free
+      cluster_arrive();
+      cluster_wait();
+    }
     const I8Item t = i8_item<false>(p, first, true);
     const int per = I8_ROWS / p.split, shift = 31 - __clz(per), quad = (warp & 3) * 32, row = quad + lane, owner = row >> shift;
-    const int half = 16 * ((warp - 4) >> 2);
-    const uint32_t d = tmem + ((uint32_t)quad << 16), pitch = 4u * (uint32_t)p.tn + 16u, ring = smem_u32(smem);
+    const int turn16 = 16 * ((warp - 4) >> 2);
+    const uint32_t d = tmem + ((uint32_t)quad << 16), pitch = 4u * (uint32_t)p.tn + 16u, ring = smem_u32(smem + p.recv_off);
     const bool mine = owner == (int)rank;
     if (warp >= 4 && !(p.split <= 4 && mine)) {   // (whole warps of a quad, unless 16 rows are a CTA's)
       const uint32_t slot = rank - (owner < (int)rank ? 1u : 0u);   // (senders in order, without the owner)
       uint32_t peer;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ring + (slot * (uint32_t)per + (uint32_t)(row & (per - 1))) * pitch), "r"(owner));
-      for (int c0 = half; c0 < t.rows; c0 += 32) {
+      for (int c0 = turn16; c0 < t.rows; c0 += 4 * I8_EPI) {
         uint32_t v[16];
         tmem_ld16(d + (uint32_t)c0, v);
         tmem_ld_wait();
@@ -387,13 +446,14 @@ __global__ void __launch_bounds__(I8_THREADS, 2) i8_kernel(const __grid_constant
         }
       }
     }
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();
     if (warp >= 4 && (p.split == 8 ? quad >> 5 == (int)rank >> 1 : mine)) {
       const int n = t.n0 + row;
       const bool live = mine && n < p.n, wide = p.split <= 4 && p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && t.n0 + quad + 32 <= p.n;
       const float ws = live ? p.w_scale[t.a_row + row] : 0.f, bias = live ? i8_bias(p, n) : 0.f;
       const uint32_t from0 = ring + (uint32_t)(row & (per - 1)) * pitch;
-      for (int c0 = half; c0 < t.rows; c0 += 32) {
+      for (int c0 = turn16; c0 < t.rows; c0 += 4 * I8_EPI) {
         uint32_t v[16];
         tmem_ld16(d + (uint32_t)c0, v);
         tmem_ld_wait();
@@ -445,19 +505,39 @@ static bool i8_map(CUtensorMap& map, const void* base, int64_t k, int64_t rows, 
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool GLU> static int i8_launch(const CUtensorMap& amap, const CUtensorMap& bmap, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
+template <bool GLU, typename FewT> static int i8_launch(const CUtensorMap& amap, const CUtensorMap& bmap, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return E_CUDA;
   if (!configured[dev & 63]) {
-    if (cudaFuncSetAttribute(i8_kernel<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
+    if (cudaFuncSetAttribute(i8_kernel<GLU, FewT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
     configured[dev & 63] = true;
   }
-  return launch_pdl_cluster(i8_kernel<GLU>, dim3((unsigned)grid), dim3(I8_THREADS), (unsigned)p.split, smem, stream, amap, bmap, p) == cudaSuccess ? E_OK : E_CUDA;
+  return launch_pdl_cluster(i8_kernel<GLU, FewT>, dim3((unsigned)grid), dim3(I8_THREADS), (unsigned)p.split, smem, stream, amap, bmap, p) == cudaSuccess ? E_OK : E_CUDA;
+}
+
+// CTAs that share a tile: as many as there are SMs for, while the stages that each is spared take longer than the exchange.  (A stage takes 0.25
+// to 0.35 us; sharing by two, 1 us + 0.025 us a token.  Whole / by 2 / by 4 in us: 1 token of 4096x4096 10.6 / 8.7 / 7.7, 128 tokens 12.1 /
+// 11.8 / 12.2, 500 tokens 15.3 / 17.1, of 4096x14336 40.8 / 30.9.)
+static int i8_split(int64_t tiles, int nk, int tn) {
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= I8_SMS && nk / (2 * split) > 5 + tn / 14) split *= 2;
+  return split;
+}
+// Whether a product of m tokens is one launch: rows that 16-byte loads can start at, the codes of a CTA's K (2 KB a stage) leave half of its
+// shared memory to the weights, and finding the tokens' largest values, which every CTA repeats, takes less than a launch.  (One / two
+// launches in us: 4096x4096, 1 token 7.2 / 9.1, 4 tokens 8.5 / 9.1, 8 tokens 9.9 / 9.1; 4096x14336, 1 token 15.0 / 16.1, 8 tokens 27 / 16.)
+constexpr int I8_FEW = 8;
+constexpr int64_t I8_FEW_VALUES = 16384;
+bool i8_few(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k) {
+  const int64_t size = dtype == DT_F32 ? 4 : 2, nk = (k + I8_BK - 1) / I8_BK;
+  if (m > I8_FEW || m * k > I8_FEW_VALUES || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || (m > 1 && ldx * size % 16 != 0)) return false;
+  const int split = i8_split((n + I8_ROWS - 1) / I8_ROWS, (int)nk, 16);
+  return (nk + split - 1) / split <= 48;
 }
 
 int launch_i8_product(const I8Product& a, cudaStream_t stream) {
-  const bool glu = a.act != 0;
+  const bool glu = a.act != 0, few = a.x != nullptr;
   const int per_tile = glu ? I8_ROWS / 2 : I8_ROWS;   // results a row tile
   I8Params p{};
   p.n = (int)a.n;
@@ -474,18 +554,21 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
     p.tn = (int)round_up((a.m + p.tt - 1) / p.tt, 16);
   }
   p.bh = !a.passes || p.tn <= 64 ? p.tn : 64;
-  p.stage_bytes = I8_A_BYTES + (int)round_up(p.tn, p.bh) * I8_BK;
-  const int per_sm = p.tn <= 64 ? 2 : 1;
+  p.stage_bytes = I8_A_BYTES + (few ? 0 : (int)round_up(p.tn, p.bh) * I8_BK);
   const int64_t tiles = a.passes ? a.max_passes * p.rt : (int64_t)p.rt * p.tt;
   if (tiles > 1 << 29) return E_TOO_LARGE;
-  p.split = 1;
-  if (!a.passes)
-    while (p.split < 8 && tiles * p.split * 2 <= I8_SMS * per_sm && p.nk >= 8 * p.split) p.split *= 2;
-  const int room = (per_sm == 2 ? 113 : 227) * 1024 - 1024 - I8_AUX - (per_sm == 2 ? 1024 : 0);
-  p.stages = room / p.stage_bytes;
+  p.split = a.passes ? 1 : i8_split(tiles, p.nk, p.tn);
+  // shared memory: ring, barriers and scales, codes of a few tokens, sums of other CTAs where they are small
+  const int recv = p.split > 1 ? I8_ROWS / p.split * (p.split - 1) * (4 * p.tn + 16) : 0;
+  const int codes = few ? (p.nk + p.split - 1) / p.split * 2048 : 0;
+  const int extra = I8_AUX + codes + (recv <= 32768 ? (int)round_up(recv, 1024) : 0);
+  p.stages = (226 * 1024 - extra) / p.stage_bytes;
   if (p.stages > I8_MAX_STAGES) p.stages = I8_MAX_STAGES;
-  p.aux_off = p.stages * p.stage_bytes;
-  p.nbuf = p.split == 1 && 2 * p.tn <= 512 / per_sm ? 2 : 1;
+  const int ring = p.stages * p.stage_bytes;
+  p.codes_off = ring;
+  p.recv_off = recv > 0 && recv <= 32768 ? ring + codes : 0;
+  p.aux_off = ring + extra - I8_AUX;
+  p.nbuf = p.split == 1 && 2 * p.tn <= 512 ? 2 : 1;
   p.tmem_cols = 32;
   while ((int)p.tmem_cols < p.nbuf * p.tn) p.tmem_cols *= 2;
   p.y = a.y;
@@ -501,12 +584,22 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.sorted = a.sorted;
   p.w_unit = a.w_unit;
   p.unit = a.unit;
+  p.x = a.x;
+  p.ldx = a.ldx;
   p.status = a.status;
-  const int64_t slots = I8_SMS * per_sm, grid = p.split > 1 ? tiles * p.split : tiles < slots ? tiles : slots;
+  const int64_t grid = p.split > 1 ? tiles * p.split : tiles < I8_SMS ? tiles : I8_SMS;
   CUtensorMap amap, bmap;
-  if (!i8_map(amap, a.w, a.k, a.experts * p.w_rows, a.ldw, glu ? 16 : I8_ROWS, glu ? 2 * a.experts : 0) || !i8_map(bmap, a.q, a.k, a.m, a.ldq, p.bh)) return E_CUDA;
+  if (!i8_map(amap, a.w, a.k, a.experts * p.w_rows, a.ldw, glu ? 16 : I8_ROWS, glu ? 2 * a.experts : 0)) return E_CUDA;
+  if (few) bmap = amap;   // (not read)
+  else if (!i8_map(bmap, a.q, a.k, a.m, a.ldq, p.bh)) return E_CUDA;
   const size_t smem = 1024 + (size_t)p.aux_off + I8_AUX;
-  return glu ? i8_launch<true>(amap, bmap, p, (int)grid, smem, stream) : i8_launch<false>(amap, bmap, p, (int)grid, smem, stream);
+  if (glu) return i8_launch<true, void>(amap, bmap, p, (int)grid, smem, stream);
+  if (!few) return i8_launch<false, void>(amap, bmap, p, (int)grid, smem, stream);
+  switch (a.dtype) {
+    case DT_F32: return i8_launch<false, float>(amap, bmap, p, (int)grid, smem, stream);
+    case DT_F16: return i8_launch<false, __half>(amap, bmap, p, (int)grid, smem, stream);
+    default: return i8_launch<false, __nv_bfloat16>(amap, bmap, p, (int)grid, smem, stream);
+  }
 }
 
 }  // namespace gguf_b200

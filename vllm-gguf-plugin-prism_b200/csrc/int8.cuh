@@ -46,8 +46,12 @@ struct I8Product {
   const int32_t* sorted;
   const float* w_unit;
   float unit;
+  // ... tokens that are not quantized yet (null: q is used; see i8_few): [m][ldx] in dtype
+  const void* x;
+  int64_t ldx;
   int* status;
 };
+bool i8_few(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k);
 int launch_i8_product(const I8Product& a, cudaStream_t stream);
 
 // The routed expert step around the products (int8_moe.cu)

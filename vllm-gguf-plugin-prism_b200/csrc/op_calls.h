@@ -307,7 +307,8 @@ template <class A> struct Calls {
     return {ldq == K ? q : A::block(q, 0, M, 0, K), s};
   }
 
-  static Tensor int8_mul_mat(const Tensor& W, const Tensor& w_scales, const Tensor& X, const std::optional<Tensor>& bias) {
+  // settled: see mul_mat
+  static Tensor int8_mul_mat(const Tensor& W, const Tensor& w_scales, const Tensor& X, const std::optional<Tensor>& bias, bool settled) {
     const char* op = "int8_mul_mat";
     const typename A::Guard guard(A::device(X));
     const ScalarType dt = X.scalar_type();
@@ -321,7 +322,9 @@ template <class A> struct Calls {
     if (M == 0 || N == 0) return Y;
     const int64_t bytes = gguf_b200_int8_scratch_bytes(M, K);
     const typename A::Scratch scratch(X, bytes);
-    check_rc(gguf_b200_int8_mul_mat(W.data_ptr(), ldw, ws, X.data_ptr(), ldx, b, Y.data_ptr(), scratch.get(), bytes, code, M, N, K, A::stream(X)), op);
+    check_rc(gguf_b200_int8_mul_mat(W.data_ptr(), ldw, ws, X.data_ptr(), ldx, b, Y.data_ptr(), scratch.get(), bytes, settled ? 0 : GGUF_B200_W_IN_FLIGHT, code, M, N, K,
+                                    A::stream(X)),
+             op);
     return Y;
   }
 

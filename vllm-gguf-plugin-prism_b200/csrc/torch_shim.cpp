@@ -76,7 +76,7 @@ std::tuple<Tensor, Tensor> moe_route(Tensor logits, std::optional<Tensor> bias, 
   return Op::moe_route(logits, bias, top_k, n_group, topk_group, scoring, renormalize, scale);
 }
 std::tuple<Tensor, Tensor> int8_quantize(Tensor X) { return Op::int8_quantize(X); }
-Tensor int8_mul_mat(Tensor W, Tensor w_scales, Tensor X, std::optional<Tensor> bias) { return Op::int8_mul_mat(W, w_scales, X, bias); }
+Tensor int8_mul_mat(Tensor W, Tensor w_scales, Tensor X, std::optional<Tensor> bias) { return Op::int8_mul_mat(W, w_scales, X, bias, false); }
 Tensor int8_mul_mat_prepared(Tensor W, Tensor w_scales, Tensor Q, Tensor q_scales, std::optional<Tensor> bias, ScalarType dtype) {
   return Op::int8_mul_mat_prepared(W, w_scales, Q, q_scales, bias, dtype);
 }

@@ -49,7 +49,7 @@ SIGNATURES = {
     "gguf_b200_moe_route": (_I, [_P, _I, _L, _P, _P, _P, _L, _L, _L, _L, _L, _I, _I, _F, _P]),
     "gguf_b200_int8_quantize": (_I, [_P, _I, _L, _P, _L, _P, _L, _L, _P]),
     "gguf_b200_int8_scratch_bytes": (_L, [_L, _L]),
-    "gguf_b200_int8_mul_mat": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _I, _L, _L, _L, _P]),
+    "gguf_b200_int8_mul_mat": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _I, _I, _L, _L, _L, _P]),
     "gguf_b200_int8_mul_mat_prepared": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _I, _I, _L, _L, _L, _P]),
     "gguf_b200_int8_moe_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
     "gguf_b200_int8_fused_moe": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _L, _L, _L, _L, _L, _P]),

@@ -306,7 +306,7 @@ def int8_mul_mat(W: torch.Tensor, w_scales: torch.Tensor, X: torch.Tensor, bias:
     """A linear layer with 8-bit integer weights ``W [N, K]`` and a scale for each of their rows: ``X [tokens, K]`` (float32, float16 or
     bfloat16) is quantized by the token as ``int8_quantize`` does it, the product is summed exactly, scaled, and rounded once.
     -> ``[tokens, N]`` in X's dtype.  The rows of W start at multiples of 16 bytes; K up to 131071."""
-    y = None if is_compiling() else native.int8_mul_mat(W, w_scales, X, bias)
+    y = None if is_compiling() else native.int8_mul_mat(W, w_scales, X, bias, False)
     return torch.ops._C_gguf.int8_mul_mat(W, w_scales, X, bias) if y is None else y
 
 
