@@ -6,18 +6,19 @@
 // box).  Weight rows sit on the 128-row side of the instruction, tokens on its column side, any multiple of 16 up to 256; so one
 // token costs no more tensor time than sixteen, and what bounds small batches is the weights' way from memory.
 //
-// A CTA: a loader, an MMA issuer, sixteen epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
+// A CTA: three loaders, an MMA issuer, sixteen epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
 // values.  Three ways to deal out the work:
 //   tiles    a CTA takes items (128 weight rows x up to 256 tokens) a grid apart, two accumulators in turn where they fit
 //   split    fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares the K of one tile.  Each sends its sums of every other's
 //            rows into the other's shared memory, which then adds and stores its rows: no scratch in memory, nothing to clear, and
 //            integer sums do not depend on the order
-//   experts  items are (pass of an expert's tokens, 128 rows).  For the gate and up product a box holds the same 64 rows of both, 16 and
-//            16 in turn: the two meet in one warp, so that act(gate) * up is formed on the way out and nothing else is stored
+//   experts  items are (pass of an expert's tokens, 128 rows).  For the gate and up product a box holds the same 64 rows of both, 8 and
+//            8 in turn: the two meet in one warp, so that act(gate) * up is formed on the way out and nothing else is stored
 //
 // A few tokens come as they are (FEW): the epilogue warps make their codes, and each CTA the ones of its K, in shared memory while the
 // weights arrive.  One launch instead of two; every CTA repeats the search for a token's largest value.
 #include <cuda.h>
+#include <math.h>
 
 #include "int8_codes.cuh"
 #include "kernels.h"
@@ -29,18 +30,17 @@ namespace gguf_b200 {
 constexpr int I8_ROWS = 128, I8_BK = 128;                 // weight rows of a box, values (= bytes) of a stage
 constexpr int I8_A_BYTES = I8_ROWS * I8_BK;
 constexpr int I8_EPI = 16;                                // epilogue warps
-constexpr int I8_THREADS = 128 + 32 * I8_EPI;             // warps 0 loader, 1 MMA issuer, 2 tensor memory, from 4 on epilogue
+constexpr int I8_THREADS = 128 + 32 * I8_EPI;             // warps 0, 2, 3 loaders, 1 MMA issuer, from 4 on epilogue
 constexpr int I8_MAX_STAGES = 16;
 constexpr int I8_SMS = 148;
-constexpr int I8_AUX = 512 + 2 * 256 * 8 + I8_EPI * 1024; // barriers; scale and output row of every token, of two items; 16 tokens x 32 rows a warp
+constexpr int I8_AUX = 512 + 2 * 256 * 8 + I8_EPI * 1024 + 128 * 16;   // barriers; scale and output row of every token, of two items; 16 tokens x 32 rows a warp; work list
 
 struct I8Params {
   int n;                   // results a token
   int w_rows;              // weight rows of an expert
   int k, nk;               // values, stages
-  int m, rt, tt, tn, bh;   // tokens; row tiles, token tiles; tokens a tile; rows of a box of tokens
+  int m, rt, tt, tn;       // tokens; row tiles, token tiles; tokens a tile
   int stages, stage_bytes, nbuf, aux_off;
-  uint32_t tmem_cols;
   int split;
   void* y;
   int64_t ldy;
@@ -60,48 +60,80 @@ struct I8Params {
   int* status;
 };
 
-// Four times D[tmem] (+)= A[smem] * B[smem], 32 values (bytes) each: +2 in the descriptors' 16-byte units
-__device__ __forceinline__ void umma_i8_ss4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, p;\n\t"
-      "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, t;\n\t"
-      "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, t;\n\t"
-      "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, t;\n\t}"
-      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead)
-      : "memory");
+// Four times D[tmem] (+)= A[smem] * B[smem], 32 values (bytes) each: +2 in the descriptors' 16-byte units.  PAIR: by two SMs, each with its half
+// of A's rows and of B's in its own shared memory, at the same place, and its rows' sums in its own tensor memory.
+template <bool PAIR> __device__ __forceinline__ void umma_i8_ss4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+#define I8_MMA4(GROUP)                                                                          \
+  asm volatile(                                                                                 \
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl;\n\t"                   \
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"             \
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"                                       \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %4, p;\n\t"                     \
+      "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t" \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %4, t;\n\t"                     \
+      "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t" \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %4, t;\n\t"                     \
+      "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t" \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %4, t;\n\t}"                    \
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead) : "memory")
+  if (PAIR) I8_MMA4("2");
+  else I8_MMA4("1");
+#undef I8_MMA4
 }
-// kind::i8 instruction descriptor: 32-bit integer sums, both operands signed, K-major, 128 rows, n columns
-__device__ __forceinline__ uint32_t i8_idesc(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(I8_ROWS >> 4) << 24);
+// kind::i8 instruction descriptor: 32-bit integer sums, both operands signed, K-major, 128 rows (or a pair's 256), n columns
+__device__ __forceinline__ uint32_t i8_idesc(bool pair, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)((pair ? 2 : 1) * I8_ROWS >> 4) << 24);
 }
-__device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
+// The MMAs so far are done: tells the barrier, of a pair both CTAs'
+template <bool PAIR> __device__ __forceinline__ void i8_commit(uint32_t bar, uint32_t lead) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred q;\n\t.reg .b16 both;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 both, 3;\n\t"
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar), "r"(lead) : "memory");
+  else
+    umma_commit(bar, lead);
 }
-__device__ __forceinline__ void i8_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
+template <bool PAIR> __device__ __forceinline__ void i8_tmem_alloc(uint32_t* slot, uint32_t cols) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR> __device__ __forceinline__ void i8_tmem_dealloc(uint32_t at, uint32_t cols) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
+  else tmem_dealloc(at, cols);
+}
+constexpr uint32_t I8_LEADER = 0xFEFFFFFFu;   // of a shared-memory address in a cluster of two: the same place in the first CTA
+// (GROUP 2: a pair's copies, each into its own shared memory, may count on the first CTA's barrier)
+template <bool PAIR> __device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(y) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <bool PAIR> __device__ __forceinline__ void i8_box5(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(0), "r"(y), "r"(z) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(0), "r"(y), "r"(z) : "memory");
 }
 __device__ __forceinline__ void i8_box_l2(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
+// mbar_wait_or, and whether it was for nothing
+__device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
+  if (mbar_try_wait(bar, parity)) return true;
+  mbar_wait_or(bar, parity, gave_up);
+  return lds32(gave_up) == 0u;
+}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 // (the approximate exponential and quotient are off by a few units in the last place, 2^-21 of the result)
 __device__ __forceinline__ float i8_silu(float g) {
   float r;
@@ -150,35 +182,71 @@ __device__ __forceinline__ void i8_store16(const I8Params& p, const int* to, int
 }
 
 struct I8Item {
-  int n0, a_row, e;        // first result, first row in the weights (gate and up: of the gate), expert
+  int n0, a_row, e;        // this CTA's first result, first row in the weights (gate and up: of the gate), expert
   int x0, rows;            // tokens
 };
-// (waited: behind this thread's pdl_wait)
-template <bool GLU> __device__ __forceinline__ I8Item i8_item(const I8Params& p, int i, bool waited) {
+// Item i.  (waited: behind this thread's pdl_wait.)
+template <bool GLU, bool PAIR> __device__ __forceinline__ I8Item i8_item(const I8Params& p, int i, int rank, bool waited) {
+  constexpr int PER = GLU ? I8_ROWS / 2 : I8_ROWS;
   I8Item t;
+  int tile;
   if (p.passes) {
-    const int4 q = waited ? p.passes[i / p.rt] : ld_older(p.passes + i / p.rt);
+    const int pass = (int)((unsigned)i / (unsigned)p.rt);
+    const int4 q = waited ? p.passes[pass] : ld_older(p.passes + pass);
+    tile = i - pass * p.rt;
     t.e = q.x;
-    t.n0 = i % p.rt * (GLU ? I8_ROWS / 2 : I8_ROWS);
-    t.a_row = q.x * p.w_rows + t.n0;
     t.x0 = q.y;
     t.rows = q.z;
   } else {   // the token tiles of a row tile are neighbours
+    tile = (int)((unsigned)i / (unsigned)p.tt);
     t.e = 0;
-    t.a_row = t.n0 = i / p.tt * I8_ROWS;
-    t.x0 = i % p.tt * p.tn;
+    t.x0 = (i - tile * p.tt) * p.tn;
     t.rows = min(p.tn, p.m - t.x0);
   }
+  t.n0 = PAIR ? (2 * tile + rank) * PER : tile * PER;
+  t.a_row = t.e * p.w_rows + t.n0;
   return t;
 }
-// The weights of a stage: 128 rows, or four times 16 gate rows and the 16 up rows that go with them
-template <bool GLU> __device__ __forceinline__ void i8_weights(const CUtensorMap* map, uint32_t at, int kb, const I8Item& t, uint32_t bar) {
-  if (GLU) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) i8_box3(at + (uint32_t)(g * 32 * I8_BK), map, kb * I8_BK, t.n0 + 16 * g, 2 * t.e, bar);
-  } else {
-    i8_box(at, map, kb * I8_BK, t.a_row, bar);
+constexpr int I8_LIST = 128;   // items of a CTA that are worked out ahead, in shared memory: {a_row, x0, rows, e}
+template <bool GLU, bool PAIR> __device__ __forceinline__ I8Item i8_item(const I8Params& p, const int4* list, int i, int j, int rank, bool waited) {
+  if (j >= I8_LIST) return i8_item<GLU, PAIR>(p, i, rank, waited);
+  const int4 q = list[j];
+  I8Item t;
+  t.a_row = q.x;
+  t.x0 = q.y;
+  t.rows = q.z;
+  t.e = q.w;
+  t.n0 = q.x - q.w * p.w_rows;
+  return t;
+}
+
+// A copy is one box wherever it can be: boxes of a few KB cost the copy engine as much as one of 16 KB.  (The weights of a stage in four
+// boxes, its tokens in up to four of 64 rows: 87 us for the gate and up products of 2048 tokens over 64 experts of 2048x1024.)
+struct I8Maps {
+  CUtensorMap w, q[5];   // tokens: boxes of 256, 128, 64, 32, 16 rows for experts; dense: q[0], tn rows
+};
+// The weights of a stage: 128 rows, or eight times 8 gate rows and the 8 up rows that go with them
+template <bool GLU, bool PAIR> __device__ __forceinline__ void i8_weights(const I8Maps& maps, uint32_t at, int kb, const I8Item& t, uint32_t bar) {
+  if (GLU) i8_box5<PAIR>(at, &maps.w, kb * I8_BK, t.n0 / 8, t.e, bar);
+  else i8_box<PAIR>(at, &maps.w, kb * I8_BK, t.a_row, bar);
+}
+// Columns of an item's instructions, and the rows of tokens that a CTA's stage takes for them: all, or a pair's half
+template <bool PAIR> __device__ __forceinline__ int i8_columns(const I8Params& p, const I8Item& t) {
+  return !p.passes ? p.tn : PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15;
+}
+template <bool PAIR> __device__ __forceinline__ void i8_tokens(const I8Params& p, const I8Maps& maps, uint32_t at, int kb, const I8Item& t, int rank, uint32_t bar) {
+  const int rows = i8_columns<PAIR>(p, t) >> (PAIR ? 1 : 0), x0 = t.x0 + (PAIR ? rank * rows : 0);
+  if (!p.passes) {
+    i8_box<PAIR>(at, &maps.q[0], kb * I8_BK, x0, bar);
+    return;
   }
+  int y = 0;
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+    if (rows & 256 >> i) {
+      i8_box<PAIR>(at + (uint32_t)(y * I8_BK), &maps.q[i], kb * I8_BK, x0 + y, bar);
+      y += 256 >> i;
+    }
 }
 
 // Codes of the tokens and their scales, by the 512 threads of the epilogue: a token's threads (all of them for one token, two warps each for
@@ -214,10 +282,9 @@ template <typename T> __device__ __forceinline__ void i8_few_codes(const I8Param
   }
 }
 
-// GLU: gate and up product of experts.  FEW: float (or void: not so), __half, __nv_bfloat16: up to eight tokens of that type
-template <bool GLU, typename FewT = void>
-__global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
-                                                           const __grid_constant__ I8Params p) {
+// GLU: gate and up product of experts.  FewT: float, __half, __nv_bfloat16: up to eight tokens of that type (void: not so).  PAIR: by pairs of CTAs
+template <bool GLU, bool PAIR, typename FewT>
+__global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant__ I8Maps maps, const __grid_constant__ I8Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // (from the shared-window address, so that the CTAs of a cluster agree about offsets)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -228,6 +295,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
   float* s_scale = reinterpret_cast<float*>(smem + p.aux_off + 512);   // [2][256]
   int* s_row = reinterpret_cast<int*>(s_scale + 512);                  // [2][256]
   uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_row + 512);          // [I8_EPI][1024]
+  int4* s_list = reinterpret_cast<int4*>(s_stage + I8_EPI * 1024);     // [I8_LIST]
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr bool FEW = !std::is_void<FewT>::value;
   uint64_t* coded = accum + 6;   // FEW: the codes are there
@@ -240,83 +308,108 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&accum[s], 1);
-      mbar_init(&drained[s], I8_EPI);
+      mbar_init(&drained[s], PAIR ? 2 * I8_EPI : I8_EPI);
     }
     *gave_up = 0;
     fence_barrier_init();
   }
-  if (p.split > 1) cluster_arrive();   // (waited for before anything is sent)
-  if (warp == 2) {
-    tmem_alloc(tmem_slot, p.tmem_cols);
-    tmem_relinquish();
-  }
+  if (!PAIR && p.split > 1) cluster_arrive();   // (waited for before anything is sent)
+  if (warp == 2) i8_tmem_alloc<PAIR>(tmem_slot, 512);
+  // (The MMA issuer's control flow and operands have to be known to be the same for all lanes, so that they stay in uniform registers: from a
+  // loop that the compiler takes for divergent an MMA takes 115 clocks, however few its tokens.  Hence the rank from the block's number, sums
+  // over the warp for what comes from memory -- a reduction's result is uniform --, and all of the tensor memory, which starts at 0.)
+  const uint32_t rank = blockIdx.x & (uint32_t)(PAIR ? 1 : p.split - 1);
+  constexpr int CTAS = PAIR ? 2 : 1;
+  const int first = !PAIR && p.split > 1 ? (int)blockIdx.x / p.split : (int)blockIdx.x / CTAS, step = !PAIR && p.split > 1 ? 1 << 30 : (int)gridDim.x / CTAS;
+  const int kb0 = !PAIR && p.split > 1 ? (int)(p.nk * rank) / p.split : 0, kb1 = !PAIR && p.split > 1 ? (int)(p.nk * (rank + 1)) / p.split : p.nk;
+  // (the work list is older than the trigger of the kernel ahead: see pdl_wait)
+  const int n_items = (int)__reduce_max_sync(0xffffffffu, (unsigned)(p.passes ? ld_older(p.n_passes) * p.rt : p.rt * p.tt));
+  if (p.passes && warp == 3)
+    for (int j = lane; j < I8_LIST && first + j * step < n_items; j += 32) {
+      const I8Item t = i8_item<GLU, PAIR>(p, first + j * step, (int)rank, false);
+      s_list[j] = make_int4(t.a_row, t.x0, t.rows, t.e);
+    }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) {   // (the partner's barriers and tensor memory are there)
+    cluster_arrive();
+    cluster_wait();
+  }
   tc_fence_after();
-  // (From lane 0 to all: the compiler then knows that a warp's lanes agree, and keeps what follows from it in uniform registers.  With a
-  // loop that it takes for divergent, an MMA takes 115 clocks however few its tokens are.)
-  const uint32_t rank = p.split > 1 ? __shfl_sync(0xffffffffu, cluster_rank(), 0) : 0u;
   pdl_trigger();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), gave_up_s = smem_u32(const_cast<const int*>(gave_up)), full_s = smem_u32(full), empty_s = smem_u32(empty);
+  constexpr uint32_t tmem = 0;
+  const uint32_t gave_up_s = smem_u32(const_cast<const int*>(gave_up)), full_s = smem_u32(full), empty_s = smem_u32(empty);
   const uint32_t accum_s = smem_u32(accum), drained_s = smem_u32(drained);
-  const int first = p.split > 1 ? (int)blockIdx.x / p.split : (int)blockIdx.x, step = p.split > 1 ? 1 << 30 : (int)gridDim.x;
-  const int kb0 = p.split > 1 ? (int)(p.nk * rank) / p.split : 0, kb1 = p.split > 1 ? (int)(p.nk * (rank + 1)) / p.split : p.nk;
-  // (the work list is older than the trigger of the kernel ahead: see pdl_wait)
-  const int n_items = p.passes ? __shfl_sync(0xffffffffu, ld_older(p.n_passes), 0) * p.rt : p.rt * p.tt;
+  auto item = [&](int i, int j, bool waited) { return p.passes ? i8_item<GLU, PAIR>(p, s_list, i, j, (int)rank, waited) : i8_item<GLU, PAIR>(p, i, (int)rank, waited); };
 
-  if (warp == 0) {
-    // ---------------- loader ----------------
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ---------------- loaders ----------------
+    // Three warps take the stages in turn: a stage's wait, announcement and two copies take one warp 440 clocks to issue, most of the 512
+    // that the tensor core takes for 256 tokens.  (One loader: 470 clocks a stage from one token to 128.)
+    constexpr int LOADERS = 3;
     const uint32_t lead = elect_one() ? 1u : 0u, ring = smem_u32(smem);
-    int s = 0, ahead = 0;
+    const int nkb = kb1 - kb0;
+    int k = warp == 0 ? 0 : warp - 1, s = k, i = first, j = 0;   // stage of the item, slot, item, its number
     uint32_t ph = 0;
-    if (first < n_items) {   // the first weights before the activations are there: into the ring, or, if they may still be written, into L2
-      const I8Item t = i8_item<GLU>(p, first, false);
-      const uint32_t bytes = (uint32_t)(I8_A_BYTES + (FEW ? 0 : (t.rows + p.bh - 1) / p.bh * p.bh * I8_BK));
-      ahead = FEW && !p.settled ? kb1 - kb0 : min(p.stages, kb1 - kb0);
-      for (int j = 0; j < ahead; ++j)
+    auto next_item = [&] {
+      while (k >= nkb && i < n_items) {
+        k -= nkb;
+        i += step;
+        ++j;
+      }
+    };
+    // The first weights before the activations are there: into the ring, or, if they may still be written, into L2.
+    int ahead = 0;
+    if (first < n_items) {
+      const I8Item t = item(first, 0, false);
+      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns<PAIR>(p, t) * I8_BK));   // (a pair's, on the first CTA's barrier)
+      ahead = FEW && !p.settled ? nkb : min(p.stages, nkb);
+      for (int g = k; g < ahead; g += LOADERS)
         if (lead) {
           if (p.settled) {
-            mbar_expect_tx(full_s + 8u * j, bytes);
-            i8_weights<GLU>(&amap, ring + (uint32_t)(j * p.stage_bytes), kb0 + j, t, full_s + 8u * j);
+            if (rank == 0 || !PAIR) mbar_expect_tx(full_s + 8u * g, bytes);
+            i8_weights<GLU, PAIR>(maps, ring + (uint32_t)(g * p.stage_bytes), kb0 + g, t, full_s + 8u * g);
           } else {
-            i8_box_l2(&amap, (kb0 + j) * I8_BK, t.a_row);
+            i8_box_l2(&maps.w, (kb0 + g) * I8_BK, t.a_row);
           }
         }
       if (!p.settled) ahead = 0;
     }
     pdl_wait();
-    for (int i = first; i < n_items; i += step) {
-      const I8Item t = i8_item<GLU>(p, i, true);
-      const int boxes = FEW ? 0 : (t.rows + p.bh - 1) / p.bh;
-      for (int kb = kb0; kb < kb1; ++kb) {
+    next_item();
+    while (i < n_items) {
+      const I8Item t = item(i, j, true);
+      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns<PAIR>(p, t) * I8_BK));
+      for (; k < nkb; k += LOADERS) {
         const uint32_t fb = full_s + 8u * s, at = ring + (uint32_t)(s * p.stage_bytes);
-        if (ahead == 0) {
-          mbar_wait_or(empty_s + 8u * s, ph ^ 1u, gave_up_s);
-          if (lds32(gave_up_s) != 0u) goto loaded;   // (no copy into a slot that may be in use)
+        const bool weights = j > 0 || k >= ahead;
+        if (weights) {
+          if (!i8_wait(empty_s + 8u * s, ph ^ 1u, gave_up_s)) goto loaded;   // (no copy into a slot that may be in use)
           __syncwarp();
-          if (lead) {
-            mbar_expect_tx(fb, (uint32_t)(I8_A_BYTES + boxes * p.bh * I8_BK));
-            i8_weights<GLU>(&amap, at, kb, t, fb);
-          }
-        } else {
-          --ahead;
         }
-        if (lead)
-          for (int b = 0; b < boxes; ++b) i8_box(at + (uint32_t)(I8_A_BYTES + b * p.bh * I8_BK), &bmap, kb * I8_BK, t.x0 + b * p.bh, fb);
-        if (++s == p.stages) { s = 0; ph ^= 1u; }
+        if (lead) {
+          if (weights) {
+            if (rank == 0 || !PAIR) mbar_expect_tx(fb, bytes);
+            i8_weights<GLU, PAIR>(maps, at, kb0 + k, t, fb);
+          }
+          if (!FEW) i8_tokens<PAIR>(p, maps, at + I8_A_BYTES, kb0 + k, t, (int)rank, fb);
+        }
+        s += LOADERS;
+        if (s >= p.stages) { s -= p.stages; ph ^= 1u; }
       }
+      next_item();
     }
   loaded:;
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
+  } else if (warp == 1 && (rank == 0 || !PAIR)) {
+    // ---------------- MMA issuer (of a pair, the first CTA's) ----------------
     const uint32_t lead = elect_one() ? 1u : 0u;
     const uint64_t d0 = umma_desc_sw128(smem_u32(smem));
     const uint32_t lo0 = (uint32_t)d0, hi = (uint32_t)(d0 >> 32), stage16 = (uint32_t)p.stage_bytes >> 4;
     int s = 0, buf = 0;
     uint32_t ph = 0, dph = 0;
-    for (int i = first; i < n_items; i += step) {
-      const int cols = (__shfl_sync(0xffffffffu, i8_item<GLU>(p, i, false).rows, 0) + 15) & ~15;
-      const uint32_t idesc = i8_idesc(cols), d = tmem + (uint32_t)(buf * p.tn);
+    for (int i = first, j = 0; i < n_items; i += step, ++j) {
+      const int cols = (int)__reduce_max_sync(0xffffffffu, (unsigned)i8_columns<PAIR>(p, item(i, j, false)));
+      const uint32_t idesc = i8_idesc(PAIR, cols), d = tmem + (uint32_t)(buf * p.tn);
       const uint32_t codes0 = (uint32_t)umma_desc_sw128(smem_u32(smem + p.codes_off));
       if (FEW) mbar_wait_or(smem_u32(coded), 0u, gave_up_s);
       mbar_wait_or(drained_s + 8u * buf, dph ^ 1u, gave_up_s);
@@ -325,11 +418,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
         __syncwarp();
         tc_fence_after();
         const uint32_t a = lo0 + (uint32_t)s * stage16;
-        umma_i8_ss4(d, a, FEW ? codes0 + (uint32_t)(kb - kb0) * (2048 >> 4) : a + (I8_A_BYTES >> 4), hi, idesc, kb > kb0, lead);
-        umma_commit(empty_s + 8u * s, lead);
+        umma_i8_ss4<PAIR>(d, a, FEW ? codes0 + (uint32_t)(kb - kb0) * (2048 >> 4) : a + (I8_A_BYTES >> 4), hi, idesc, kb > kb0, lead);
+        i8_commit<PAIR>(empty_s + 8u * s, lead);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
-      umma_commit(accum_s + 8u * buf, lead);
+      i8_commit<PAIR>(accum_s + 8u * buf, lead);
       if (++buf == p.nbuf) { buf = 0; dph ^= 1u; }
     }
     __syncwarp();
@@ -343,8 +436,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     int buf = 0, turn = 0;
     uint32_t aph = 0;
     pdl_wait();
-    for (int i = first; i < n_items; i += step) {
-      const I8Item t = i8_item<GLU>(p, i, true);
+    for (int i = first, j = 0; i < n_items; i += step, ++j) {
+      const I8Item t = item(i, j, true);
       float* xs = s_scale + (FEW ? 0 : turn * 256);   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
       int* xr = s_row + turn * 256;
       turn ^= 1;
@@ -360,10 +453,10 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(coded);
       }
-      // this lane's row: of 128, or, gate and up, lanes 0 to 15 a gate row and lanes 16 to 31 its up row
-      const int r = GLU ? quad / 2 + (lane & 15) : row, n = t.n0 + r;
+      // this lane's row: of 128, or, gate and up, of 64 gate rows or (lanes with bit 3) their up rows
+      const int r = GLU ? quad / 2 + (lane >> 4) * 8 + (lane & 7) : row, n = t.n0 + r;
       const bool live = n < p.n, wide = wide_y && t.n0 + quad + 32 <= p.n;
-      float ws = live ? p.w_scale[t.a_row + r + (GLU && lane >= 16 ? p.n : 0)] : 0.f;
+      float ws = live ? p.w_scale[t.a_row + r + (GLU && (lane & 8) ? p.n : 0)] : 0.f;
       if (down) ws = ws * p.w_unit[t.e] * p.unit;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
@@ -384,11 +477,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
           for (int j = 0; j < 16; ++j) f[j] = (float)(int)v[j] * (reinterpret_cast<const float*>(x)[j] * ws) + bias;
           const int count = min(16, t.rows - c0);
           if (GLU) {   // of two tokens, the lanes of the gate take the first and those of up the second
-            const bool up = lane >= 16;
+            const bool up = (lane & 8) != 0;
             float g[8], u[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float got = __shfl_xor_sync(0xffffffffu, up ? f[2 * j] : f[2 * j + 1], 16);
+              const float got = __shfl_xor_sync(0xffffffffu, up ? f[2 * j] : f[2 * j + 1], 8);
               g[j] = up ? got : f[2 * j];
               u[j] = up ? f[2 * j + 1] : got;
             }
@@ -410,13 +503,18 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(drained_s + 8u * buf);
+        if (lane == 0) {
+          if (PAIR)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"((drained_s + 8u * buf) & I8_LEADER) : "memory");
+          else
+            mbar_arrive(drained_s + 8u * buf);
+        }
       }
       if (++buf == p.nbuf) { buf = 0; aph ^= 1u; }
     }
   }
   __syncwarp();
-  if (!GLU && p.split > 1) {
+  if (!GLU && !PAIR && p.split > 1) {
     // ---------------- split: the sums of rows [per * rank, per * (rank + 1)) of the tile are this CTA's to add and store ----------------
     // The rows of another CTA go into its shared memory, [sender][row][token], rows 16 bytes more than tn words apart (eight lanes' 16 bytes then
     // lie in different banks).  A lane keeps its row to the end.
@@ -425,7 +523,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
       cluster_arrive();
       cluster_wait();
     }
-    const I8Item t = i8_item<false>(p, first, true);
+    const I8Item t = i8_item<false, false>(p, first, 0, true);
     const int per = I8_ROWS / p.split, shift = 31 - __clz(per), quad = (warp & 3) * 32, row = quad + lane, owner = row >> shift;
     const int turn16 = 16 * ((warp - 4) >> 2);
     const uint32_t d = tmem + ((uint32_t)quad << 16), pitch = 4u * (uint32_t)p.tn + 16u, ring = smem_u32(smem + p.recv_off);
@@ -480,10 +578,12 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     if (threadIdx.x == 0) atomicExch(p.status, E_TIMEOUT);
     // A bounded wait ran out in this CTA.  What it started has to finish before its tensor memory is given up: the commit covers the
     // tensor pipe, and the copies in flight land within microseconds.
-    if (warp == 1) {
+    if (warp == 1 && (rank == 0 || !PAIR)) {
       if (lane == 0) mbar_init(last, 1);
       __syncwarp();
-      if (elect_one()) umma_commit(last);
+      if (PAIR) {
+        if (elect_one()) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(last)) : "memory");
+      } else if (elect_one()) umma_commit(last);
       __syncwarp();
       mbar_wait_bounded(last, 0);
     }
@@ -491,38 +591,76 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     tc_fence_before();
     __syncthreads();
   }
-  if (warp == 2) tmem_dealloc(tmem, p.tmem_cols);
+  if (PAIR) {   // (the partner's shared memory and tensor memory are in use until here)
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == 2) i8_tmem_dealloc<PAIR>(tmem, 512);
 }
 
-// rows of k bytes; planes > 0: as [planes][rows / planes], boxes of box_rows rows of two planes
-static bool i8_map(CUtensorMap& map, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows, int64_t planes = 0) {
+// rows of k bytes in boxes of box_rows; experts > 0: [experts][gate, up][rows / 8][8] in boxes of eight times 8 gate and 8 up rows
+static bool i8_map(CUtensorMap& map, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows, int64_t experts = 0) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (!enc) return false;
-  const int64_t per = planes ? rows / planes : rows;
-  const cuuint64_t dims[3] = {(cuuint64_t)k, (cuuint64_t)per, (cuuint64_t)planes}, strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(per * pitch)};
-  const cuuint32_t box[3] = {I8_BK, (cuuint32_t)box_rows, 2}, one[3] = {1, 1, 1};
-  return enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  auto encode = [&](int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    return enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (experts) {
+    const cuuint64_t dims[5] = {(cuuint64_t)k, 8, 2, (cuuint64_t)rows / 8, (cuuint64_t)experts};
+    const cuuint64_t strides[4] = {(cuuint64_t)pitch, (cuuint64_t)(rows * pitch), (cuuint64_t)(8 * pitch), (cuuint64_t)(2 * rows * pitch)};
+    const cuuint32_t box[5] = {I8_BK, 8, 2, 8, 1};
+    return encode(5, dims, strides, box);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {I8_BK, (cuuint32_t)box_rows};
+  return encode(2, dims, strides, box);
 }
 
-template <bool GLU, typename FewT> static int i8_launch(const CUtensorMap& amap, const CUtensorMap& bmap, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
+template <bool GLU, bool PAIR, typename FewT> static int i8_launch(const I8Maps& maps, const I8Params& p, int grid, size_t smem, cudaStream_t stream) {
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return E_CUDA;
   if (!configured[dev & 63]) {
-    if (cudaFuncSetAttribute(i8_kernel<GLU, FewT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
+    if (cudaFuncSetAttribute(i8_kernel<GLU, PAIR, FewT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return E_CUDA;
     configured[dev & 63] = true;
   }
-  return launch_pdl_cluster(i8_kernel<GLU, FewT>, dim3((unsigned)grid), dim3(I8_THREADS), (unsigned)p.split, smem, stream, amap, bmap, p) == cudaSuccess ? E_OK : E_CUDA;
+  return launch_pdl_cluster(i8_kernel<GLU, PAIR, FewT>, dim3((unsigned)grid), dim3(I8_THREADS), PAIR ? 2u : (unsigned)p.split, smem, stream, maps, p) == cudaSuccess ? E_OK : E_CUDA;
 }
 
-// CTAs that share a tile: as many as there are SMs for, while the stages that each is spared take longer than the exchange.  (A stage takes 0.25
-// to 0.35 us; sharing by two, 1 us + 0.025 us a token.  Whole / by 2 / by 4 in us: 1 token of 4096x4096 10.6 / 8.7 / 7.7, 128 tokens 12.1 /
-// 11.8 / 12.2, 500 tokens 15.3 / 17.1, of 4096x14336 40.8 / 30.9.)
-static int i8_split(int64_t tiles, int nk, int tn) {
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= I8_SMS && nk / (2 * split) > 5 + tn / 14) split *= 2;
-  return split;
+// How a dense product is dealt out: tokens a tile, whether pairs of CTAs take 256 rows together, how many CTAs share a tile's K.  What takes
+// the least time by this model, in us on a chip that is not held back by its power limit: a stage 0.08 + 0.00094 a token (a pair: 0.065 +
+// 0.00092), 5 for start and end (a pair 0.8 more), 0.012 a token for the last tile's way out, 1 + 0.025 a token for an exchange of sums.
+// Measured, single / pair / shared by two: 500 tokens of 4096x14336 27.5 (tiles of 128) / 25.9 (128) / 30.4 (256); of 4096x4096 10.7 / 11.5 /
+// 17.1; of 14336x4096 28.7 (256) / 26.1 (256); 1000 tokens of 4096x4096 16.3 (256) / 16.6 (128); 4096 tokens of 14336x4096 173 / 149;
+// 1 token of 4096x4096 whole 10.6, by two 8.7, by four 7.7.
+struct I8Deal {
+  int tn, tt, split;
+  bool pair;
+};
+static I8Deal i8_deal(int64_t m, int64_t n, int nk) {
+  I8Deal best{};
+  float least = INFINITY;
+  for (int most = 256; most >= 32; most -= 32) {
+    const int64_t tt = (m + most - 1) / most, each = (m + tt - 1) / tt;
+    if (tt > 1 && most < 256 && tt == (m + most + 31) / (most + 32)) continue;   // (as the tile size before)
+    for (int pair = 0; pair < 2; ++pair) {
+      const int tn = (int)round_up(each, pair ? 32 : 16), rows = pair ? 2 * I8_ROWS : I8_ROWS;
+      const int64_t tiles = (n + rows - 1) / rows * tt, slots = pair ? I8_SMS / 2 : I8_SMS;
+      for (int split = 1; split <= (pair ? 1 : 8) && (split == 1 || (tiles * split <= slots && nk >= 4 * split)); split *= 2) {
+        const float stage = pair ? 0.065f + 0.00092f * tn : 0.08f + 0.00094f * tn;
+        const int64_t waves = split > 1 ? 1 : (tiles + slots - 1) / slots;
+        const float t = waves * ((nk + split - 1) / split) * stage + (pair ? 0.8f : 0.f) + 0.012f * tn + (split > 1 ? 1.f + 0.025f * tn : 0.f);
+        if (t < least) {
+          least = t;
+          best = I8Deal{tn, (int)tt, split, pair != 0};
+        }
+      }
+    }
+    if (each <= 32) break;
+  }
+  return best;
 }
 // Whether a product of m tokens is one launch: rows that 16-byte loads can start at, the codes of a CTA's K (2 KB a stage) leave half of its
 // shared memory to the weights, and finding the tokens' largest values, which every CTA repeats, takes less than a launch.  (One / two
@@ -532,7 +670,7 @@ constexpr int64_t I8_FEW_VALUES = 16384;
 bool i8_few(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k) {
   const int64_t size = dtype == DT_F32 ? 4 : 2, nk = (k + I8_BK - 1) / I8_BK;
   if (m > I8_FEW || m * k > I8_FEW_VALUES || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || (m > 1 && ldx * size % 16 != 0)) return false;
-  const int split = i8_split((n + I8_ROWS - 1) / I8_ROWS, (int)nk, 16);
+  const int split = i8_deal(m, n, (int)nk).split;
   return (nk + split - 1) / split <= 48;
 }
 
@@ -545,19 +683,15 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.k = (int)a.k;
   p.nk = (int)((a.k + I8_BK - 1) / I8_BK);
   p.m = (int)a.m;
-  p.rt = (int)((a.n + per_tile - 1) / per_tile);
-  if (a.passes) {
-    p.tn = (int)a.pass_rows;
-    p.tt = 1;
-  } else {
-    p.tt = (int)((a.m + 255) / 256);
-    p.tn = (int)round_up((a.m + p.tt - 1) / p.tt, 16);
-  }
-  p.bh = !a.passes || p.tn <= 64 ? p.tn : 64;
-  p.stage_bytes = I8_A_BYTES + (few ? 0 : (int)round_up(p.tn, p.bh) * I8_BK);
+  const I8Deal deal = a.passes ? I8Deal{(int)round_up(a.pass_rows, 32), 1, 1, false} : i8_deal(a.m, a.n, p.nk);
+  const bool pair = deal.pair;
+  p.rt = (int)((a.n + per_tile * (pair ? 2 : 1) - 1) / (per_tile * (pair ? 2 : 1)));
+  p.tn = deal.tn;
+  p.tt = deal.tt;
+  p.split = deal.split;
+  p.stage_bytes = I8_A_BYTES + (few ? 0 : p.tn * I8_BK / (pair ? 2 : 1));
   const int64_t tiles = a.passes ? a.max_passes * p.rt : (int64_t)p.rt * p.tt;
   if (tiles > 1 << 29) return E_TOO_LARGE;
-  p.split = a.passes ? 1 : i8_split(tiles, p.nk, p.tn);
   // shared memory: ring, barriers and scales, codes of a few tokens, sums of other CTAs where they are small
   const int recv = p.split > 1 ? I8_ROWS / p.split * (p.split - 1) * (4 * p.tn + 16) : 0;
   const int codes = few ? (p.nk + p.split - 1) / p.split * 2048 : 0;
@@ -569,8 +703,6 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.recv_off = recv > 0 && recv <= 32768 ? ring + codes : 0;
   p.aux_off = ring + extra - I8_AUX;
   p.nbuf = p.split == 1 && 2 * p.tn <= 512 ? 2 : 1;
-  p.tmem_cols = 32;
-  while ((int)p.tmem_cols < p.nbuf * p.tn) p.tmem_cols *= 2;
   p.y = a.y;
   p.ldy = a.ldy;
   p.dtype = a.dtype;
@@ -587,18 +719,19 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.x = a.x;
   p.ldx = a.ldx;
   p.status = a.status;
-  const int64_t grid = p.split > 1 ? tiles * p.split : tiles < I8_SMS ? tiles : I8_SMS;
-  CUtensorMap amap, bmap;
-  if (!i8_map(amap, a.w, a.k, a.experts * p.w_rows, a.ldw, glu ? 16 : I8_ROWS, glu ? 2 * a.experts : 0)) return E_CUDA;
-  if (few) bmap = amap;   // (not read)
-  else if (!i8_map(bmap, a.q, a.k, a.m, a.ldq, p.bh)) return E_CUDA;
+  const int64_t slots = pair ? I8_SMS / 2 : I8_SMS, grid = p.split > 1 ? tiles * p.split : (tiles < slots ? tiles : slots) * (pair ? 2 : 1);
+  I8Maps maps;
+  if (!i8_map(maps.w, a.w, a.k, glu ? a.n : a.experts * p.w_rows, a.ldw, I8_ROWS, glu ? a.experts : 0)) return E_CUDA;
+  for (int i = 0; i < (few ? 0 : a.passes ? 5 : 1); ++i)
+    if (!i8_map(maps.q[i], a.q, a.k, a.m, a.ldq, a.passes ? 256 >> i : p.tn / (pair ? 2 : 1))) return E_CUDA;
   const size_t smem = 1024 + (size_t)p.aux_off + I8_AUX;
-  if (glu) return i8_launch<true, void>(amap, bmap, p, (int)grid, smem, stream);
-  if (!few) return i8_launch<false, void>(amap, bmap, p, (int)grid, smem, stream);
+  if (glu) return pair ? i8_launch<true, true, void>(maps, p, (int)grid, smem, stream) : i8_launch<true, false, void>(maps, p, (int)grid, smem, stream);
+  if (pair) return i8_launch<false, true, void>(maps, p, (int)grid, smem, stream);
+  if (!few) return i8_launch<false, false, void>(maps, p, (int)grid, smem, stream);
   switch (a.dtype) {
-    case DT_F32: return i8_launch<false, float>(amap, bmap, p, (int)grid, smem, stream);
-    case DT_F16: return i8_launch<false, __half>(amap, bmap, p, (int)grid, smem, stream);
-    default: return i8_launch<false, __nv_bfloat16>(amap, bmap, p, (int)grid, smem, stream);
+    case DT_F32: return i8_launch<false, false, float>(maps, p, (int)grid, smem, stream);
+    case DT_F16: return i8_launch<false, false, __half>(maps, p, (int)grid, smem, stream);
+    default: return i8_launch<false, false, __nv_bfloat16>(maps, p, (int)grid, smem, stream);
   }
 }
 

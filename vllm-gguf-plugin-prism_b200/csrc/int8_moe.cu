@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
 int64_t i8_moe_pass_rows(int64_t slots, int64_t experts) {
   const double mean = (double)slots / (double)experts;
   const int64_t rows = round_up((int64_t)(mean + 3.0 * sqrt(mean)) + 1, 16);
-  return rows <= 64 ? rows : rows <= 256 ? round_up(rows, 64) : 256;
+  return rows < 256 ? rows : 256;
 }
 int64_t i8_moe_passes(int64_t slots, int64_t experts, int64_t pass_rows) {
   const int64_t worst = slots / pass_rows + experts;
