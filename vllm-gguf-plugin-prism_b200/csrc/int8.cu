@@ -107,21 +107,29 @@ template <bool PAIR> __device__ __forceinline__ void i8_tmem_dealloc(uint32_t at
 }
 constexpr uint32_t I8_LEADER = 0xFEFFFFFFu;   // of a shared-memory address in a cluster of two: the same place in the first CTA
 // (GROUP 2: a pair's copies, each into its own shared memory, may count on the first CTA's barrier)
-template <bool PAIR> __device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+template <bool PAIR> __device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t keep) {
   if (PAIR)
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(y), "l"(keep) : "memory");
   else
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "l"(keep) : "memory");
 }
-template <bool PAIR> __device__ __forceinline__ void i8_box5(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+template <bool PAIR> __device__ __forceinline__ void i8_box5(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar, uint64_t keep) {
   if (PAIR)
-    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(0), "r"(y), "r"(z) : "memory");
+    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %4, %5, %6}], [%2], %7;"
+                 ::"r"(dst), "l"(map), "r"(bar & I8_LEADER), "r"(x), "r"(0), "r"(y), "r"(z), "l"(keep) : "memory");
   else
-    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(0), "r"(y), "r"(z) : "memory");
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %4, %5, %6}], [%2], %7;"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(0), "r"(y), "r"(z), "l"(keep) : "memory");
+}
+// How long L2 should keep what a copy brings: weights that no other tile asks for leave first, so that what the next kernel reads stays (an
+// expert step of 2048 tokens moves 130 MB of hidden rows and results through L2 between its kernels)
+__device__ __forceinline__ uint64_t i8_policy(bool once) {
+  uint64_t p;
+  if (once) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  else asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 __device__ __forceinline__ void i8_box_l2(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
@@ -226,25 +234,25 @@ struct I8Maps {
   CUtensorMap w, q[5];   // tokens: boxes of 256, 128, 64, 32, 16 rows for experts; dense: q[0], tn rows
 };
 // The weights of a stage: 128 rows, or eight times 8 gate rows and the 8 up rows that go with them
-template <bool GLU, bool PAIR> __device__ __forceinline__ void i8_weights(const I8Maps& maps, uint32_t at, int kb, const I8Item& t, uint32_t bar) {
-  if (GLU) i8_box5<PAIR>(at, &maps.w, kb * I8_BK, t.n0 / 8, t.e, bar);
-  else i8_box<PAIR>(at, &maps.w, kb * I8_BK, t.a_row, bar);
+template <bool GLU, bool PAIR> __device__ __forceinline__ void i8_weights(const I8Maps& maps, uint32_t at, int kb, const I8Item& t, uint32_t bar, uint64_t keep) {
+  if (GLU) i8_box5<PAIR>(at, &maps.w, kb * I8_BK, t.n0 / 8, t.e, bar, keep);
+  else i8_box<PAIR>(at, &maps.w, kb * I8_BK, t.a_row, bar, keep);
 }
 // Columns of an item's instructions, and the rows of tokens that a CTA's stage takes for them: all, or a pair's half
 template <bool PAIR> __device__ __forceinline__ int i8_columns(const I8Params& p, const I8Item& t) {
   return !p.passes ? p.tn : PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15;
 }
-template <bool PAIR> __device__ __forceinline__ void i8_tokens(const I8Params& p, const I8Maps& maps, uint32_t at, int kb, const I8Item& t, int rank, uint32_t bar) {
+template <bool PAIR> __device__ __forceinline__ void i8_tokens(const I8Params& p, const I8Maps& maps, uint32_t at, int kb, const I8Item& t, int rank, uint32_t bar, uint64_t keep) {
   const int rows = i8_columns<PAIR>(p, t) >> (PAIR ? 1 : 0), x0 = t.x0 + (PAIR ? rank * rows : 0);
   if (!p.passes) {
-    i8_box<PAIR>(at, &maps.q[0], kb * I8_BK, x0, bar);
+    i8_box<PAIR>(at, &maps.q[0], kb * I8_BK, x0, bar, keep);
     return;
   }
   int y = 0;
 #pragma unroll
   for (int i = 0; i < 5; ++i)
     if (rows & 256 >> i) {
-      i8_box<PAIR>(at + (uint32_t)(y * I8_BK), &maps.q[i], kb * I8_BK, x0 + y, bar);
+      i8_box<PAIR>(at + (uint32_t)(y * I8_BK), &maps.q[i], kb * I8_BK, x0 + y, bar, keep);
       y += 256 >> i;
     }
 }
@@ -349,6 +357,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     constexpr int LOADERS = 3;
     const uint32_t lead = elect_one() ? 1u : 0u, ring = smem_u32(smem);
     const int nkb = kb1 - kb0;
+    const uint64_t weights_stay = i8_policy(p.tt == 1), tokens_stay = i8_policy(false);
     int k = warp == 0 ? 0 : warp - 1, s = k, i = first, j = 0;   // stage of the item, slot, item, its number
     uint32_t ph = 0;
     auto next_item = [&] {
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
         if (lead) {
           if (p.settled) {
             if (rank == 0 || !PAIR) mbar_expect_tx(full_s + 8u * g, bytes);
-            i8_weights<GLU, PAIR>(maps, ring + (uint32_t)(g * p.stage_bytes), kb0 + g, t, full_s + 8u * g);
+            i8_weights<GLU, PAIR>(maps, ring + (uint32_t)(g * p.stage_bytes), kb0 + g, t, full_s + 8u * g, weights_stay);
           } else {
             i8_box_l2(&maps.w, (kb0 + g) * I8_BK, t.a_row);
           }
@@ -390,9 +399,9 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
         if (lead) {
           if (weights) {
             if (rank == 0 || !PAIR) mbar_expect_tx(fb, bytes);
-            i8_weights<GLU, PAIR>(maps, at, kb0 + k, t, fb);
+            i8_weights<GLU, PAIR>(maps, at, kb0 + k, t, fb, weights_stay);
           }
-          if (!FEW) i8_tokens<PAIR>(p, maps, at + I8_A_BYTES, kb0 + k, t, (int)rank, fb);
+          if (!FEW) i8_tokens<PAIR>(p, maps, at + I8_A_BYTES, kb0 + k, t, (int)rank, fb, tokens_stay);
         }
         s += LOADERS;
         if (s >= p.stages) { s -= p.stages; ph ^= 1u; }

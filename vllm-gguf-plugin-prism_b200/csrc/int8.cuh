@@ -19,6 +19,11 @@ struct I8Quantize {
   const int32_t* scatter;
   int copies;
   const int32_t* n_used;
+  // factor != null (hidden rows of experts): instead of the scale, factor[sorted[r]] = scale * what the sum multiplies the slot's result by
+  const int32_t *sorted, *topk_ids;
+  const float *topk_weights, *w_top;
+  float unit;
+  float* factor;
 };
 int launch_i8_quantize(const I8Quantize& a, cudaStream_t stream);
 
@@ -45,7 +50,7 @@ struct I8Product {
   // ... down product: y[sorted[row]] = D * w_scale * w_unit[expert] * unit (q_scale and the routing weight are left to launch_i8_sum)
   const int32_t* sorted;
   const float* w_unit;
-  float unit;
+  float unit;                // what the products are multiplied by
   // ... tokens that are not quantized yet (null: q is used; see i8_few): [m][ldx] in dtype
   const void* x;
   int64_t ldx;
@@ -73,10 +78,8 @@ int launch_i8_plan(const I8Plan& a, cudaStream_t stream);
 struct I8Sum {
   const void* y;             // [slots][h], fp16, fp32 where dtype is
   void* out;                 // [tokens][h] in dtype
-  const int32_t* place;
-  const int32_t* topk_ids;
-  const float *topk_weights, *q_scale, *w_top;
-  float unit;                // what the products were divided by
+  const int32_t* place;      // [slots]; negative: the slot has no result
+  const float* factor;       // [slots]
   int64_t tokens, top_k, h;
   int dtype;
 };

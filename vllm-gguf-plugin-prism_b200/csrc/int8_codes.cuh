@@ -59,14 +59,14 @@ static __device__ __noinline__ uint32_t i8q_exact4(float x0, float x1, float x2,
 }
 // What the codes of a row go by; a is lifted (by a power of two, exactly) so that 127 / a and 254 a stay in range
 struct I8Row {
-  float a, inv, r, lift, y;   // 127 / a, 1 / a, 127 * lift
+  float a, inv, r, lift, y;   // 127 / a, 1 / a (both to a few units in the last place), 127 * lift
 };
 __device__ __forceinline__ I8Row i8q_row(float a) {
   I8Row w;
   w.lift = a < 0x1p-90f ? 0x1p64f : a > 0x1p100f ? 0x1p-64f : 1.f;
   w.a = a * w.lift;
-  w.inv = 127.f / w.a;
-  w.r = 1.f / w.a;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w.r) : "f"(w.a));
+  w.inv = 127.f * w.r;
   w.y = 127.f * w.lift;
   return w;
 }

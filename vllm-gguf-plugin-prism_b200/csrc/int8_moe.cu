@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
   pdl_wait();
   pdl_trigger();
   __shared__ int32_t s_cnt[32][I8_MAX_EXPERTS + 1];   // first: counts of all slots, by warp modulo 8; then a warp's slots of a step, and its first place
-  __shared__ int32_t s_before[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS];
+  __shared__ int32_t s_before[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS], s_order[I8_MAX_EXPERTS];
   __shared__ float s_top[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.experts;
   if ((int)blockIdx.x >= blocks) {   // largest scale of an expert (a scale that is not finite: as if it were not there)
@@ -61,9 +61,13 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
   const int slots = (int)p.slots, s0 = min(slots, (int)blockIdx.x * run), s1 = min(slots, s0 + run);
   for (int i = threadIdx.x; i < 16 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
   __syncthreads();
-  for (int s = threadIdx.x; s < slots; s += 1024) {
-    const int e = p.topk_ids[s];
-    if (e >= 0 && e < E) atomicAdd(&s_cnt[(warp & 7) + (s < s0 ? 0 : 8)][e], 1);
+  for (int b = threadIdx.x; b < slots; b += 8 * 1024) {   // (eight loads in flight)
+    int e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = b + i * 1024 < slots ? p.topk_ids[b + i * 1024] : -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e[i] >= 0 && e[i] < E) atomicAdd(&s_cnt[(warp & 7) + (b + i * 1024 < s0 ? 0 : 8)][e[i]], 1);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += 1024) {
@@ -77,10 +81,29 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
     s_total[e] = before + rest;
   }
   __syncthreads();
-  if (warp == 0) {   // prefix sums over the experts: rows and passes
+  // Large passes are dealt out by size, the largest first: CTAs that take them in turn then get like shares.
+  if (blockIdx.x == 0) {
+    if ((int)threadIdx.x < E) s_pass[threadIdx.x] = i8_pass_size(s_total[threadIdx.x], p.pass_rows);
+    __syncthreads();
+    const int e = threadIdx.x >> 2, size = e < E ? s_pass[e] : 0;
+    int rank = e;
+    if (p.pass_rows > 64) {
+      rank = 0;
+      for (int o = threadIdx.x & 3; o < E; o += 4) {
+        const int other = s_pass[o];
+        rank += other > size || (other == size && o < e);
+      }
+      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    }
+    if (e < E && (threadIdx.x & 3) == 0) s_order[rank] = e;
+    __syncthreads();
+  }
+  if (warp == 0) {   // prefix sums over the experts: rows, and passes in that order
     int rows = 0, ps = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, c = e < E ? s_total[e] : 0, np = i8_pass_count(c, p.pass_rows);
+      const int e = e0 + lane, c = e < E ? s_total[e] : 0, by_size = e < E && blockIdx.x == 0 ? s_order[e] : 0;
+      const int np = e < E && blockIdx.x == 0 ? i8_pass_count(s_total[by_size], p.pass_rows) : 0;
       int a = c, b = np;
 #pragma unroll
       for (int m = 1; m < 32; m <<= 1) {
@@ -89,7 +112,7 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
       }
       if (e < E) {
         s_next[e] = rows + a - c + s_before[e];
-        s_pass[e] = ps + b - np;
+        if (blockIdx.x == 0) s_pass[by_size] = ps + b - np;
       }
       rows += __shfl_sync(0xffffffffu, a, 31);
       ps += __shfl_sync(0xffffffffu, b, 31);
@@ -155,46 +178,39 @@ int launch_i8_plan(const I8Plan& a, cudaStream_t stream) {
   return launch_pdl(i8_plan_kernel, dim3((unsigned)(blocks + a.experts)), dim3(1024), 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
 }
 
-// Eight columns a thread.
+// Eight columns a thread, eight experts' rows of fp16 (four of fp32) in flight.
 template <typename Y, typename T> __global__ void __launch_bounds__(256) i8_sum_kernel(const I8Sum p) {
   pdl_wait();
   pdl_trigger();
-  constexpr int WI = sizeof(Y) / 2, WO = sizeof(T) / 2;   // 16-byte words of eight values
+  constexpr int WI = sizeof(Y) / 2, WO = sizeof(T) / 2, ROWS = 16 / sizeof(Y);   // 16-byte words of eight values
   const unsigned per_row = (unsigned)(p.h / 8), top_k = (unsigned)p.top_k;
-  const unsigned total = (unsigned)p.tokens * per_row;
-  if (const unsigned i = blockIdx.x * 256 + threadIdx.x; i < total) {
-    const unsigned t = i / per_row, c = 8 * (i - t * per_row), slot0 = t * top_k;
-    const Y* in = static_cast<const Y*>(p.y) + (int64_t)slot0 * p.h + c;
-    float s[8];
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= (unsigned)p.tokens * per_row) return;
+  const unsigned t = i / per_row, c = 8 * (i - t * per_row), slot0 = t * top_k;
+  const Y* in = static_cast<const Y*>(p.y) + (int64_t)slot0 * p.h + c;
+  float s[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] = 0.f;
-    for (unsigned j0 = 0; j0 < top_k; j0 += 4, in += 4 * p.h) {   // four experts' rows in flight
-      uint4 v[4][WI];
-      float f[4];
+  for (int k = 0; k < 8; ++k) s[k] = 0.f;
+  for (unsigned j0 = 0; j0 < top_k; j0 += ROWS, in += ROWS * p.h) {
+    uint4 v[ROWS][WI];
+    float f[ROWS];
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) {
-        const int at = j0 + j < top_k ? __ldg(p.place + slot0 + j0 + j) : -1;
-        f[j] = 0.f;
-        if (at >= 0) {     // (a slot without a valid expert contributes nothing)
+    for (unsigned j = 0; j < ROWS; ++j) {
+      const bool live = j0 + j < top_k && __ldg(p.place + slot0 + j0 + j) >= 0;   // (a slot without a valid expert contributes nothing)
+      f[j] = live ? __ldg(p.factor + slot0 + j0 + j) : 0.f;
 #pragma unroll
-          for (int k = 0; k < WI; ++k) v[j][k] = reinterpret_cast<const uint4*>(in + j * p.h)[k];
-          f[j] = __ldg(p.topk_weights + slot0 + j0 + j) * __ldg(p.q_scale + at) * (__ldg(p.w_top + __ldg(p.topk_ids + slot0 + j0 + j)) * p.unit);
-        } else {
-#pragma unroll
-          for (int k = 0; k < WI; ++k) v[j][k] = make_uint4(0, 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] = fmaf(to_float<Y>(reinterpret_cast<const Y*>(v[j])[k]), f[j], s[k]);
+      for (int k = 0; k < WI; ++k) v[j][k] = live ? reinterpret_cast<const uint4*>(in + j * p.h)[k] : make_uint4(0, 0, 0, 0);
     }
-    uint4 o[WO];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(o)[k] = from_float<T>(s[k]);
+    for (int j = 0; j < ROWS; ++j)
 #pragma unroll
-    for (int k = 0; k < WO; ++k) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)t * p.h + c)[k] = o[k];
+      for (int k = 0; k < 8; ++k) s[k] = fmaf(to_float<Y>(reinterpret_cast<const Y*>(v[j])[k]), f[j], s[k]);
   }
+  uint4 o[WO];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(o)[k] = from_float<T>(s[k]);
+#pragma unroll
+  for (int k = 0; k < WO; ++k) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)t * p.h + c)[k] = o[k];
 }
 
 int launch_i8_sum(const I8Sum& a, cudaStream_t stream) {

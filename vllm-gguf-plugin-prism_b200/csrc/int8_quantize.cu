@@ -72,7 +72,14 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD *
     for (int j = 0; j < copies; ++j) {
       const int64_t o = !live ? -1 : p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
       if (o < 0) continue;
-      if (lane == 0) p.scale[o] = scale;
+      if (lane == 0) {
+        if (p.factor) {
+          const int slot = p.sorted[r];
+          p.factor[slot] = scale * p.topk_weights[slot] * (p.w_top[p.topk_ids[slot]] * p.unit);
+        } else {
+          p.scale[o] = scale;
+        }
+      }
 #pragma unroll
       for (int h = 0; h < HOLD; ++h) {
         const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
