@@ -310,3 +310,45 @@ def set_wait_limit_cycles(cycles: int) -> None:
 
 def last_status() -> int:
     return lib().gguf_b200_last_status()
+
+
+# ---- router, 8-bit integer products (the caller's matrices: rows at multiples of 16 bytes) ----
+
+
+def moe_route(logits, top_k, *, sigmoid=False, bias=None, n_group=1, topk_group=1, renormalize=True, scale=1.0):
+    T, E = logits.shape
+    w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
+    _check(lib().gguf_b200_moe_route(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), None if bias is None else bias.data_ptr(), w.data_ptr(),
+                                     ids.data_ptr(), T, E, top_k, n_group, topk_group, 2 if sigmoid else 1, int(renormalize), scale, _stream(logits)),
+           "moe_route")
+    return w, ids
+
+
+def int8_quantize(X):
+    M, K = X.shape
+    q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=X.device)
+    s = torch.empty((M,), dtype=torch.float32, device=X.device)
+    _check(lib().gguf_b200_int8_quantize(X.data_ptr(), _DT[X.dtype], X.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), M, K, _stream(X)), "int8_quantize")
+    return q[:, :K], s
+
+
+def int8_mul_mat(W, w_scales, X, bias=None, flags=0):
+    (M, K), N = X.shape, W.shape[0]
+    Y = torch.empty((M, N), dtype=X.dtype, device=X.device)
+    n = lib().gguf_b200_int8_scratch_bytes(M, K)
+    ws = _ws(X, n)
+    _check(lib().gguf_b200_int8_mul_mat(W.data_ptr(), W.stride(0), w_scales.data_ptr(), X.data_ptr(), X.stride(0), None if bias is None else bias.data_ptr(),
+                                        Y.data_ptr(), ws.data_ptr(), n, flags, _DT[X.dtype], M, N, K, _stream(X)), "int8_mul_mat")
+    return Y
+
+
+def int8_fused_moe(X, W13, w13_scales, W2, w2_scales, topk_weights, topk_ids, act=1):
+    (T, H), (E, _, I), top_k = X.shape, W2.shape, topk_ids.shape[1]
+    Y = torch.empty((T, H), dtype=X.dtype, device=X.device)
+    n = lib().gguf_b200_int8_moe_workspace_bytes(T, top_k, E, H, I)
+    ws = _ws(X, n)
+    _check(lib().gguf_b200_int8_fused_moe(X.data_ptr(), X.stride(0), W13.data_ptr(), W13.stride(1), w13_scales.data_ptr(), W2.data_ptr(), W2.stride(1),
+                                          w2_scales.data_ptr(), Y.data_ptr(), topk_ids.data_ptr(), topk_weights.data_ptr(), ws.data_ptr(), n,
+                                          _DT[X.dtype], act, T, top_k, E, H, I, _stream(X)), "int8_fused_moe")
+    return Y

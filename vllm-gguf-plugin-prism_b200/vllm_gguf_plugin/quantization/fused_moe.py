@@ -220,3 +220,19 @@ class GGUFMoEMethod(FusedMoEMethodBase):
         step = fused_moe_gguf if is_compiling() else _fused_moe_gguf   # eager: no custom-op dispatch in between
         return step(x, layer.w13_weight, layer.w2_weight, topk_weights, topk_ids,
                               layer.w13_weight_type.weight_type, layer.w2_weight_type.weight_type, activation)
+
+    @staticmethod
+    def route(layer, router_logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(topk_weights, topk_ids) of the router's logits ``[tokens, experts]``, by what vLLM's MoE layers say about it: ``top_k``,
+        ``renormalize``, ``scoring_func``, ``e_score_correction_bias``, ``use_grouped_topk`` with ``num_expert_group`` and ``topk_group``,
+        ``routed_scaling_factor``.  (The serving engine does this for the reference's method.)"""
+        grouped = getattr(layer, "use_grouped_topk", False)
+        return ops.moe_route(router_logits, layer.top_k, scoring=getattr(layer, "scoring_func", "softmax"),
+                             bias=getattr(layer, "e_score_correction_bias", None),
+                             n_group=(getattr(layer, "num_expert_group", None) or 1) if grouped else 1,
+                             topk_group=(getattr(layer, "topk_group", None) or 1) if grouped else 1,
+                             renormalize=getattr(layer, "renormalize", True), scale=getattr(layer, "routed_scaling_factor", None) or 1.0)
+
+    def apply_logits(self, layer, x: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
+        """The whole MoE layer behind its gate: ``route``, then ``apply``."""
+        return self.apply(layer, x, *self.route(layer, router_logits))
