@@ -123,7 +123,9 @@ def test_quantize_strides(ops, dtype):
 SIZES = [(1, 1, 1), (1, 1, 16), (1, 7, 33), (1, 128, 128), (2, 129, 127), (1, 4096, 4096), (2, 1000, 2064), (3, 200, 4096), (5, 300, 1040), (7, 128, 14336),
          (8, 513, 5000), (1, 19072, 6144), (4, 19072, 6160), (9, 130, 4096), (16, 256, 1024), (17, 4000, 512), (27, 384, 8192),
          (33, 300, 2048), (64, 640, 4096), (65, 130, 4100), (128, 1000, 640), (200, 256, 14336), (255, 130, 256), (256, 130, 640), (257, 130, 640),
-         (300, 4096, 1536), (513, 257, 384), (1000, 520, 1040), (2049, 2100, 400)]
+         (300, 4096, 1536), (513, 257, 384), (1000, 520, 1040), (2049, 2100, 400),
+         # shared by two, by four; pairs, odd numbers of 128-row tiles among them
+         (3, 2050, 9000), (20, 2100, 14000), (90, 1030, 13000), (520, 4224, 12345), (450, 9000, 2080), (2100, 6000, 1030)]
 
 
 @pytest.mark.gpu

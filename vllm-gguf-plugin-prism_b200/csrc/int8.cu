@@ -639,11 +639,12 @@ template <bool GLU, bool PAIR, typename FewT> static int i8_launch(const I8Maps&
 }
 
 // How a dense product is dealt out: tokens a tile, whether pairs of CTAs take 256 rows together, how many CTAs share a tile's K.  What takes
-// the least time by this model, in us on a chip that is not held back by its power limit: a stage 0.08 + 0.00094 a token (a pair: 0.065 +
-// 0.00092), 5 for start and end (a pair 0.8 more), 0.012 a token for the last tile's way out, 1 + 0.025 a token for an exchange of sums.
+// the least time by this model, in us on a chip that is not held back by its power limit: a stage 0.09 + 0.00088 a token (a pair: 0.065 +
+// 0.00092), 5 for start and end (a pair 0.8 more), 0.012 a token for the last tile's way out, 2.8 + 0.012 a token for an exchange of sums
+// (1 more by four or eight), and no less than its copies take from L2 at 17.5 TB/s.
 // Measured, single / pair / shared by two: 500 tokens of 4096x14336 27.5 (tiles of 128) / 25.9 (128) / 30.4 (256); of 4096x4096 10.7 / 11.5 /
-// 17.1; of 14336x4096 28.7 (256) / 26.1 (256); 1000 tokens of 4096x4096 16.3 (256) / 16.6 (128); 4096 tokens of 14336x4096 173 / 149;
-// 1 token of 4096x4096 whole 10.6, by two 8.7, by four 7.7.
+// 17.1; of 14336x4096 28.7 (256) / 26.1 (256); 1000 tokens of 4096x4096 16.3 (256) / 16.6 (128); 4096 tokens of 14336x4096 173 / 149.  Whole / by
+// two / by four: 1 token of 4096x4096 6.6 / 7.7 / 7.9, of 4096x14336 15.3 / 13.6 / 12.3; 128 tokens of 4096x4096 9.7 / 11.1 / 12.1.
 struct I8Deal {
   int tn, tt, split;
   bool pair;
@@ -658,9 +659,10 @@ static I8Deal i8_deal(int64_t m, int64_t n, int nk) {
       const int tn = (int)round_up(each, pair ? 32 : 16), rows = pair ? 2 * I8_ROWS : I8_ROWS;
       const int64_t tiles = (n + rows - 1) / rows * tt, slots = pair ? I8_SMS / 2 : I8_SMS;
       for (int split = 1; split <= (pair ? 1 : 8) && (split == 1 || (tiles * split <= slots && nk >= 4 * split)); split *= 2) {
-        const float stage = pair ? 0.065f + 0.00092f * tn : 0.08f + 0.00094f * tn;
+        const float stage = pair ? 0.065f + 0.00092f * tn : 0.09f + 0.00088f * tn;
         const int64_t waves = split > 1 ? 1 : (tiles + slots - 1) / slots;
-        const float t = waves * ((nk + split - 1) / split) * stage + (pair ? 0.8f : 0.f) + 0.012f * tn + (split > 1 ? 1.f + 0.025f * tn : 0.f);
+        const float copied = (float)tiles * (float)nk * (float)(rows + tn) * (float)I8_BK / 17.5e6f;
+        const float t = fmaxf(waves * ((nk + split - 1) / split) * stage, copied) + (pair ? 0.8f : 0.f) + 0.012f * tn + (split > 1 ? 2.8f + 0.012f * tn : 0.f) + (split > 2 ? 1.f : 0.f);
         if (t < least) {
           least = t;
           best = I8Deal{tn, (int)tt, split, pair != 0};
@@ -673,7 +675,7 @@ static I8Deal i8_deal(int64_t m, int64_t n, int nk) {
 }
 // Whether a product of m tokens is one launch: rows that 16-byte loads can start at, the codes of a CTA's K (2 KB a stage) leave half of its
 // shared memory to the weights, and finding the tokens' largest values, which every CTA repeats, takes less than a launch.  (One / two
-// launches in us: 4096x4096, 1 token 7.2 / 9.1, 4 tokens 8.5 / 9.1, 8 tokens 9.9 / 9.1; 4096x14336, 1 token 15.0 / 16.1, 8 tokens 27 / 16.)
+// launches in us: 4096x4096, 1 token 7.2 / 8.6, 4 tokens 8.1 / 8.6, 8 tokens 9.4 / 8.6; 4096x14336, 1 token 13.8 / 15.5, 8 tokens 27 / 15.5.)
 constexpr int I8_FEW = 8;
 constexpr int64_t I8_FEW_VALUES = 16384;
 bool i8_few(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k) {
