@@ -59,51 +59,86 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
     return;
   }
   const int slots = (int)p.slots, s0 = min(slots, (int)blockIdx.x * run), s1 = min(slots, s0 + run);
-  for (int i = threadIdx.x; i < 16 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
+  // Whether a slot has a valid expert, and how many lanes below this one have the same
+  auto match = [&](int e, unsigned& below) {
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const bool valid = e >= 0 && e < E;
+    below = __popc(same & ((1u << lane) - 1u));
+    if (valid && below == 0) s_cnt[warp][e] = __popc(same);
+    return valid;
+  };
+  // Of counts by warp: where a warp's first slot of the expert goes, from `at` on; returns where the next would
+  auto spread = [&](int e, int at, int warps) {
+    for (int w0 = 0; w0 < warps; w0 += 8) {   // (eight loads in flight)
+      int v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = s_cnt[w0 + i][e];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s_cnt[w0 + i][e] = at;
+        at += v[i];
+      }
+    }
+    return at;
+  };
+  // One block for all slots counts them and places them in one go.
+  const bool alone = blocks == 1;
+  const int my_slot = threadIdx.x, warps = alone ? ((slots + 31) / 32 + 7) / 8 * 8 : 32;
+  const int my_e = alone && my_slot < slots ? p.topk_ids[my_slot] : -1;
+  unsigned my_below = 0;
+  bool my_valid = false;
+  for (int i = threadIdx.x; i < (alone ? warps : 16) * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
   __syncthreads();
-  for (int b = threadIdx.x; b < slots; b += 8 * 1024) {   // (eight loads in flight)
-    int e[8];
+  if (alone) {
+    my_valid = match(my_e, my_below);
+  } else {
+    for (int b = threadIdx.x; b < slots; b += 8 * 1024) {   // (eight loads in flight)
+      int e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = b + i * 1024 < slots ? p.topk_ids[b + i * 1024] : -1;
+      for (int i = 0; i < 8; ++i) e[i] = b + i * 1024 < slots ? p.topk_ids[b + i * 1024] : -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (e[i] >= 0 && e[i] < E) atomicAdd(&s_cnt[(warp & 7) + (b + i * 1024 < s0 ? 0 : 8)][e[i]], 1);
+      for (int i = 0; i < 8; ++i)
+        if (e[i] >= 0 && e[i] < E) atomicAdd(&s_cnt[(warp & 7) + (b + i * 1024 < s0 ? 0 : 8)][e[i]], 1);
+    }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += 1024) {
-    int before = 0, rest = 0;
+  const bool by_size = p.pass_rows > 64 && blockIdx.x == 0;
+  if ((int)threadIdx.x < E) {
+    const int e = threadIdx.x;
+    int before = 0, total = 0;
+    if (alone) {
+      total = spread(e, 0, warps);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      before += s_cnt[i][e];
-      rest += s_cnt[8 + i][e];
+      for (int i = 0; i < 8; ++i) {
+        before += s_cnt[i][e];
+        total += s_cnt[8 + i][e];
+      }
+      total += before;
     }
     s_before[e] = before;
-    s_total[e] = before + rest;
+    s_total[e] = total;
+    if (by_size) s_pass[e] = i8_pass_size(total, p.pass_rows);
   }
   __syncthreads();
   // Large passes are dealt out by size, the largest first: CTAs that take them in turn then get like shares.
-  if (blockIdx.x == 0) {
-    if ((int)threadIdx.x < E) s_pass[threadIdx.x] = i8_pass_size(s_total[threadIdx.x], p.pass_rows);
-    __syncthreads();
+  if (by_size) {
     const int e = threadIdx.x >> 2, size = e < E ? s_pass[e] : 0;
-    int rank = e;
-    if (p.pass_rows > 64) {
-      rank = 0;
-      for (int o = threadIdx.x & 3; o < E; o += 4) {
-        const int other = s_pass[o];
-        rank += other > size || (other == size && o < e);
-      }
-      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    int rank = 0;
+    for (int o = threadIdx.x & 3; o < E; o += 4) {
+      const int other = s_pass[o];
+      rank += other > size || (other == size && o < e);
     }
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     if (e < E && (threadIdx.x & 3) == 0) s_order[rank] = e;
     __syncthreads();
   }
   if (warp == 0) {   // prefix sums over the experts: rows, and passes in that order
     int rows = 0, ps = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, c = e < E ? s_total[e] : 0, by_size = e < E && blockIdx.x == 0 ? s_order[e] : 0;
-      const int np = e < E && blockIdx.x == 0 ? i8_pass_count(s_total[by_size], p.pass_rows) : 0;
+      const int e = e0 + lane, c = e < E ? s_total[e] : 0, o = by_size && e < E ? s_order[e] : e;
+      const int np = e < E && blockIdx.x == 0 ? i8_pass_count(s_total[o], p.pass_rows) : 0;
       int a = c, b = np;
 #pragma unroll
       for (int m = 1; m < 32; m <<= 1) {
@@ -112,7 +147,7 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
       }
       if (e < E) {
         s_next[e] = rows + a - c + s_before[e];
-        if (blockIdx.x == 0) s_pass[by_size] = ps + b - np;
+        s_pass[o] = ps + b - np;
       }
       rows += __shfl_sync(0xffffffffu, a, 31);
       ps += __shfl_sync(0xffffffffu, b, 31);
@@ -128,35 +163,25 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
       const int c = s_total[e], per = i8_pass_size(c, p.pass_rows);
       for (int i = lane; i * per < c; i += 32) static_cast<int4*>(p.passes)[s_pass[e] + i] = make_int4(e, s_next[e] + i * per, min(per, c - i * per), 0);
     }
+  auto put = [&](int s, int at) {
+    if (at >= 0) p.sorted[at] = s;
+    p.place[s] = at;
+  };
+  if (alone) {
+    if (my_slot < slots) put(my_slot, my_valid ? s_next[my_e] + s_cnt[warp][my_e] + (int)my_below : -1);
+    return;
+  }
   __syncthreads();   // (s_next moves on below)
   for (int b = s0; b < s1; b += 1024) {
     for (int i = threadIdx.x; i < 32 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
     __syncthreads();
     const int s = b + threadIdx.x, e = s < s1 ? p.topk_ids[s] : -1;
-    const bool valid = e >= 0 && e < E;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (valid && lane == __ffs(same) - 1) s_cnt[warp][e] = __popc(same);
+    unsigned below;
+    const bool valid = match(e, below);
     __syncthreads();
-    if ((int)threadIdx.x < E) {   // per expert: first place of every warp
-      int at = s_next[threadIdx.x];
-      for (int w0 = 0; w0 < 32; w0 += 8) {   // (eight loads in flight)
-        int v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s_cnt[w0 + i][threadIdx.x];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          s_cnt[w0 + i][threadIdx.x] = at;
-          at += v[i];
-        }
-      }
-      s_next[threadIdx.x] = at;
-    }
+    if ((int)threadIdx.x < E) s_next[threadIdx.x] = spread(threadIdx.x, s_next[threadIdx.x], 32);
     __syncthreads();
-    if (s < s1) {
-      const int at = valid ? s_cnt[warp][e] + __popc(same & ((1u << lane) - 1u)) : -1;
-      if (valid) p.sorted[at] = s;
-      p.place[s] = at;
-    }
+    if (s < s1) put(s, valid ? s_cnt[warp][e] + (int)below : -1);
     __syncthreads();
   }
 }
