@@ -7,16 +7,24 @@
 // token costs no more tensor time than sixteen, and what bounds small batches is the weights' way from memory.
 //
 // A CTA: three loaders, an MMA issuer, sixteen epilogue warps (lane = weight row = lane of tensor memory), over a ring of stages of 128
-// values.  Three ways to deal out the work:
-//   tiles    a CTA takes items (128 weight rows x up to 256 tokens) a grid apart, two accumulators in turn where they fit
+// values.  Four ways to deal out the work:
+//   tiles    a CTA takes items (128 weight rows x up to 256 tokens) a grid apart, two accumulators in turn
+//   pairs    two CTAs take 256 rows together (cta_group::2): each brings its 128 rows and half of the tokens, and the tensor cores of both
+//            read both halves, so that a CTA's copies and shared memory carry a third less for the same product
 //   split    fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares the K of one tile.  Each sends its sums of every other's
 //            rows into the other's shared memory, which then adds and stores its rows: no scratch in memory, nothing to clear, and
 //            integer sums do not depend on the order
 //   experts  items are (pass of an expert's tokens, 128 rows).  For the gate and up product a box holds the same 64 rows of both, 8 and
 //            8 in turn: the two meet in one warp, so that act(gate) * up is formed on the way out and nothing else is stored
 //
-// A few tokens come as they are (FEW): the epilogue warps make their codes, and each CTA the ones of its K, in shared memory while the
+// A few tokens come as they are (FEW): the epilogue warps make their codes, each CTA the ones of its K, in shared memory while the
 // weights arrive.  One launch instead of two; every CTA repeats the search for a token's largest value.
+//
+// What bounds it (B200): one to 64 tokens, the weights from memory and 4 to 5 us of start and end (27 tokens of 14336x4096: 59 MB in 11.9 us,
+// 9.1 at the copy rate); large batches, the tensor core and the power limit (4096 tokens of 14336x4096: 149 to 155 us, 3.1 to 3.2 P operations a
+// second, the tensor pipe active 93 % of the time; single CTAs 173); experts of some 250 tokens, L2 and memory (2048 tokens over 64 experts
+// of 2048x1024: 76 us for gate and up, 45 us for down, the tensor pipe at 46 and 41 %).  Without 16-byte stores from sixteen warps and with one
+// loader the same 4096 tokens took 260 us.
 #include <cuda.h>
 #include <math.h>
 
@@ -106,7 +114,7 @@ template <bool PAIR> __device__ __forceinline__ void i8_tmem_dealloc(uint32_t at
   else tmem_dealloc(at, cols);
 }
 constexpr uint32_t I8_LEADER = 0xFEFFFFFFu;   // of a shared-memory address in a cluster of two: the same place in the first CTA
-// (GROUP 2: a pair's copies, each into its own shared memory, may count on the first CTA's barrier)
+// (A pair's copies go each into its own shared memory and count on the first CTA's barrier.)
 template <bool PAIR> __device__ __forceinline__ void i8_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t keep) {
   if (PAIR)
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
@@ -228,8 +236,7 @@ template <bool GLU, bool PAIR> __device__ __forceinline__ I8Item i8_item(const I
   return t;
 }
 
-// A copy is one box wherever it can be: boxes of a few KB cost the copy engine as much as one of 16 KB.  (The weights of a stage in four
-// boxes, its tokens in up to four of 64 rows: 87 us for the gate and up products of 2048 tokens over 64 experts of 2048x1024.)
+// A copy is one box wherever it can be.  (The weights of a stage in two / four / eight boxes instead of one cost one loader 22 / 68 / 158 ns more.)
 struct I8Maps {
   CUtensorMap w, q[5];   // tokens: boxes of 256, 128, 64, 32, 16 rows for experts; dense: q[0], tn rows
 };
@@ -238,21 +245,19 @@ template <bool GLU, bool PAIR> __device__ __forceinline__ void i8_weights(const 
   if (GLU) i8_box5<PAIR>(at, &maps.w, kb * I8_BK, t.n0 / 8, t.e, bar, keep);
   else i8_box<PAIR>(at, &maps.w, kb * I8_BK, t.a_row, bar, keep);
 }
-// Columns of an item's instructions, and the rows of tokens that a CTA's stage takes for them: all, or a pair's half
-template <bool PAIR> __device__ __forceinline__ int i8_columns(const I8Params& p, const I8Item& t) {
-  return !p.passes ? p.tn : PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15;
-}
+// Columns of an item's instructions, and the copies of a stage's tokens: all of them, or (dense) a pair's half
+__device__ __forceinline__ int i8_columns(const I8Params& p, const I8Item& t) { return p.passes ? (t.rows + 15) & ~15 : p.tn; }
 template <bool PAIR> __device__ __forceinline__ void i8_tokens(const I8Params& p, const I8Maps& maps, uint32_t at, int kb, const I8Item& t, int rank, uint32_t bar, uint64_t keep) {
-  const int rows = i8_columns<PAIR>(p, t) >> (PAIR ? 1 : 0), x0 = t.x0 + (PAIR ? rank * rows : 0);
   if (!p.passes) {
-    i8_box<PAIR>(at, &maps.q[0], kb * I8_BK, x0, bar, keep);
+    i8_box<PAIR>(at, &maps.q[0], kb * I8_BK, t.x0 + (PAIR ? rank * p.tn / 2 : 0), bar, keep);
     return;
   }
+  const int rows = i8_columns(p, t);
   int y = 0;
 #pragma unroll
   for (int i = 0; i < 5; ++i)
     if (rows & 256 >> i) {
-      i8_box<PAIR>(at + (uint32_t)(y * I8_BK), &maps.q[i], kb * I8_BK, x0 + y, bar, keep);
+      i8_box<PAIR>(at + (uint32_t)(y * I8_BK), &maps.q[i], kb * I8_BK, t.x0 + y, bar, keep);
       y += 256 >> i;
     }
 }
@@ -323,9 +328,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
   }
   if (!PAIR && p.split > 1) cluster_arrive();   // (waited for before anything is sent)
   if (warp == 2) i8_tmem_alloc<PAIR>(tmem_slot, 512);
-  // (The MMA issuer's control flow and operands have to be known to be the same for all lanes, so that they stay in uniform registers: from a
-  // loop that the compiler takes for divergent an MMA takes 115 clocks, however few its tokens.  Hence the rank from the block's number, sums
-  // over the warp for what comes from memory -- a reduction's result is uniform --, and all of the tensor memory, which starts at 0.)
+  // (The MMA issuer's control flow and operands are known to be the same for all lanes and stay in uniform registers -- the rank from the block's
+  // number, a warp's maximum of what comes from memory, all of the tensor memory, which starts at 0 --: a stage takes 50 clocks to issue.)
   const uint32_t rank = blockIdx.x & (uint32_t)(PAIR ? 1 : p.split - 1);
   constexpr int CTAS = PAIR ? 2 : 1;
   const int first = !PAIR && p.split > 1 ? (int)blockIdx.x / p.split : (int)blockIdx.x / CTAS, step = !PAIR && p.split > 1 ? 1 << 30 : (int)gridDim.x / CTAS;
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     int ahead = 0;
     if (first < n_items) {
       const I8Item t = item(first, 0, false);
-      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns<PAIR>(p, t) * I8_BK));   // (a pair's, on the first CTA's barrier)
+      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns(p, t) * I8_BK));   // (a pair's, on the first CTA's barrier)
       ahead = FEW && !p.settled ? nkb : min(p.stages, nkb);
       for (int g = k; g < ahead; g += LOADERS)
         if (lead) {
@@ -388,7 +392,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     next_item();
     while (i < n_items) {
       const I8Item t = item(i, j, true);
-      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns<PAIR>(p, t) * I8_BK));
+      const uint32_t bytes = (uint32_t)(CTAS * I8_A_BYTES + (FEW ? 0 : i8_columns(p, t) * I8_BK));
       for (; k < nkb; k += LOADERS) {
         const uint32_t fb = full_s + 8u * s, at = ring + (uint32_t)(s * p.stage_bytes);
         const bool weights = j > 0 || k >= ahead;
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     int s = 0, buf = 0;
     uint32_t ph = 0, dph = 0;
     for (int i = first, j = 0; i < n_items; i += step, ++j) {
-      const int cols = (int)__reduce_max_sync(0xffffffffu, (unsigned)i8_columns<PAIR>(p, item(i, j, false)));
+      const int cols = (int)__reduce_max_sync(0xffffffffu, (unsigned)i8_columns(p, item(i, j, false)));
       const uint32_t idesc = i8_idesc(PAIR, cols), d = tmem + (uint32_t)(buf * p.tn);
       const uint32_t codes0 = (uint32_t)umma_desc_sw128(smem_u32(smem + p.codes_off));
       if (FEW) mbar_wait_or(smem_u32(coded), 0u, gave_up_s);
@@ -694,7 +698,8 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.k = (int)a.k;
   p.nk = (int)((a.k + I8_BK - 1) / I8_BK);
   p.m = (int)a.m;
-  const I8Deal deal = a.passes ? I8Deal{(int)round_up(a.pass_rows, 32), 1, 1, false} : i8_deal(a.m, a.n, p.nk);
+  // (experts: pairs, and passes of 144 to 256 tokens, make no difference: 2048 tokens over 64 experts 177 to 181 us throughout)
+  const I8Deal deal = a.passes ? I8Deal{(int)a.pass_rows, 1, 1, false} : i8_deal(a.m, a.n, p.nk);
   const bool pair = deal.pair;
   p.rt = (int)((a.n + per_tile * (pair ? 2 : 1) - 1) / (per_tile * (pair ? 2 : 1)));
   p.tn = deal.tn;
@@ -736,7 +741,7 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   for (int i = 0; i < (few ? 0 : a.passes ? 5 : 1); ++i)
     if (!i8_map(maps.q[i], a.q, a.k, a.m, a.ldq, a.passes ? 256 >> i : p.tn / (pair ? 2 : 1))) return E_CUDA;
   const size_t smem = 1024 + (size_t)p.aux_off + I8_AUX;
-  if (glu) return pair ? i8_launch<true, true, void>(maps, p, (int)grid, smem, stream) : i8_launch<true, false, void>(maps, p, (int)grid, smem, stream);
+  if (glu) return i8_launch<true, false, void>(maps, p, (int)grid, smem, stream);
   if (pair) return i8_launch<false, true, void>(maps, p, (int)grid, smem, stream);
   if (!few) return i8_launch<false, false, void>(maps, p, (int)grid, smem, stream);
   switch (a.dtype) {
