@@ -221,7 +221,7 @@ def test_streams_graphs_and_threads(ops):
     """Two captured graphs replayed on two streams at once, and eager calls beside them, give what one call alone gives."""
     gen = torch.Generator(device="cuda").manual_seed(9)
     cases = []
-    for m, n, k in ((1, 2048, 2048), (40, 1024, 4096), (300, 512, 1024)):
+    for m, n, k in ((1, 2048, 2048), (40, 1024, 4096), (300, 512, 1024), (3, 2050, 9000), (500, 4096, 8192)):   # (one launch; two; shared; pairs)
         w, ws = weights(n, k, gen)
         x = torch.randn(m, k, device="cuda", generator=gen).to(torch.bfloat16)
         cases.append((w, ws, x, ops.int8_mul_mat(w, ws, x)))
@@ -372,6 +372,7 @@ def test_c_abi_refuses_before_any_launch(native_libs):
     assert q(p, 1, 64, p, 64, p, -1, 64, null) == -3 and q(p, 1, 64, p, 64, p, 1, 0, null) == -3
     assert q(null, 1, 64, p, 64, p, 1, 64, null) == -4 and q(p, 1, 64, odd, 64, p, 1, 64, null) == -4
     assert q(p, 1, 64, p, 48, p, 1, 64, null) == -4 and q(p, 1, 64, p, 72, p, 1, 64, null) == -4 and q(p, 1, 64, p, 64, null, 1, 64, null) == -4
+    assert q(ctypes.c_void_p(4097), 1, 64, p, 64, p, 1, 64, null) == -4 and q(ctypes.c_void_p(4098), 0, 64, p, 64, p, 1, 64, null) == -4
     assert q(null, 1, 64, null, 64, null, 0, 64, null) == 0
     m = lib.gguf_b200_int8_mul_mat
     assert lib.gguf_b200_int8_scratch_bytes(3, 100) == 512 + 256 and lib.gguf_b200_int8_scratch_bytes(0, 100) == 0
@@ -393,7 +394,7 @@ def test_c_abi_refuses_before_any_launch(native_libs):
 
     assert call(act=3) == -3 and call(h=60) == -3 and call(i=36) == -3 and call(top_k=0) == -3 and call(e=0) == -3
     assert call(dtype=5) == -2 and call(e=257) == -7 and call(w13=odd) == -4 and call(ld13=72) == -4 and call(ids=null) == -4 and call(y=odd) == -4
-    assert call(ws=room - 1) == -5
+    assert call(ws=room - 1) == -5 and call(top_k=257) == -7
 
 
 def test_shapes_under_tracing(ops):

@@ -155,7 +155,7 @@ def test_c_abi_refuses_before_any_launch(native_libs):
                 dict(k=17)):
         assert call(**bad) == -3, bad
     assert call(e=520, groups=1, topk_group=1) == -7 and call(k=33, topk_group=8) == -7 and call(groups=64, topk_group=64) == -7
-    assert call(logits=None) == -4 and call(weights=None) == -4 and call(ids=None) == -4
+    assert call(logits=ctypes.c_void_p(4098)) == -4 and call(logits=None) == -4 and call(weights=None) == -4 and call(ids=None) == -4
     assert call(tokens=0, logits=None) == 0
 
 
