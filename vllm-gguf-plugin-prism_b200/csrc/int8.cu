@@ -263,35 +263,39 @@ template <bool PAIR> __device__ __forceinline__ void i8_tokens(const I8Params& p
 }
 
 // Codes of the tokens and their scales, by the 512 threads of the epilogue: a token's threads (all of them for one token, two warps each for
-// five to eight) read its row once for the largest value, and the part [k0, k1) again for the codes, which go where a TMA box of 16 rows
-// with the 128-byte swizzle would have put them.
+// five to eight) read its row once, up to two units each (I8_FEW_VALUES), and those that have units of [k0, k1) put the codes where a TMA box of
+// 16 rows with the 128-byte swizzle would have.  (Behind K the weights are zeros, whatever the codes.)
+constexpr int64_t I8_FEW = 8, I8_FEW_VALUES = 32 * I8_EPI * 2 * I8Q_UNIT;
+__host__ __device__ constexpr int i8_few_rows(int m) { return m <= 2 ? m : m <= 4 ? 4 : 8; }
 template <typename T> __device__ __forceinline__ void i8_few_codes(const I8Params& p, int k0, int k1, uint32_t codes, float* scale, uint32_t* top_of, int tid) {
-  const int lanes = 32 * I8_EPI / (p.m <= 2 ? p.m : p.m <= 4 ? 4 : 8), tok = tid / lanes, lane = tid % lanes;
+  const int lanes = 32 * I8_EPI / i8_few_rows(p.m), warps = lanes / 32, tok = tid / lanes, lane = tid % lanes;
   const bool live = tok < p.m;
   const T* x = static_cast<const T*>(p.x) + (live ? tok : 0) * p.ldx;
+  const int k = live ? p.k : 0;
+  T v[2][I8Q_UNIT];
   uint32_t top = 0;
-  for (int at = lane * I8Q_UNIT; at < (live ? p.k : 0); at += lanes * I8Q_UNIT) {
-    T v[I8Q_UNIT];
-    i8q_load<T, true>(x, p.k, at, v);
-    top = i8q_top<T>(v, top);
-  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if ((h * lanes + lane) * I8Q_UNIT < k) i8q_load<T, true>(x, k, (h * lanes + lane) * I8Q_UNIT, v[h]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if ((h * lanes + lane) * I8Q_UNIT < k) top = i8q_top<T>(v[h], top);
   top = __reduce_max_sync(0xffffffffu, i8q_top_bits<T>(top));
   if ((tid & 31) == 0) top_of[tid >> 5] = top;
   asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
-  for (int i = 0; i < lanes / 32; ++i) top = max(top, top_of[tok * (lanes / 32) + i]);
+  top = __reduce_max_sync(0xffffffffu, (tid & 31) < warps ? top_of[tok * warps + (tid & 31)] : 0u);
   const bool finite = top < 0x7f800000u, zero = !finite || top == 0;
   const float a = __uint_as_float(top);
   const I8Row w = i8q_row(zero ? 1.f : a);
   if (live && lane == 0) scale[tok] = finite ? a / 127.f : __uint_as_float(0x7fc00000u);
-  for (int at = k0 + lane * I8Q_UNIT; at < (live ? k1 : 0); at += lanes * I8Q_UNIT) {
-    uint4 c = make_uint4(0, 0, 0, 0);
-    if (at < p.k && !zero) {
-      T v[I8Q_UNIT];
-      i8q_load<T, true>(x, p.k, at, v);
-      c = i8q_unit<T>(v, w);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = (h * lanes + lane) * I8Q_UNIT;
+    if (at < k && at >= k0 && at < k1) {
+      const uint4 c = zero ? make_uint4(0, 0, 0, 0) : i8q_unit<T>(v[h], w);
+      const uint32_t to = codes + (uint32_t)((at - k0) / I8_BK * 2048 + tok * 128 + ((at / 16 ^ tok) & 7) * 16);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w) : "memory");
     }
-    const uint32_t to = codes + (uint32_t)((at - k0) / I8_BK * 2048 + tok * 128 + ((at / 16 ^ tok) & 7) * 16);
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w) : "memory");
   }
 }
 
@@ -653,6 +657,23 @@ struct I8Deal {
   int tn, tt, split;
   bool pair;
 };
+// A few tokens (their product begins when the codes are made): a stage 0.127, an exchange 1.65 / 2.1 / 2.7 by two / four / eight, and no less than
+// the weights at 9 TB/s.  (Whole / by two / by four / by eight: 1 token of 1024x4096 6.5 / 6.2 / 5.6 / 5.7, of 4096x4096 7.1 / 6.8 / 7.1, of 2048x2048 4.8 /
+// 5.4 / 5.2.)
+static I8Deal i8_deal_few(int64_t n, int nk) {
+  const int64_t tiles = (n + I8_ROWS - 1) / I8_ROWS;
+  const float exchange[4] = {0.f, 1.65f, 2.1f, 2.7f}, weights = (float)tiles * (float)nk * (float)I8_A_BYTES / 9e6f;
+  I8Deal best{16, 1, 1, false};
+  float least = INFINITY;
+  for (int i = 0; i < 4 && (i == 0 || (tiles << i <= I8_SMS && nk >= 4 << i)); ++i) {
+    const float t = fmaxf((float)((nk + (1 << i) - 1) >> i) * 0.127f, weights) + exchange[i];
+    if (t < least) {
+      least = t;
+      best.split = 1 << i;
+    }
+  }
+  return best;
+}
 static I8Deal i8_deal(int64_t m, int64_t n, int nk) {
   I8Deal best{};
   float least = INFINITY;
@@ -679,13 +700,11 @@ static I8Deal i8_deal(int64_t m, int64_t n, int nk) {
 }
 // Whether a product of m tokens is one launch: rows that 16-byte loads can start at, the codes of a CTA's K (2 KB a stage) leave half of its
 // shared memory to the weights, and finding the tokens' largest values, which every CTA repeats, takes less than a launch.  (One / two
-// launches in us: 4096x4096, 1 token 7.2 / 8.6, 4 tokens 8.1 / 8.6, 8 tokens 9.4 / 8.6; 4096x14336, 1 token 13.8 / 15.5, 8 tokens 27 / 15.5.)
-constexpr int I8_FEW = 8;
-constexpr int64_t I8_FEW_VALUES = 16384;
+// launches in us, 4096x4096: 1 token 6.8 / 8.6, 4 tokens 7.4 / 8.6, 8 tokens 9.4 / 8.6; 4096x14336, 1 token 13.6 / 15.5, 8 tokens 27 / 15.5.)
 bool i8_few(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k) {
   const int64_t size = dtype == DT_F32 ? 4 : 2, nk = (k + I8_BK - 1) / I8_BK;
-  if (m > I8_FEW || m * k > I8_FEW_VALUES || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || (m > 1 && ldx * size % 16 != 0)) return false;
-  const int split = i8_deal(m, n, (int)nk).split;
+  if (m > I8_FEW || i8_few_rows((int)m) * k > I8_FEW_VALUES || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || (m > 1 && ldx * size % 16 != 0)) return false;
+  const int split = i8_deal_few(n, (int)nk).split;
   return (nk + split - 1) / split <= 48;
 }
 
@@ -699,7 +718,7 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.nk = (int)((a.k + I8_BK - 1) / I8_BK);
   p.m = (int)a.m;
   // (experts: pairs, and passes of 144 to 256 tokens, make no difference: 2048 tokens over 64 experts 177 to 181 us throughout)
-  const I8Deal deal = a.passes ? I8Deal{(int)a.pass_rows, 1, 1, false} : i8_deal(a.m, a.n, p.nk);
+  const I8Deal deal = a.passes ? I8Deal{(int)a.pass_rows, 1, 1, false} : few ? i8_deal_few(a.n, p.nk) : i8_deal(a.m, a.n, p.nk);
   const bool pair = deal.pair;
   p.rt = (int)((a.n + per_tile * (pair ? 2 : 1) - 1) / (per_tile * (pair ? 2 : 1)));
   p.tn = deal.tn;
