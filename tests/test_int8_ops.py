@@ -55,7 +55,7 @@ def check_product(y, q, qs, w, ws, bias, dtype, msg=""):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k", [(1, 1), (1, 15), (3, 16), (7, 33), (1, 4096), (9, 1000), (130, 2048), (5, 2049), (2, 4100), (3, 16384), (2, 16400),
-                                    (2, 40007), (1, 131072), (1500, 64)])
+                                    (2, 40007), (1, 131072), (1500, 64), (41003, 48), (21001, 1040), (10003, 2064), (5003, 4109)])
 def test_quantize_matches_exact_codes(ops, dtype, rows, k):
     gen = torch.Generator(device="cuda").manual_seed(rows * 7 + k)
     x = torch.randn(rows, k, device="cuda", generator=gen).to(dtype)

@@ -5,7 +5,7 @@
 // every result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once (copies of it as often as asked).
-// 28672x8192 fp16 in 125 us, 5.6 TB/s, 0.87 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 231, 5.1 TB/s.
+// 28672x8192 fp16 in 116 us, 6.1 TB/s, 0.94 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 233, 5.0 TB/s.
 #include "int8_codes.cuh"
 
 namespace gguf_b200 {
@@ -22,15 +22,26 @@ __device__ __forceinline__ void i8q_store(uint4 c, int8_t* __restrict__ q, int64
 }
 
 // LANES threads a row, 256 / LANES rows a block; HOLD units of a thread stay in registers between the maximum and the codes, what is
-// beyond is read again
-template <typename T, bool VEC, int LANES, int HOLD>
-__global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD * sizeof(T) <= 8 ? 4 : 2) : 2) i8_quantize_kernel(const I8Quantize p) {
+// beyond is read again.  AHEAD: a block that walks over many rows asks for the next one while it makes this one's codes.
+template <typename T, bool VEC, int LANES, int HOLD, bool AHEAD>
+__global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 5 : HOLD * sizeof(T) <= 8 ? 4 : 2) : 2) i8_quantize_kernel(const I8Quantize p) {
   __shared__ uint32_t s_top[2][8];
   int turn = 0;
   const int lane = threadIdx.x % LANES;
   pdl_wait();
   pdl_trigger();
   const int64_t rows = p.n_used ? *p.n_used : p.rows;
+  T next[AHEAD ? HOLD : 1][I8Q_UNIT];
+  auto ask = [&](int64_t row) {
+    const T* x = static_cast<const T*>(p.x) + (row < rows ? row : 0) * p.ldx;
+    const int64_t k = row < rows ? p.k : 0;
+#pragma unroll
+    for (int h = 0; h < (AHEAD ? HOLD : 0); ++h) {
+      const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
+      if (at < k) i8q_load<T, VEC>(x, k, at, next[h]);
+    }
+  };
+  ask((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES);
   for (int64_t r0 = (int64_t)blockIdx.x * (256 / LANES); r0 < rows; r0 += (int64_t)gridDim.x * (256 / LANES)) {
     const int64_t r = r0 + threadIdx.x / LANES;
     const bool live = r < rows;
@@ -41,8 +52,14 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD *
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
       const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
-      if (at < k) i8q_load<T, VEC>(x, k, at, v[h]);
+      if (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < I8Q_UNIT; ++i) v[h][i] = next[AHEAD ? h : 0][i];
+      } else if (at < k) {
+        i8q_load<T, VEC>(x, k, at, v[h]);
+      }
     }
+    ask(r + (int64_t)gridDim.x * (256 / LANES));
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
       if ((int64_t)(h * LANES + lane) * I8Q_UNIT < k) top = i8q_top<T>(v[h], top);
@@ -99,10 +116,15 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 ? 5 : HOLD *
   }
 }
 
+// Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 116 us (125 without),
+// 28672x4096 65.8 (68.4), but 4096x4096 12.2 (10.8); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the rest: rows that are
+// read by single values, 100000x500, 90 us (97 with 64).
 template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quantize_form(const I8Quantize& a, cudaStream_t stream) {
   const int per = 256 / LANES;
-  const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 64;
-  return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
+  const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 16;
+  if constexpr (VEC && sizeof(T) == 2 && HOLD == 2)
+    if (blocks >= 148 * 32) return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, true>, dim3(148 * 16), dim3(256), 0, stream, a);
+  return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
 }
 // Two units a thread where there are rows enough to fill the GPU; a block a row where there are not.
 template <typename T, bool VEC> static cudaError_t i8_quantize_rows(const I8Quantize& a, cudaStream_t stream) {
