@@ -115,6 +115,31 @@ def test_route_choices_next_to_one_another(ops, scoring):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("e,k", [(60, 8), (300, 32), (512, 5), (33, 32)])
+def test_route_runs_of_equals(ops, scoring, with_bias, e, k):
+    """Runs of equal, or nearly equal, choices that begin before the last place and end behind it, of a few experts and of more than a warp has lanes."""
+    gen = torch.Generator().manual_seed(e + k)
+    rows = []
+    for run in (2, 3, 9, 31, 32, 33, 34, 40, e):
+        for start in (0, 1, k - 1, k, max(0, k - run), max(0, k + 1 - run)):
+            row = torch.linspace(3, -3, e) + 1e-3 * torch.rand(e, generator=gen)
+            row[start:start + run] = row[min(start, e - 1)]
+            row[e - 3:] = torch.where(torch.rand(3, generator=gen) > 0.5, -INF, row[e - 3:])
+            rows.append(row[torch.randperm(e, generator=gen)])
+            rows.append(torch.nextafter(rows[-1], torch.tensor(9.0)).where(torch.rand(e, generator=gen) > 0.5, rows[-1]))
+    logits = torch.stack(rows)
+    logits[3, ::2] = INF
+    logits[5, ::3], logits[5, 1::3] = INF, torch.finfo(torch.float32).max
+    bias = torch.full((e,), 0.125) if with_bias else None
+    for renormalize in (True, False):
+        kw = dict(scoring=scoring, n_group=1, topk_group=1, renormalize=renormalize)
+        check(ops.moe_route(logits.cuda(), k, bias=None if bias is None else bias.cuda(), **kw), route(logits, k, bias=bias, **kw),
+              scoring == "softmax" and not renormalize)
+
+
+@pytest.mark.gpu
 def test_route_strides_streams_and_empty(ops):
     gen = torch.Generator(device="cuda").manual_seed(8)
     big = torch.randn(30, 201, device="cuda", generator=gen)

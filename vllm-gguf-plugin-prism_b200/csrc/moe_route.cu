@@ -9,12 +9,14 @@
 //
 // One warp a token, expert 32 j + l in lane l.  A choice becomes an unsigned key of the same order, and the maximum over the warp is a
 // hardware reduction.  In the first pass a key is 32 bits, the lowest of which say which of a lane's experts it is; where what is left of the
-// numbers (in fp32, scores with an error bound) does not settle an order that matters, the row is done again with 64-bit keys: of
-// scores about one row in a thousand, of fp32 logits those with equals.
+// numbers (in fp32, scores with an error bound) does not settle an order that matters, keys are taken until the next one is out of
+// question, and these candidates, a lane each, are ordered by 64-bit keys: of scores one row in some hundred, of fp32 logits those with equals.
+// More than 32 candidates, an order of groups that is not settled and a softmax with a bias (which wants its sum in fp64) do the whole row again.
 //
-// Bound by the integer pipe, which runs at half the issue rate, and by the last row that is done twice: 8192 tokens, 256 experts in eight
-// groups with a bias, 19.5 us (45 with 64-bit keys throughout, 24 with keys that kept 0 for "out", exact maxima for every row and fp64 in
-// the weights); without groups and bias 8.5.  A token alone 2.5, of which the launch is most.
+// Bound by the integer pipe, which runs at half the issue rate, and by the last row that is done again: 8192 tokens, 256 experts in eight
+// groups with a bias, 15.4 us (17.8 where a row is among them whose groups are not settled; 45 with 64-bit keys throughout, 24 with keys that
+// kept 0 for "out", exact maxima for every row and fp64 in the weights, 19 to 20 with whole rows done again); fp32 logits with equals, no groups,
+// 11.1 (16.2 with whole rows, though 6.8 and not 6.6 for 64 experts without equals).  A token alone 2.5, of which the launch is most.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -185,13 +187,13 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); t < p.tokens; t += (int64_t)gridDim.x * 4) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
     auto least = [](float v) { return fmaxf(v, -INFINITY); };              // (a NaN becomes -infinity)
-    auto most = [](float v) { return fminf(v, 3.402823466e+38f); };
+    auto logit = [&](int e) { return fminf(least(to_float<T>(row[e])), 3.402823466e+38f); };   // (+infinity is the largest number)
     float x[V];
     uint32_t key[V];   // V is a power of two: the lowest bits hold V - 1 - j
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int e = 32 * j + lane;
-      x[j] = e < p.experts ? least(to_float<T>(row[e])) : -INFINITY;
+      x[j] = e < p.experts ? logit(e) : -INFINITY;
     }
     // A softmax: the largest logit and the sum, where they are needed.  (Weights that are divided by their own sum, of experts chosen by
     // their logits, go by the first choice.)
@@ -199,10 +201,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
     if (!p.sigmoid && (SCORES || !p.renormalize)) {
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x[j] = most(x[j]);
-        top = max(top, route_key(x[j]));
-      }
+      for (int j = 0; j < V; ++j) top = max(top, route_key(x[j]));
       top = warp_max(top);
       if (!route_out(top)) high = route_value(top);
       if (!p.renormalize) {
@@ -215,10 +214,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
       float s[V];
       if (p.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          x[j] = most(x[j]);
-          s[j] = route_rcp(1.f + route_exp(-x[j]));
-        }
+        for (int j = 0; j < V; ++j) s[j] = route_rcp(1.f + route_exp(-x[j]));
       } else {
         float sum = 0.f;
 #pragma unroll
@@ -262,24 +258,46 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
               key[i + j + d] = min(u, v);
             }
     // Of equal keys the one in the lowest lane is taken: the same j, so the lowest expert.  16-bit logits lose nothing in their keys.
+    // Where they may have, keys are taken until the next one is below the last for certain: these and no others can be the top_k best.
     constexpr bool CHECK = SCORES || sizeof(T) == 4;
-    int id = -1;
+    const bool grouped = sure;
+    int id = -1, i = 0;
     uint32_t before = 0;
 #pragma unroll 1
-    for (int i = 0; i < p.top_k + (CHECK ? 1 : 0); ++i) {
+    for (; i < (CHECK ? 33 : p.top_k); ++i) {
       const uint32_t best = warp_max(key[0]);
       if (route_out(best)) break;
-      if (CHECK && i > 0) sure = sure && (SCORES ? route_above<V>(route_value(before), route_value(best), off) : (before / V) > (best / V));
+      if (CHECK && i > 0) {
+        const bool above = SCORES ? route_above<V>(route_value(before), route_value(best), off) : (before / V) > (best / V);
+        sure = sure && above;
+        if (i >= p.top_k && above) break;
+      }
       before = best;
       const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-      if (lane == i && i < p.top_k) id = 32 * (V - 1 - (int)(best & (V - 1))) + owner;
+      if (lane == i) id = 32 * (V - 1 - (int)(best & (V - 1))) + owner;
       if (lane == owner) {
 #pragma unroll
         for (int j = 0; j + 1 < V; ++j) key[j] = key[j + 1];
         key[V - 1] = 0;
       }
     }
-    if (CHECK && !sure) {
+    if (CHECK && __builtin_expect(!sure, 0) && grouped && i < 33 && (!SCORES || p.sigmoid)) {   // (a softmax wants its sum in fp64 too)
+      uint64_t mine = 0;
+      if (id >= 0) {
+        const double d = (double)logit(id);
+        mine = route_key(SCORES ? 1.0 / (1.0 + exp(-d)) + (double)p.bias[id] : d);
+      }
+      int e = -1;
+#pragma unroll 1
+      for (int i = 0; i < p.top_k; ++i) {
+        const uint64_t best = warp_max(mine);
+        if (best == 0) break;
+        const unsigned first = __reduce_min_sync(0xffffffffu, mine == best ? (unsigned)id : 0xffffffffu);
+        if (lane == i) e = (int)first;
+        if ((unsigned)id == first) mine = 0;
+      }
+      id = e;
+    } else if (CHECK && __builtin_expect(!sure, 0)) {
       uint64_t wide[V];
       if constexpr (SCORES) {
         double s[V], all = 0.0;
@@ -297,8 +315,10 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
         for (int j = 0; j < V; ++j) wide[j] = route_key((double)x[j]);
       }
       id = route_exact<V, SCORES>(p, wide, lane);
+    } else if (CHECK && lane >= p.top_k) {
+      id = -1;
     }
-    const float v = id >= 0 ? most(to_float<T>(row[id])) : 0.f;
+    const float v = id >= 0 ? logit(id) : 0.f;
     if (!SCORES && p.renormalize && !p.sigmoid) high = __shfl_sync(0xffffffffu, v, 0);
     float w = 0.f;
     if (id >= 0) {
