@@ -358,6 +358,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
   const uint32_t accum_s = smem_u32(accum), drained_s = smem_u32(drained);
   auto item = [&](int i, int j, bool waited) { return p.passes ? i8_item<GLU, PAIR>(p, s_list, i, j, (int)rank, waited) : i8_item<GLU, PAIR>(p, i, (int)rank, waited); };
 
+  float ws = 0.f, bias = 0.f, scale = 1.f, unit = 1.f, next_ws = 0.f, next_bias = 0.f;   // epilogue: of this lane's row and (scale, to) this thread's token
+  int to = 0;
   if (warp == 0 || warp == 2 || warp == 3) {
     // ---------------- loaders ----------------
     // Three warps take the stages in turn: a stage's wait, announcement and two copies take one warp 440 clocks to issue, most of the 512
@@ -452,36 +454,51 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     const bool wide_y = p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
     int buf = 0, turn = 0;
     uint32_t aph = 0;
+    // this lane's row: of 128, or, gate and up, of 64 gate rows or (lanes with bit 3) their up rows
+    const int r = GLU ? quad / 2 + (lane >> 4) * 8 + (lane & 7) : row;
+    const bool down = !GLU && p.passes;   // (left to the sum over the experts: scale of the token, routing weight)
+    // What an item's end looks up in memory, a token a thread and a row a lane: asked for while the item before it is on its way out.
+    auto older = [](const float* q) { return __int_as_float(ld_older(reinterpret_cast<const int32_t*>(q))); };
+    auto look_up = [&](const I8Item& t, bool waited) {
+      const int at = t.x0 + tid, n = t.n0 + r;
+      const bool mine = tid < t.rows, live = n < p.n;
+      scale = !FEW && !down && mine ? p.q_scale[at] : 1.f;
+      to = !(down && mine) ? at : waited ? p.sorted[at] : ld_older(p.sorted + at);
+      unit = !down ? 1.f : waited ? p.w_unit[t.e] : older(p.w_unit + t.e);
+      const float* w = p.w_scale + t.a_row + r + (GLU && (lane & 8) ? p.n : 0);
+      next_ws = !live ? 0.f : waited ? *w : older(w);
+      next_bias = !GLU && live ? i8_bias(p, n) : 0.f;
+    };
+    if (down && first < n_items) look_up(item(first, 0, false), false);
     pdl_wait();
+    if (!FEW && !down && first < n_items) look_up(item(first, 0, true), true);
     for (int i = first, j = 0; i < n_items; i += step, ++j) {
       const I8Item t = item(i, j, true);
       float* xs = s_scale + (FEW ? 0 : turn * 256);   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
       int* xr = s_row + turn * 256;
       turn ^= 1;
-      const bool down = !GLU && p.passes;   // (left to the sum over the experts: scale of the token, routing weight)
-      for (int c = tid; c < p.tn; c += 32 * I8_EPI) {
-        const int at = t.x0 + c;
-        if (!FEW) xs[c] = c < t.rows && !down ? p.q_scale[at] : 1.f;
-        xr[c] = c < t.rows && down ? p.sorted[at] : at;
+      if (tid < p.tn) {
+        if (!FEW) xs[tid] = scale;
+        xr[tid] = FEW ? t.x0 + tid : to;
       }
       if constexpr (FEW) if (i == first) {   // (the same for all of a CTA's items)
         i8_few_codes<FewT>(p, kb0 * I8_BK, kb1 * I8_BK, smem_u32(smem + p.codes_off), xs, reinterpret_cast<uint32_t*>(s_stage), tid);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(coded);
+        look_up(t, true);   // (not ahead of the codes: they would wait for it)
       }
-      // this lane's row: of 128, or, gate and up, of 64 gate rows or (lanes with bit 3) their up rows
-      const int r = GLU ? quad / 2 + (lane >> 4) * 8 + (lane & 7) : row, n = t.n0 + r;
+      const int n = t.n0 + r;
       const bool live = n < p.n, wide = wide_y && t.n0 + quad + 32 <= p.n;
-      float ws = live ? p.w_scale[t.a_row + r + (GLU && (lane & 8) ? p.n : 0)] : 0.f;
-      if (down) ws = ws * p.w_unit[t.e] * p.unit;
+      ws = down ? next_ws * unit * p.unit : next_ws;
+      bias = next_bias;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
+      if (i + step < n_items) look_up(item(i + step, j + 1, true), true);
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
       __syncwarp();
       tc_fence_after();
       if (p.split == 1) {
         const uint32_t d = t_lane + (uint32_t)(buf * p.tn);
-        const float bias = !GLU && live ? i8_bias(p, n) : 0.f;
         for (int c0 = turn16; c0 < t.rows; c0 += 4 * I8_EPI) {
           uint32_t v[16];
           tmem_ld16(d + (uint32_t)c0, v);
@@ -566,7 +583,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     if (warp >= 4 && (p.split == 8 ? quad >> 5 == (int)rank >> 1 : mine)) {
       const int n = t.n0 + row;
       const bool live = mine && n < p.n, wide = p.split <= 4 && p.dtype != DT_F32 && p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && t.n0 + quad + 32 <= p.n;
-      const float ws = live ? p.w_scale[t.a_row + row] : 0.f, bias = live ? i8_bias(p, n) : 0.f;
       const uint32_t from0 = ring + (uint32_t)(row & (per - 1)) * pitch;
       for (int c0 = turn16; c0 < t.rows; c0 += 4 * I8_EPI) {
         uint32_t v[16];
