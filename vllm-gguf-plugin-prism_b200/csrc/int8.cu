@@ -148,8 +148,6 @@ __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, uint32_t 
   mbar_wait_or(bar, parity, gave_up);
   return lds32(gave_up) == 0u;
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // (the approximate exponential and quotient are off by a few units in the last place, 2^-21 of the result)
 __device__ __forceinline__ float i8_silu(float g) {
   float r;

@@ -1,8 +1,11 @@
 // The routed expert step around its products of 8-bit integers: the order of the slots, and the sum over a token's experts.
 //
-//   i8_plan_kernel  slots (token * top_k + j) sorted by expert, in their order; every expert's rows in passes of like size.  Blocks take
-//                   equal runs of slots; each counts all slots for itself (16 k of them are 64 KB, from L2), those ahead of its run apart,
-//                   and places its own: no block waits for another.  More blocks, one an expert, look for the expert's largest scale.
+//   i8_plan_kernel  slots (token * top_k + j) sorted by expert, in their order; every expert's rows in passes of like size.  One block
+//                   takes up to 1024 slots; of more, a cluster of eight blocks takes equal runs, which learn of one another's counts
+//                   through shared memory.  A warp counts its share of the run and, once the sums over warps, blocks and experts are
+//                   there, places it, 32 slots at a time.  More blocks, one an expert, look for the expert's largest scale.
+//                   Latencies bound it: 16384 slots of 64 experts 8.4 us behind the kernel ahead, 64 slots 3.1 (10.6 with 16 blocks that
+//                   each counted all slots and summed over their warps for every 1024 of them, and 4.5 with divisions between the sums).
 //   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * factor, in fp32, rounded once
 //
 // The experts' results y = D * w_scale travel from the down product to the sum in fp16 for 16-bit tokens (fp32 for fp32): half the bytes of
@@ -17,27 +20,30 @@
 
 namespace gguf_b200 {
 
-constexpr int I8_MAX_EXPERTS = 256, I8_PLAN_BLOCKS = 32;
+constexpr int I8_MAX_EXPERTS = 256, I8_PLAN_BLOCKS = 8;
 
 // An expert's c rows in passes of like size: whole groups of 16 tokens but for the last, at most pass_rows
 __device__ __forceinline__ int i8_pass_size(int c, int pass_rows) {
   const int np = (c + pass_rows - 1) / pass_rows;
   return np > 0 ? ((c + np - 1) / np + 15) / 16 * 16 : 16;
 }
-__device__ __forceinline__ int i8_pass_count(int c, int pass_rows) {
-  const int per = i8_pass_size(c, pass_rows);
-  return (c + per - 1) / per;
-}
 
-__global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int blocks, int run) {
+__global__ void __launch_bounds__(1024, 1) i8_plan_kernel(const I8Plan p, int blocks, int run) {
+  __shared__ int32_t s_cnt[32][I8_MAX_EXPERTS + 1];   // a warp's slots of an expert; then where its next one goes, from the block's first
+  __shared__ int32_t s_run[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS];   // the block's slots, all, the block's first place
+  __shared__ int32_t s_size[I8_MAX_EXPERTS], s_passes[I8_MAX_EXPERTS], s_order[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS];   // block 0: passes
+  __shared__ float s_top[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.experts, slots = (int)p.slots;
+  // One block for all slots has one for every thread.
+  const bool alone = blocks == 1, counts = (int)blockIdx.x < blocks;
+  const int warps = alone ? ((slots + 31) / 32 + 7) / 8 * 8 : 32;
+  if (counts)
+    for (int i = threadIdx.x; i < warps * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
   pdl_wait();
   pdl_trigger();
-  __shared__ int32_t s_cnt[32][I8_MAX_EXPERTS + 1];   // first: counts of all slots, by warp modulo 8; then a warp's slots of a step, and its first place
-  __shared__ int32_t s_before[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS], s_order[I8_MAX_EXPERTS];
-  __shared__ float s_top[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.experts;
-  if ((int)blockIdx.x >= blocks) {   // largest scale of an expert (a scale that is not finite: as if it were not there)
+  if (!counts) {   // largest scale of an expert (a scale that is not finite: as if it were not there)
     const int e = blockIdx.x - blocks;
+    if (e >= E) return;
     float top = 0.f;
     for (int64_t i = threadIdx.x; i < p.h; i += 1024) {
       const float v = fabsf(p.w2_scale[e * p.h + i]);
@@ -58,132 +64,146 @@ __global__ void __launch_bounds__(1024) i8_plan_kernel(const I8Plan p, int block
     }
     return;
   }
-  const int slots = (int)p.slots, s0 = min(slots, (int)blockIdx.x * run), s1 = min(slots, s0 + run);
-  // Whether a slot has a valid expert, and how many lanes below this one have the same
-  auto match = [&](int e, unsigned& below) {
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const bool valid = e >= 0 && e < E;
-    below = __popc(same & ((1u << lane) - 1u));
-    if (valid && below == 0) s_cnt[warp][e] = __popc(same);
-    return valid;
+  // A warp's slots: a 32nd of the block's, in their order, 32 at a time
+  const int own = run / 32, s0 = min(slots, (int)blockIdx.x * run + warp * own), s1 = min(slots, s0 + own);
+  // Lanes with this one's expert, and how many of them are below it
+  auto match = [&](int e, unsigned& same) {
+    same = __match_any_sync(0xffffffffu, e);
+    return __popc(same & ((1u << lane) - 1u));
   };
-  // Of counts by warp: where a warp's first slot of the expert goes, from `at` on; returns where the next would
-  auto spread = [&](int e, int at, int warps) {
+  auto valid = [&](int e) { return e >= 0 && e < E; };
+  int my_e = -1, my_below = 0;
+  if (alone && s0 + lane < s1) my_e = p.topk_ids[s0 + lane];
+  __syncthreads();
+  if (alone) {
+    unsigned same;
+    my_below = match(my_e, same);
+    if (valid(my_e) && my_below == 0) s_cnt[warp][my_e] = __popc(same);
+  } else {
+    for (int b = s0 + lane; b < s1; b += 8 * 32) {   // (eight loads in flight)
+      int e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = b + i * 32 < s1 ? p.topk_ids[b + i * 32] : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (valid(e[i])) atomicAdd(&s_cnt[warp][e[i]], 1);
+    }
+  }
+  __syncthreads();
+  int total = 0, before = 0;   // of expert threadIdx.x: in all blocks, in those ahead
+  if ((int)threadIdx.x < E) {
     for (int w0 = 0; w0 < warps; w0 += 8) {   // (eight loads in flight)
       int v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = s_cnt[w0 + i][e];
+      for (int i = 0; i < 8; ++i) v[i] = s_cnt[w0 + i][threadIdx.x];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s_cnt[w0 + i][e] = at;
-        at += v[i];
+        s_cnt[w0 + i][threadIdx.x] = total;
+        total += v[i];
       }
     }
-    return at;
-  };
-  // One block for all slots counts them and places them in one go.
-  const bool alone = blocks == 1;
-  const int my_slot = threadIdx.x, warps = alone ? ((slots + 31) / 32 + 7) / 8 * 8 : 32;
-  const int my_e = alone && my_slot < slots ? p.topk_ids[my_slot] : -1;
-  unsigned my_below = 0;
-  bool my_valid = false;
-  for (int i = threadIdx.x; i < (alone ? warps : 16) * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
-  __syncthreads();
-  if (alone) {
-    my_valid = match(my_e, my_below);
-  } else {
-    for (int b = threadIdx.x; b < slots; b += 8 * 1024) {   // (eight loads in flight)
-      int e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = b + i * 1024 < slots ? p.topk_ids[b + i * 1024] : -1;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (e[i] >= 0 && e[i] < E) atomicAdd(&s_cnt[(warp & 7) + (b + i * 1024 < s0 ? 0 : 8)][e[i]], 1);
-    }
+    s_run[threadIdx.x] = total;
   }
-  __syncthreads();
-  const bool by_size = p.pass_rows > 64 && blockIdx.x == 0;
+  if (!alone) {
+    cluster_arrive();
+    cluster_wait();
+    if ((int)threadIdx.x < E) {
+      int c[I8_PLAN_BLOCKS];
+#pragma unroll
+      for (int i = 0; i < I8_PLAN_BLOCKS; ++i) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_run[threadIdx.x])), "r"(i));
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c[i]) : "r"(at) : "memory");
+      }
+      total = 0;
+#pragma unroll
+      for (int i = 0; i < I8_PLAN_BLOCKS; ++i) {
+        if (i < (int)blockIdx.x) before += c[i];
+        total += c[i];
+      }
+    }
+    cluster_arrive();   // (the others' counts are not read again; waited for before the end)
+  }
+  const bool by_size = p.pass_rows > 64;
   if ((int)threadIdx.x < E) {
     const int e = threadIdx.x;
-    int before = 0, total = 0;
-    if (alone) {
-      total = spread(e, 0, warps);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        before += s_cnt[i][e];
-        total += s_cnt[8 + i][e];
-      }
-      total += before;
-    }
-    s_before[e] = before;
     s_total[e] = total;
-    if (by_size) s_pass[e] = i8_pass_size(total, p.pass_rows);
+    s_next[e] = before;
+    if (blockIdx.x == 0) {
+      s_size[e] = i8_pass_size(total, p.pass_rows);
+      s_passes[e] = (total + s_size[e] - 1) / s_size[e];
+      s_order[e] = e;
+    }
   }
   __syncthreads();
   // Large passes are dealt out by size, the largest first: CTAs that take them in turn then get like shares.
-  if (by_size) {
-    const int e = threadIdx.x >> 2, size = e < E ? s_pass[e] : 0;
+  if (blockIdx.x == 0 && by_size) {
+    const int team = E <= 64 ? 16 : 4, e = threadIdx.x / team, size = e < E ? s_size[e] : 0;
     int rank = 0;
-    for (int o = threadIdx.x & 3; o < E; o += 4) {
-      const int other = s_pass[o];
+    for (int o = threadIdx.x % team; o < E; o += team) {
+      const int other = s_size[o];
       rank += other > size || (other == size && o < e);
     }
-    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-    if (e < E && (threadIdx.x & 3) == 0) s_order[rank] = e;
+    for (int m = 1; m < team; m <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, m);
+    if (e < E && threadIdx.x % team == 0) s_order[rank] = e;
     __syncthreads();
   }
-  if (warp == 0) {   // prefix sums over the experts: rows, and passes in that order
-    int rows = 0, ps = 0;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, c = e < E ? s_total[e] : 0, o = by_size && e < E ? s_order[e] : e;
-      const int np = e < E && blockIdx.x == 0 ? i8_pass_count(s_total[o], p.pass_rows) : 0;
-      int a = c, b = np;
+  // Prefix sums over the experts: rows (warp 0), and passes in that order (block 0's warp 1).  A lane takes neighbours.
+  if (warp == 0 || (warp == 1 && blockIdx.x == 0)) {
+    const int per = (E + 31) / 32, e0 = min(E, lane * per), e1 = min(E, e0 + per);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) sum += warp == 0 ? s_total[e] : s_passes[s_order[e]];
+    int a = sum;
 #pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, a, m), v = __shfl_up_sync(0xffffffffu, b, m);
-        if (lane >= m) { a += u; b += v; }
-      }
-      if (e < E) {
-        s_next[e] = rows + a - c + s_before[e];
-        s_pass[o] = ps + b - np;
-      }
-      rows += __shfl_sync(0xffffffffu, a, 31);
-      ps += __shfl_sync(0xffffffffu, b, 31);
+    for (int m = 1; m < 32; m <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, a, m);
+      if (lane >= m) a += u;
     }
-    if (lane == 0 && blockIdx.x == 0) {
-      p.n_passes[0] = ps;
-      p.n_passes[1] = rows;
+    if (lane == 31 && blockIdx.x == 0) p.n_passes[warp == 0 ? 1 : 0] = a;
+    a -= sum;
+    for (int e = e0; e < e1; ++e) {
+      if (warp == 0) {
+        s_next[e] += a;
+        a += s_total[e];
+      } else {
+        s_pass[s_order[e]] = a;
+        a += s_passes[s_order[e]];
+      }
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int e = warp; e < E; e += 32) {
-      const int c = s_total[e], per = i8_pass_size(c, p.pass_rows);
-      for (int i = lane; i * per < c; i += 32) static_cast<int4*>(p.passes)[s_pass[e] + i] = make_int4(e, s_next[e] + i * per, min(per, c - i * per), 0);
-    }
   auto put = [&](int s, int at) {
     if (at >= 0) p.sorted[at] = s;
     p.place[s] = at;
   };
   if (alone) {
-    if (my_slot < slots) put(my_slot, my_valid ? s_next[my_e] + s_cnt[warp][my_e] + (int)my_below : -1);
-    return;
+    if (s0 + lane < s1) put(s0 + lane, valid(my_e) ? s_next[my_e] + s_cnt[warp][my_e] + my_below : -1);
+  } else {
+    for (int b = s0; b < s1; b += 8 * 32) {
+      int e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = b + i * 32 + lane < s1 ? p.topk_ids[b + i * 32 + lane] : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (b + i * 32 >= s1) break;
+        unsigned same;
+        const int below = match(e[i], same);
+        const int at = valid(e[i]) ? s_cnt[warp][e[i]] + below : -1;
+        __syncwarp();
+        if (valid(e[i]) && below == 0) s_cnt[warp][e[i]] += __popc(same);
+        __syncwarp();
+        if (b + i * 32 + lane < s1) put(b + i * 32 + lane, at < 0 ? -1 : s_next[e[i]] + at);
+      }
+    }
   }
-  __syncthreads();   // (s_next moves on below)
-  for (int b = s0; b < s1; b += 1024) {
-    for (int i = threadIdx.x; i < 32 * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
-    __syncthreads();
-    const int s = b + threadIdx.x, e = s < s1 ? p.topk_ids[s] : -1;
-    unsigned below;
-    const bool valid = match(e, below);
-    __syncthreads();
-    if ((int)threadIdx.x < E) s_next[threadIdx.x] = spread(threadIdx.x, s_next[threadIdx.x], 32);
-    __syncthreads();
-    if (s < s1) put(s, valid ? s_cnt[warp][e] + (int)below : -1);
-    __syncthreads();
+  if (blockIdx.x == 0) {   // four threads an expert
+    const int e = threadIdx.x >> 2;
+    if (e < E) {
+      const int c = s_total[e], per = s_size[e];
+      for (int i = threadIdx.x & 3; i < s_passes[e]; i += 4) static_cast<int4*>(p.passes)[s_pass[e] + i] = make_int4(e, s_next[e] + i * per, min(per, c - i * per), 0);
+    }
   }
+  if (!alone) cluster_wait();
 }
 
 // Tokens of an expert's pass, at most 256: its average share of the slots and three standard deviations
@@ -198,9 +218,9 @@ int64_t i8_moe_passes(int64_t slots, int64_t experts, int64_t pass_rows) {
 }
 int launch_i8_plan(const I8Plan& a, cudaStream_t stream) {
   if (a.experts < 1 || a.experts > I8_MAX_EXPERTS || a.slots > 1 << 24) return E_BAD_SHAPE;
-  const int64_t steps = (a.slots + 1023) / 1024, per = (steps + I8_PLAN_BLOCKS - 1) / I8_PLAN_BLOCKS;
-  const int run = (int)per * 1024, blocks = (int)((a.slots + run - 1) / run);
-  return launch_pdl(i8_plan_kernel, dim3((unsigned)(blocks + a.experts)), dim3(1024), 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
+  const int blocks = a.slots <= 1024 ? 1 : I8_PLAN_BLOCKS, run = (int)((a.slots + blocks - 1) / blocks + 1023) / 1024 * 1024;
+  const dim3 grid((unsigned)round_up(blocks + a.experts, blocks));
+  return launch_pdl_cluster(i8_plan_kernel, grid, dim3(1024), (unsigned)blocks, 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
 }
 
 // Eight columns a thread, ROWS experts' rows in flight: four of fp32, eight of fp16, four of fp16 where a token has no more experts (150 blocks of
