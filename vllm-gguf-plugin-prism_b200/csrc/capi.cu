@@ -951,26 +951,26 @@ int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_
   q2.q = reinterpret_cast<int8_t*>(base + L.o_q2); q2.ldq = i8_ld(I);
   q2.rows = slots; q2.k = I;
   q2.n_used = npass + 1;
-  const float unit = exp2f(ceilf(log2f((float)I)) - 1.f);   // 128 * 127 * I / unit <= 2^15
-  q2.sorted = sorted; q2.topk_ids = topk_ids; q2.topk_weights = topk_weights; q2.w_top = units + n_experts; q2.unit = unit;
-  q2.factor = reinterpret_cast<float*>(base + L.o_s2);
+  q2.scale = reinterpret_cast<float*>(base + L.o_s2);
   rc = launch_i8_quantize(q2, s);
   if (rc) return rc;
   // 5. down products, back in the order of the slots, divided by powers of two (int8_moe.cu)
+  const float unit = exp2f(ceilf(log2f((float)I)) - 1.f);   // 128 * 127 * I / unit <= 2^15
   a.w = static_cast<const int8_t*>(W2); a.ldw = ld2; a.w_scale = w2_scales;
-  a.q = q2.q; a.ldq = q2.ldq; a.q_scale = nullptr;
+  a.q = q2.q; a.ldq = q2.ldq; a.q_scale = q2.scale;
   a.dtype = dtype == DT_F32 ? DT_F32 : DT_F16;
   a.ldy = H;
   a.n = H; a.k = I;
   a.act = 0;
   a.sorted = sorted;
-  a.w_unit = units;
+  a.w_unit = units; a.w_top = units + n_experts; a.topk_weights = topk_weights;
+  a.factor = reinterpret_cast<float*>(base + L.o_s1);   // (the tokens' scales are done with)
   a.unit = 1.f / unit;
   rc = launch_i8_product(a, s);
   if (rc) return rc;
   // 6. weighted sum over the top_k slots of every token
   I8Sum y{};
-  y.y = base + L.o_h; y.out = Y; y.place = place; y.factor = q2.factor;
+  y.y = base + L.o_h; y.out = Y; y.place = place; y.factor = a.factor;
   y.tokens = tokens; y.top_k = top_k; y.h = H; y.dtype = dtype;
   return launch_i8_sum(y, s);
 }

@@ -60,7 +60,8 @@ struct I8Params {
   const int32_t* n_passes;
   int act;
   const int32_t* sorted;
-  const float* w_unit;
+  const float *w_unit, *w_top, *topk_weights;
+  float* factor;
   float unit;
   const void* x;           // FEW: [m][ldx], behind the ring the codes of this CTA's K (2 KB a stage)
   int64_t ldx;
@@ -492,6 +493,10 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
       bias = next_bias;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
       if (i + step < n_items) look_up(item(i + step, j + 1, true), true);
+      if (down && t.n0 == 0 && tid < t.rows) {   // (for the sum, while the products are made)
+        const int slot = xr[tid];
+        p.factor[slot] = p.q_scale[t.x0 + tid] * p.topk_weights[slot] * (p.w_top[t.e] / p.unit);
+      }
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
       __syncwarp();
       tc_fence_after();
@@ -764,6 +769,9 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.act = a.act;
   p.sorted = a.sorted;
   p.w_unit = a.w_unit;
+  p.w_top = a.w_top;
+  p.topk_weights = a.topk_weights;
+  p.factor = a.factor;
   p.unit = a.unit;
   p.x = a.x;
   p.ldx = a.ldx;

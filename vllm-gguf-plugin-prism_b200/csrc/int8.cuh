@@ -19,11 +19,6 @@ struct I8Quantize {
   const int32_t* scatter;
   int copies;
   const int32_t* n_used;
-  // factor != null (hidden rows of experts): instead of the scale, factor[sorted[r]] = scale * what the sum multiplies the slot's result by
-  const int32_t *sorted, *topk_ids;
-  const float *topk_weights, *w_top;
-  float unit;
-  float* factor;
 };
 int launch_i8_quantize(const I8Quantize& a, cudaStream_t stream);
 
@@ -47,9 +42,11 @@ struct I8Product {
   int64_t experts, max_passes, pass_rows;
   // ... gate and up product: w has n gate rows, then n up rows an expert; y[row] = act(gate) * up in fp32, in the order of q's rows
   int act;                   // 1 silu, 2 gelu; 0: down product
-  // ... down product: y[sorted[row]] = D * w_scale * w_unit[expert] * unit (q_scale and the routing weight are left to launch_i8_sum)
+  // ... down product: y[slot] = D * w_scale * w_unit[expert] * unit, slot = sorted[row]; what is left to launch_i8_sum,
+  // factor[slot] = q_scale * topk_weights[slot] * w_top[expert] / unit, is written beside it
   const int32_t* sorted;
-  const float* w_unit;
+  const float *w_unit, *w_top, *topk_weights;
+  float* factor;
   float unit;                // what the products are multiplied by
   // ... tokens that are not quantized yet (null: q is used; see i8_few): [m][ldx] in dtype
   const void* x;

@@ -5,7 +5,7 @@
 // every result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once (copies of it as often as asked).
-// 28672x8192 fp16 in 116 us, 6.1 TB/s, 0.94 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 233, 5.0 TB/s.
+// 28672x8192 fp16 in 113 us, 6.2 TB/s, 0.97 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 233, 5.0 TB/s.
 #include "int8_codes.cuh"
 
 namespace gguf_b200 {
@@ -90,14 +90,7 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
     for (int j = 0; j < copies; ++j) {
       const int64_t o = !live ? -1 : p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
       if (o < 0) continue;
-      if (lane == 0) {
-        if (p.factor) {
-          const int slot = p.sorted[r];
-          p.factor[slot] = scale * p.topk_weights[slot] * (p.w_top[p.topk_ids[slot]] * p.unit);
-        } else {
-          p.scale[o] = scale;
-        }
-      }
+      if (lane == 0) p.scale[o] = scale;
 #pragma unroll
       for (int h = 0; h < HOLD; ++h) {
         const int64_t at = (int64_t)(h * LANES + lane) * I8Q_UNIT;
@@ -116,9 +109,9 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
   }
 }
 
-// Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 116 us (125 without),
-// 28672x4096 65.8 (68.4), but 4096x4096 12.2 (10.8); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the rest: rows that are
-// read by single values, 100000x500, 90 us (97 with 64).
+// Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 113 us (125 without),
+// 28672x4096 65.0 (68.4), but 4096x4096 12.2 (10.5); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the rest: rows that are
+// read by single values, 100000x500, 87 us (97 with 64).
 template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quantize_form(const I8Quantize& a, cudaStream_t stream) {
   const int per = 256 / LANES;
   const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 16;
