@@ -7,9 +7,7 @@
 //                   Latencies bound it: 16384 slots of 64 experts 8.4 us behind the kernel ahead, 64 slots 3.1 (10.6 with 16 blocks that
 //                   each counted all slots and summed over their warps for every 1024 of them, and 4.5 with divisions between the sums).
 //   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * factor, in fp32, rounded once.  The down product writes the factors beside its
-//                   results (with the
-//                   look-ups in the hidden rows' quantizer that took 2 us longer for 16384 rows of 1024, and its other uses 3 to 5 %;
-//                   with them here, this kernel 4 us)
+//                   results (looked up by the hidden rows' quantizer they cost 2 us for 16384 rows of 1024; by this kernel, 4 us)
 //
 // The experts' results y = D * w_scale travel from the down product to the sum in fp16 for 16-bit tokens (fp32 for fp32): half the bytes of
 // the step's largest buffer.  They are divided by powers of two first, one above the expert's largest scale and one that brings the

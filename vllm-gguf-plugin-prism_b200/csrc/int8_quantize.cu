@@ -5,7 +5,8 @@
 // every result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once (copies of it as often as asked).
-// 28672x8192 fp16 in 113 us, 6.2 TB/s, 0.97 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 233, 5.0 TB/s.
+// 28672x8192 fp16 in 110 us, 6.4 TB/s, 0.99 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 195,
+// 6.0 TB/s.
 #include "int8_codes.cuh"
 
 namespace gguf_b200 {
@@ -22,8 +23,9 @@ __device__ __forceinline__ void i8q_store(uint4 c, int8_t* __restrict__ q, int64
 }
 
 // LANES threads a row, 256 / LANES rows a block; HOLD units of a thread stay in registers between the maximum and the codes, what is
-// beyond is read again.  AHEAD: a block that walks over many rows asks for the next one while it makes this one's codes.
-template <typename T, bool VEC, int LANES, int HOLD, bool AHEAD>
+// beyond is read again.  AHEAD: a block that walks over many rows asks for the next one while it makes this one's codes.  SCATTER:
+// see I8Quantize::scatter.
+template <typename T, bool VEC, int LANES, int HOLD, bool AHEAD, bool SCATTER>
 __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 5 : HOLD * sizeof(T) <= 8 ? 4 : 2) : 2) i8_quantize_kernel(const I8Quantize p) {
   __shared__ uint32_t s_top[2][8];
   int turn = 0;
@@ -60,6 +62,9 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
       }
     }
     ask(r + (int64_t)gridDim.x * (256 / LANES));
+    const int copies = SCATTER ? p.copies : 1;
+    int place = -1;   // of the first 32 copies, a lane each
+    if (SCATTER && live && (int)(threadIdx.x & 31) < copies) place = __ldg(p.scatter + r * copies + (threadIdx.x & 31));
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
       if ((int64_t)(h * LANES + lane) * I8Q_UNIT < k) top = i8q_top<T>(v[h], top);
@@ -82,13 +87,12 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
     const bool finite = top < 0x7f800000u, zero = !finite || top == 0;
     const float a = __uint_as_float(top), scale = finite ? a / 127.f : __uint_as_float(0x7fc00000u);
     const I8Row w = i8q_row(zero ? 1.f : a);
-    const int copies = p.scatter ? p.copies : 1;
     uint4 c[HOLD];
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) c[h] = zero ? make_uint4(0, 0, 0, 0) : i8q_unit<T>(v[h], w);
 #pragma unroll 4
     for (int j = 0; j < copies; ++j) {
-      const int64_t o = !live ? -1 : p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
+      const int64_t o = !live ? -1 : !SCATTER ? r : j < 32 ? __shfl_sync(0xffffffffu, place, j) : __ldg(p.scatter + r * copies + j);
       if (o < 0) continue;
       if (lane == 0) p.scale[o] = scale;
 #pragma unroll
@@ -102,22 +106,24 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
       i8q_load<T, VEC>(x, k, at, u);
       const uint4 c = zero ? make_uint4(0, 0, 0, 0) : i8q_unit<T>(u, w);
       for (int j = 0; j < copies; ++j) {
-        const int64_t o = p.scatter ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
+        const int64_t o = SCATTER ? (int64_t)__ldg(p.scatter + r * copies + j) : r;
         if (o >= 0) i8q_store(c, p.q + o * p.ldq, k, at);
       }
     }
   }
 }
 
-// Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 113 us (125 without),
-// 28672x4096 65.0 (68.4), but 4096x4096 12.2 (10.5); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the rest: rows that are
-// read by single values, 100000x500, 87 us (97 with 64).
+// Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 110 us (122 without),
+// 28672x4096 61.8 (64.8), 60000x1024 33.6 (33.1), but 4096x4096 12.2 (10.5); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the
+// rest: rows that are read by single values, 100000x500, 84 us (95 with 64).  Rows that go to places have a kernel of their own: without it the
+// others took longer (fp32 28672x8192 235, fp16 4096x4096 10.5 instead of 10.0), and so did a place looked up only when it is written to.
 template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quantize_form(const I8Quantize& a, cudaStream_t stream) {
   const int per = 256 / LANES;
   const int64_t blocks = (a.rows + per - 1) / per, most = 148 * 16;
+  if (a.scatter) return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, false, true>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
   if constexpr (VEC && sizeof(T) == 2 && HOLD == 2)
-    if (blocks >= 148 * 32) return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, true>, dim3(148 * 16), dim3(256), 0, stream, a);
-  return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
+    if (blocks >= 148 * 32) return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, true, false>, dim3(148 * 16), dim3(256), 0, stream, a);
+  return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, false, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
 }
 // Two units a thread where there are rows enough to fill the GPU; a block a row where there are not.
 template <typename T, bool VEC> static cudaError_t i8_quantize_rows(const I8Quantize& a, cudaStream_t stream) {
