@@ -5,8 +5,8 @@
 // every result it enters is NaN.
 //
 // Bound by memory: a row is read once, into registers (up to 64 values a thread), and written once (copies of it as often as asked).
-// 28672x8192 fp16 in 110 us, 6.4 TB/s, 0.99 of the copy rate (309 with codes by fp64 comparisons and 100 registers a thread); fp32 in 195,
-// 6.0 TB/s.
+// 28672x8192 fp16 in 106 us, 6.6 TB/s, the copy rate (two thirds of the bytes are read; 309 with codes by fp64 comparisons and 100 registers a
+// thread); fp32 in 194, 6.1 TB/s.
 #include "int8_codes.cuh"
 
 namespace gguf_b200 {
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256, VEC ? (HOLD * sizeof(T) <= 4 && !AHEAD ? 
 }
 
 // Rows ahead cost a block of five on an SM, so they are for 16-bit rows that fill the GPU many times over: 28672x8192 110 us (122 without),
-// 28672x4096 61.8 (64.8), 60000x1024 33.6 (33.1), but 4096x4096 12.2 (10.5); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the
+// 28672x4096 61.8 (64.8), 60000x1024 33.6 (33.1), all with one number to an instruction (int8_codes.cuh), but 4096x4096 12.2 (10.5); in fp32 28672x8192 279 (233).  At most 16 blocks an SM walk over the
 // rest: rows that are read by single values, 100000x500, 84 us (95 with 64).  Rows that go to places have a kernel of their own: without it the
 // others took longer (fp32 28672x8192 235, fp16 4096x4096 10.5 instead of 10.0), and so did a place looked up only when it is written to.
 template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quantize_form(const I8Quantize& a, cudaStream_t stream) {
