@@ -289,7 +289,8 @@ def experts(e, h, i, gen):
 
 MOE = [(1, 4, 2, 64, 32), (1, 64, 8, 256, 128), (3, 8, 1, 136, 264), (8, 64, 8, 512, 256), (33, 16, 4, 264, 392), (100, 8, 2, 384, 128), (257, 8, 8, 512, 384),
        (64, 256, 8, 128, 64), (600, 4, 3, 256, 136), (1500, 16, 4, 128, 256),
-       (128, 9, 8, 64, 32), (1025, 65, 1, 64, 32), (2049, 64, 4, 64, 32), (1500, 256, 7, 64, 32), (9001, 100, 2, 64, 32), (5, 64, 40, 64, 32), (7, 3, 2, 16408, 40)]
+       (128, 9, 8, 64, 32), (1025, 65, 1, 64, 32), (2049, 64, 4, 64, 32), (1500, 256, 7, 64, 32), (9001, 100, 2, 64, 32), (5, 64, 40, 64, 32), (7, 3, 2, 16408, 40),
+       (601, 4, 2, 1160, 40), (600, 3, 1, 2056, 32)]
 
 
 @pytest.mark.gpu

@@ -125,11 +125,15 @@ template <typename T, bool VEC, int LANES, int HOLD> static cudaError_t i8_quant
     if (blocks >= 148 * 32) return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, true, false>, dim3(148 * 16), dim3(256), 0, stream, a);
   return launch_pdl(i8_quantize_kernel<T, VEC, LANES, HOLD, false, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a);
 }
-// Two units a thread where there are rows enough to fill the GPU; a block a row where there are not.
+// Two units a thread where there are rows enough to fill the GPU; a block a row where there are not.  Rows that go to places, whose copies take
+// longest, have a unit a thread (2048 rows of 2048 to eight places 9.6 us, 10.6 with two; hidden rows of 1024 in fp32 22.6, but 20.8 with two).
 template <typename T, bool VEC> static cudaError_t i8_quantize_rows(const I8Quantize& a, cudaStream_t stream) {
   if (a.k > 512 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 4>(a, stream);
   if (a.k > 256 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 2>(a, stream);
   if (a.rows < 148 * 4) return i8_quantize_form<T, VEC, 256, 1>(a, stream);
+  if (a.scatter && a.k > 128 * I8Q_UNIT) return i8_quantize_form<T, VEC, 256, 1>(a, stream);
+  if (a.scatter && a.k > 64 * I8Q_UNIT) return i8_quantize_form<T, VEC, 128, 1>(a, stream);
+  if (a.scatter) return i8_quantize_form<T, VEC, 64, 1>(a, stream);
   if (a.k > 128 * I8Q_UNIT) return i8_quantize_form<T, VEC, 128, 2>(a, stream);
   if (a.k > 64 * I8Q_UNIT) return i8_quantize_form<T, VEC, 64, 2>(a, stream);
   return i8_quantize_form<T, VEC, 32, 2>(a, stream);
