@@ -217,8 +217,7 @@ int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_s
  * ld13 bytes apart) with w13_scales [E][2I], W2 [E][H][I] with w2_scales [E][H].  Tokens are quantized by the row, and so are the
  * hidden rows act(gate) * up, in fp32, of every slot; Y[t] = sum over j of topk_weights[t][j] * down, rounded to dtype once.
  * act: 1 silu, 2 gelu (erf form).  n_experts <= 256, top_k <= 256, tokens * top_k <= 2^24, tokens * H < 2^34, H and I multiples of 8; Y 16-byte
- * aligned.  For f16 / bf16 an expert's result is rounded to fp16 once on its way to the sum, in a range of its own.  Slots with an id outside [0, n_experts) contribute
- * nothing. */
+ * aligned.  Hidden rows, the experts' results and their sum are fp32 whatever dtype is.  Slots with an id outside [0, n_experts) contribute nothing. */
 int64_t gguf_b200_int8_moe_workspace_bytes(int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H, int64_t I);
 int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_t ld13, const float* w13_scales, const void* W2, int64_t ld2,
                              const float* w2_scales, void* Y, const int32_t* topk_ids, const float* topk_weights, void* workspace,

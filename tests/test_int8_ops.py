@@ -361,6 +361,26 @@ def test_moe_in_a_graph_with_the_router(ops):
         assert bool(((out[0].double() - want).abs() <= 2 * room).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,i", [(1, 8, 4, 256, 128), (40, 8, 2, 264, 136), (600, 4, 3, 128, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_moe_of_16_bit_tokens_sums_in_fp32(ops, t, e, k, h, i, dtype):
+    """Nothing between the tokens and the result has fewer than 32 bits: the room of fp32 tokens of the same values, and one rounding to the
+    type.  Rows of W2 with scales over eight powers of ten keep their precision too."""
+    gen = torch.Generator(device="cuda").manual_seed(t + i)
+    w13, s13, w2, _ = experts(e, h, i, gen)
+    s2 = 10.0 ** (-8 * torch.rand(e, h, device="cuda", generator=gen))
+    s2[:, 0], s2[:, 1] = 1.0, 1e-8
+    x = torch.randn(t, h, device="cuda", generator=gen).to(dtype)
+    weights_, ids = torch.randn(t, e, device="cuda", generator=gen).softmax(-1).topk(k, dim=-1)
+    ids = ids.to(torch.int32)
+    y = ops.int8_fused_moe(x, w13, s13, w2, s2, weights_, ids, "silu")
+    want, room = moe_want(x.float(), w13, s13, w2, s2, weights_, ids, "silu")
+    room = room + torch.finfo(dtype).eps / 2 * (want.abs() + room) + TINY[dtype] + 2.0 ** -22 * want.abs()
+    assert y.dtype == dtype and bool(torch.isfinite(want).all())
+    assert bool(((y.double() - want).abs() <= room).all())
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 

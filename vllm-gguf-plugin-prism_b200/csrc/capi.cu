@@ -807,7 +807,7 @@ int i8_check(int dtype, int64_t M, int64_t N, int64_t K) {
   return E_OK;
 }
 struct I8MoeLayout {
-  int64_t pass_rows, passes, o_sorted, o_place, o_passes, o_npass, o_units, o_q1, o_s1, o_q2, o_s2, o_h, total;
+  int64_t pass_rows, passes, o_sorted, o_place, o_passes, o_npass, o_q1, o_s1, o_q2, o_s2, o_h, total;
 };
 I8MoeLayout i8_moe_layout(int64_t tokens, int64_t top_k, int64_t E, int64_t H, int64_t I) {
   I8MoeLayout L{};
@@ -820,7 +820,6 @@ I8MoeLayout i8_moe_layout(int64_t tokens, int64_t top_k, int64_t E, int64_t H, i
   L.o_place = take(slots * 4);
   L.o_passes = take(L.passes * 16);
   L.o_npass = take(8);
-  L.o_units = take(2 * E * 4);
   L.o_q1 = take(slots * i8_ld(H));
   L.o_s1 = take(slots * 4);
   L.o_q2 = take(slots * i8_ld(I));
@@ -916,13 +915,10 @@ int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_
   const int64_t slots = tokens * top_k;
   int32_t *sorted = reinterpret_cast<int32_t*>(base + L.o_sorted), *place = reinterpret_cast<int32_t*>(base + L.o_place),
           *npass = reinterpret_cast<int32_t*>(base + L.o_npass);
-  float* units = reinterpret_cast<float*>(base + L.o_units);
   // 1. expert-sorted slots and the passes over them; slots without a valid expert are in none, and the sum skips them
   I8Plan plan{};
   plan.topk_ids = topk_ids; plan.slots = slots; plan.experts = (int)n_experts; plan.pass_rows = (int)L.pass_rows;
-  plan.w2_scale = w2_scales; plan.h = H;
   plan.sorted = sorted; plan.place = place; plan.passes = base + L.o_passes; plan.n_passes = npass;
-  plan.w_unit = units; plan.w_top = units + n_experts;
   rc = launch_i8_plan(plan, s);
   if (rc) return rc;
   // 2. the tokens, quantized, a copy in the place of every slot
@@ -954,23 +950,18 @@ int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_
   q2.scale = reinterpret_cast<float*>(base + L.o_s2);
   rc = launch_i8_quantize(q2, s);
   if (rc) return rc;
-  // 5. down products, back in the order of the slots, divided by powers of two (int8_moe.cu)
-  const float unit = exp2f(ceilf(log2f((float)I)) - 1.f);   // 128 * 127 * I / unit <= 2^15
+  // 5. down products, in fp32, back in the order of the slots
   a.w = static_cast<const int8_t*>(W2); a.ldw = ld2; a.w_scale = w2_scales;
   a.q = q2.q; a.ldq = q2.ldq; a.q_scale = q2.scale;
-  a.dtype = dtype == DT_F32 ? DT_F32 : DT_F16;
   a.ldy = H;
   a.n = H; a.k = I;
   a.act = 0;
   a.sorted = sorted;
-  a.w_unit = units; a.w_top = units + n_experts; a.topk_weights = topk_weights;
-  a.factor = reinterpret_cast<float*>(base + L.o_s1);   // (the tokens' scales are done with)
-  a.unit = 1.f / unit;
   rc = launch_i8_product(a, s);
   if (rc) return rc;
   // 6. weighted sum over the top_k slots of every token
   I8Sum y{};
-  y.y = base + L.o_h; y.out = Y; y.place = place; y.factor = a.factor;
+  y.y = reinterpret_cast<const float*>(base + L.o_h); y.out = Y; y.place = place; y.weights = topk_weights;
   y.tokens = tokens; y.top_k = top_k; y.h = H; y.dtype = dtype;
   return launch_i8_sum(y, s);
 }

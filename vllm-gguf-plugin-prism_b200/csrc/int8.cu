@@ -60,9 +60,6 @@ struct I8Params {
   const int32_t* n_passes;
   int act;
   const int32_t* sorted;
-  const float *w_unit, *w_top, *topk_weights;
-  float* factor;
-  float unit;
   const void* x;           // FEW: [m][ldx], behind the ring the codes of this CTA's K (2 KB a stage)
   int64_t ldx;
   int codes_off, recv_off; // recv_off: room for other CTAs' sums, 0: in the ring
@@ -357,7 +354,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
   const uint32_t accum_s = smem_u32(accum), drained_s = smem_u32(drained);
   auto item = [&](int i, int j, bool waited) { return p.passes ? i8_item<GLU, PAIR>(p, s_list, i, j, (int)rank, waited) : i8_item<GLU, PAIR>(p, i, (int)rank, waited); };
 
-  float ws = 0.f, bias = 0.f, scale = 1.f, unit = 1.f, next_ws = 0.f, next_bias = 0.f;   // epilogue: of this lane's row and (scale, to) this thread's token
+  float ws = 0.f, bias = 0.f, scale = 1.f, next_ws = 0.f, next_bias = 0.f;   // epilogue: of this lane's row and (scale, to) this thread's token
   int to = 0;
   if (warp == 0 || warp == 2 || warp == 3) {
     // ---------------- loaders ----------------
@@ -455,15 +452,15 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     uint32_t aph = 0;
     // this lane's row: of 128, or, gate and up, of 64 gate rows or (lanes with bit 3) their up rows
     const int r = GLU ? quad / 2 + (lane >> 4) * 8 + (lane & 7) : row;
-    const bool down = !GLU && p.passes;   // (left to the sum over the experts: scale of the token, routing weight)
+    const bool down = !GLU && p.passes;
     // What an item's end looks up in memory, a token a thread and a row a lane: asked for while the item before it is on its way out.
     auto older = [](const float* q) { return __int_as_float(ld_older(reinterpret_cast<const int32_t*>(q))); };
+    // (a token's scale is written by the kernel ahead: behind the wait only)
     auto look_up = [&](const I8Item& t, bool waited) {
       const int at = t.x0 + tid, n = t.n0 + r;
       const bool mine = tid < t.rows, live = n < p.n;
-      scale = !FEW && !down && mine ? p.q_scale[at] : 1.f;
+      scale = !FEW && waited && mine ? p.q_scale[at] : 1.f;
       to = !(down && mine) ? at : waited ? p.sorted[at] : ld_older(p.sorted + at);
-      unit = !down ? 1.f : waited ? p.w_unit[t.e] : older(p.w_unit + t.e);
       const float* w = p.w_scale + t.a_row + r + (GLU && (lane & 8) ? p.n : 0);
       next_ws = !live ? 0.f : waited ? *w : older(w);
       next_bias = !GLU && live ? i8_bias(p, n) : 0.f;
@@ -471,6 +468,10 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
     if (down && first < n_items) look_up(item(first, 0, false), false);
     pdl_wait();
     if (!FEW && !down && first < n_items) look_up(item(first, 0, true), true);
+    if (down && first < n_items) {
+      const I8Item t = item(first, 0, true);
+      if (tid < t.rows) scale = p.q_scale[t.x0 + tid];
+    }
     for (int i = first, j = 0; i < n_items; i += step, ++j) {
       const I8Item t = item(i, j, true);
       float* xs = s_scale + (FEW ? 0 : turn * 256);   // (in turn: whoever has passed the last item's barrier is done with those of the item before it)
@@ -489,14 +490,10 @@ __global__ void __launch_bounds__(I8_THREADS, 1) i8_kernel(const __grid_constant
       }
       const int n = t.n0 + r;
       const bool live = n < p.n, wide = wide_y && t.n0 + quad + 32 <= p.n;
-      ws = down ? next_ws * unit * p.unit : next_ws;
+      ws = next_ws;
       bias = next_bias;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * I8_EPI) : "memory");
       if (i + step < n_items) look_up(item(i + step, j + 1, true), true);
-      if (down && t.n0 == 0 && tid < t.rows) {   // (for the sum, while the products are made)
-        const int slot = xr[tid];
-        p.factor[slot] = p.q_scale[t.x0 + tid] * p.topk_weights[slot] * (p.w_top[t.e] / p.unit);
-      }
       mbar_wait_or(accum_s + 8u * buf, aph, gave_up_s);
       __syncwarp();
       tc_fence_after();
@@ -768,11 +765,6 @@ int launch_i8_product(const I8Product& a, cudaStream_t stream) {
   p.n_passes = a.n_passes;
   p.act = a.act;
   p.sorted = a.sorted;
-  p.w_unit = a.w_unit;
-  p.w_top = a.w_top;
-  p.topk_weights = a.topk_weights;
-  p.factor = a.factor;
-  p.unit = a.unit;
   p.x = a.x;
   p.ldx = a.ldx;
   p.status = a.status;

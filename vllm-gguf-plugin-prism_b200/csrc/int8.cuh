@@ -42,12 +42,8 @@ struct I8Product {
   int64_t experts, max_passes, pass_rows;
   // ... gate and up product: w has n gate rows, then n up rows an expert; y[row] = act(gate) * up in fp32, in the order of q's rows
   int act;                   // 1 silu, 2 gelu; 0: down product
-  // ... down product: y[slot] = D * w_scale * w_unit[expert] * unit, slot = sorted[row]; what is left to launch_i8_sum,
-  // factor[slot] = q_scale * topk_weights[slot] * w_top[expert] / unit, is written beside it
+  // ... down product: y[sorted[row]], in fp32
   const int32_t* sorted;
-  const float *w_unit, *w_top, *topk_weights;
-  float* factor;
-  float unit;                // what the products are multiplied by
   // ... tokens that are not quantized yet (null: q is used; see i8_few): [m][ldx] in dtype
   const void* x;
   int64_t ldx;
@@ -63,20 +59,17 @@ struct I8Plan {
   const int32_t* topk_ids;
   int64_t slots;
   int experts, pass_rows;
-  const float* w2_scale;     // [experts][h]
-  int64_t h;
   int32_t* sorted;           // [slots] slots with a valid expert, sorted by it, in their order
   int32_t* place;            // [slots] where in that order a slot is; -1: it has no expert
   void* passes;              // int4 {expert, first row, rows, 0}: an expert's rows in passes of like size, at most pass_rows
   int32_t* n_passes;         // [0] passes, [1] rows
-  float *w_unit, *w_top;     // [experts] a power of two above the expert's largest scale, and its inverse (w_unit)
 };
 int launch_i8_plan(const I8Plan& a, cudaStream_t stream);
 struct I8Sum {
-  const void* y;             // [slots][h], fp16, fp32 where dtype is
+  const float* y;            // [slots][h]
   void* out;                 // [tokens][h] in dtype
   const int32_t* place;      // [slots]; negative: the slot has no result
-  const float* factor;       // [slots]
+  const float* weights;      // [slots]
   int64_t tokens, top_k, h;
   int dtype;
 };

@@ -3,17 +3,15 @@
 //   i8_plan_kernel  slots (token * top_k + j) sorted by expert, in their order; every expert's rows in passes of like size.  One block
 //                   takes up to 1024 slots; of more, a cluster of eight blocks takes equal runs, which learn of one another's counts
 //                   through shared memory.  A warp counts its share of the run and, once the sums over warps, blocks and experts are
-//                   there, places it, 32 slots at a time.  More blocks, one an expert, look for the expert's largest scale.
+//                   there, places it, 32 slots at a time.
 //                   Latencies bound it: 16384 slots of 64 experts 8.4 us behind the kernel ahead, 64 slots 3.1 (10.6 with 16 blocks that
 //                   each counted all slots and summed over their warps for every 1024 of them, and 4.5 with divisions between the sums).
-//   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * factor, in fp32, rounded once.  The down product writes the factors beside its
-//                   results (looked up by the hidden rows' quantizer they cost 2 us for 16384 rows of 1024; by this kernel, 4 us)
+//   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * weight, in fp32, rounded once.
 //
-// The experts' results y = D * w_scale travel from the down product to the sum in fp16 for 16-bit tokens (fp32 for fp32): half the bytes of
-// the step's largest buffer.  They are divided by powers of two first, one above the expert's largest scale and one that brings the
-// largest |D| there can be (128 * 127 * I) to 2^15 at most, so that nothing overflows whatever the scales.  It is one rounding of at most 2^-11
-// of a result, an eighth of the sum's own for bf16, the same as the sum's own for fp16; of results below fp16's normal numbers, at
-// most I * 2^-25 of one unit of D (at the expert's largest scale).
+// The experts' results travel from the down product to the sum in fp32, whatever the tokens' type: the step's largest buffer, 134 MB for 2048 tokens
+// of 2048 columns with eight experts each, written and read again.  (In fp16, with powers of two taken out, the same step took 200 us instead of
+// 224, but an fp16 result was off by 2.9e-4 instead of 2.0e-4, and rows of W2 whose scale is far below the expert's largest lost their bits.
+// The product and the sum in two halves of the columns, so that the buffer stays in L2: 226.)
 #include <math.h>
 
 #include "common.cuh"
@@ -33,38 +31,13 @@ __global__ void __launch_bounds__(1024, 1) i8_plan_kernel(const I8Plan p, int bl
   __shared__ int32_t s_cnt[32][I8_MAX_EXPERTS + 1];   // a warp's slots of an expert; then where its next one goes, from the block's first
   __shared__ int32_t s_run[I8_MAX_EXPERTS], s_total[I8_MAX_EXPERTS], s_next[I8_MAX_EXPERTS];   // the block's slots, all, the block's first place
   __shared__ int32_t s_size[I8_MAX_EXPERTS], s_passes[I8_MAX_EXPERTS], s_order[I8_MAX_EXPERTS], s_pass[I8_MAX_EXPERTS];   // block 0: passes
-  __shared__ float s_top[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.experts, slots = (int)p.slots;
   // One block for all slots has one for every thread.
-  const bool alone = blocks == 1, counts = (int)blockIdx.x < blocks;
+  const bool alone = blocks == 1;
   const int warps = alone ? ((slots + 31) / 32 + 7) / 8 * 8 : 32;
-  if (counts)
-    for (int i = threadIdx.x; i < warps * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < warps * (I8_MAX_EXPERTS + 1); i += 1024) (&s_cnt[0][0])[i] = 0;
   pdl_wait();
   pdl_trigger();
-  if (!counts) {   // largest scale of an expert (a scale that is not finite: as if it were not there)
-    const int e = blockIdx.x - blocks;
-    if (e >= E) return;
-    float top = 0.f;
-    for (int64_t i = threadIdx.x; i < p.h; i += 1024) {
-      const float v = fabsf(p.w2_scale[e * p.h + i]);
-      if (v <= 3.402823466e+38f) top = fmaxf(top, v);
-    }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-    if (warp == 0) {
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s_top[lane])));
-      if (lane == 0) {
-        int x = 0;
-        frexpf(top, &x);
-        x = max(-126, min(127, x));
-        p.w_top[e] = exp2f((float)x);
-        p.w_unit[e] = exp2f((float)-x);
-      }
-    }
-    return;
-  }
   // A warp's slots: a 32nd of the block's, in their order, 32 at a time
   const int own = run / 32, s0 = min(slots, (int)blockIdx.x * run + warp * own), s1 = min(slots, s0 + own);
   // Lanes with this one's expert, and how many of them are below it
@@ -220,63 +193,56 @@ int64_t i8_moe_passes(int64_t slots, int64_t experts, int64_t pass_rows) {
 int launch_i8_plan(const I8Plan& a, cudaStream_t stream) {
   if (a.experts < 1 || a.experts > I8_MAX_EXPERTS || a.slots > 1 << 24) return E_BAD_SHAPE;
   const int blocks = a.slots <= 1024 ? 1 : I8_PLAN_BLOCKS, run = (int)((a.slots + blocks - 1) / blocks + 1023) / 1024 * 1024;
-  const dim3 grid((unsigned)round_up(blocks + a.experts, blocks));
-  return launch_pdl_cluster(i8_plan_kernel, grid, dim3(1024), (unsigned)blocks, 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
+  return launch_pdl_cluster(i8_plan_kernel, dim3((unsigned)blocks), dim3(1024), (unsigned)blocks, 0, stream, a, blocks, run) == cudaSuccess ? E_OK : E_CUDA;
 }
 
-// Eight columns a thread, ROWS experts' rows in flight: four of fp32, eight of fp16, four of fp16 where a token has no more experts (150 blocks of
-// 1536 columns 3.0 us and 3.5).  2048 tokens of 2048 columns, eight experts, from L2 and memory: 16.5 us (19.2 when a row was asked for only
-// once its place was known).
-template <typename Y, typename T, int ROWS> __global__ void __launch_bounds__(128) i8_sum_kernel(const I8Sum p) {
+// Four columns a thread, ROWS experts' rows in flight: of eight tokens 1 us less than eight columns and four rows, of 2048 tokens 2 us less.
+template <typename T, int ROWS> __global__ void __launch_bounds__(128) i8_sum_kernel(const I8Sum p) {
   pdl_wait();
   pdl_trigger();
-  constexpr int WI = sizeof(Y) / 2, WO = sizeof(T) / 2;   // 16-byte words of eight values
-  const unsigned per_row = (unsigned)(p.h / 8), top_k = (unsigned)p.top_k;
-  const unsigned i = blockIdx.x * 128 + threadIdx.x;
-  if (i >= (unsigned)p.tokens * per_row) return;
-  const unsigned t = i / per_row, c = 8 * (i - t * per_row), slot0 = t * top_k;
-  const Y* in = static_cast<const Y*>(p.y) + (int64_t)slot0 * p.h + c;
-  float s[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) s[k] = 0.f;
+  const unsigned per_row = (unsigned)(p.h / 4), top_k = (unsigned)p.top_k;
+  const uint64_t at = (uint64_t)blockIdx.x * 128 + threadIdx.x;
+  if (at >= (uint64_t)p.tokens * per_row) return;
+  const unsigned i = (unsigned)at, t = i / per_row, c = 4 * (i - t * per_row), slot0 = t * top_k;   // (fewer than 2^32)
+  const float* in = p.y + (int64_t)slot0 * p.h + c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   for (unsigned j0 = 0; j0 < top_k; j0 += ROWS, in += ROWS * p.h) {
-    uint4 v[ROWS][WI];
+    float4 v[ROWS];
     float f[ROWS];
 #pragma unroll
     for (unsigned j = 0; j < ROWS; ++j)   // (a row that nothing was written to is read as well, and left out below: none waits for its place)
-#pragma unroll
-      for (int k = 0; k < WI; ++k) v[j][k] = j0 + j < top_k ? reinterpret_cast<const uint4*>(in + j * p.h)[k] : make_uint4(0, 0, 0, 0);
+      v[j] = j0 + j < top_k ? __ldcs(reinterpret_cast<const float4*>(in + j * p.h)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (unsigned j = 0; j < ROWS; ++j) {
       const bool live = j0 + j < top_k && __ldg(p.place + slot0 + j0 + j) >= 0;   // (a slot without a valid expert contributes nothing)
-      f[j] = j0 + j < top_k ? __ldg(p.factor + slot0 + j0 + j) : 0.f;
-      if (!live) {
-        f[j] = 0.f;
-#pragma unroll
-        for (int k = 0; k < WI; ++k) v[j][k] = make_uint4(0, 0, 0, 0);
-      }
+      f[j] = live ? __ldg(p.weights + slot0 + j0 + j) : 0.f;
+      if (!live) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = fmaf(to_float<Y>(reinterpret_cast<const Y*>(v[j])[k]), f[j], s[k]);
+      for (int k = 0; k < 4; ++k) s[k] = fmaf(reinterpret_cast<const float*>(&v[j])[k], f[j], s[k]);
   }
-  uint4 o[WO];
+  alignas(16) T o[4];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(o)[k] = from_float<T>(s[k]);
-#pragma unroll
-  for (int k = 0; k < WO; ++k) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)t * p.h + c)[k] = o[k];
+  for (int k = 0; k < 4; ++k) o[k] = from_float<T>(s[k]);
+  T* out = static_cast<T*>(p.out) + (int64_t)t * p.h + c;
+  if (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+  else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
 }
 
+template <typename T> static cudaError_t i8_sum_typed(const I8Sum& a, dim3 grid, cudaStream_t stream) {
+  return a.top_k <= 4 ? launch_pdl(i8_sum_kernel<T, 4>, grid, dim3(128), 0, stream, a) : launch_pdl(i8_sum_kernel<T, 8>, grid, dim3(128), 0, stream, a);
+}
 int launch_i8_sum(const I8Sum& a, cudaStream_t stream) {
-  const int64_t total = a.tokens * (a.h / 8);
-  if (a.h % 8 != 0 || total >= (int64_t)1 << 31) return E_TOO_LARGE;
+  const int64_t total = a.tokens * (a.h / 4);
+  if (a.h % 8 != 0 || total >= (int64_t)1 << 32) return E_TOO_LARGE;
   const dim3 grid((unsigned)((total + 127) / 128));
   cudaError_t e;
   switch (a.dtype) {
-    case DT_F32: e = launch_pdl(i8_sum_kernel<float, float, 4>, grid, dim3(128), 0, stream, a); break;
-    case DT_F16: e = a.top_k <= 4 ? launch_pdl(i8_sum_kernel<__half, __half, 4>, grid, dim3(128), 0, stream, a) : launch_pdl(i8_sum_kernel<__half, __half, 8>, grid, dim3(128), 0, stream, a); break;
-    case DT_BF16: e = a.top_k <= 4 ? launch_pdl(i8_sum_kernel<__half, __nv_bfloat16, 4>, grid, dim3(128), 0, stream, a) : launch_pdl(i8_sum_kernel<__half, __nv_bfloat16, 8>, grid, dim3(128), 0, stream, a); break;
+    case DT_F32: e = i8_sum_typed<float>(a, grid, stream); break;
+    case DT_F16: e = i8_sum_typed<__half>(a, grid, stream); break;
+    case DT_BF16: e = i8_sum_typed<__nv_bfloat16>(a, grid, stream); break;
     default: return E_BAD_DTYPE;
   }
   return e == cudaSuccess ? E_OK : E_CUDA;
