@@ -381,6 +381,53 @@ def test_moe_of_16_bit_tokens_sums_in_fp32(ops, t, e, k, h, i, dtype):
     assert bool(((y.double() - want).abs() <= room).all())
 
 
+def rows_of_gates(act, lo, hi, t, i, gen):
+    """(x, w13, s13) of two experts whose gates all lie between lo and hi, within 5 %, up halves of both signs."""
+    h = 96
+    x = 1 + 0.05 * torch.rand(t, h, device="cuda", generator=gen)
+    w13, s13 = weights(2 * 2 * i, h, gen)
+    w13, s13 = w13.unflatten(0, (2, 2 * i)), s13.view(2, 2 * i)
+    w13[:, :i] = -(w13[:, :i].abs().clamp(min=1).clamp(max=127))
+    q, qs = codes_of(x)
+    mean = (q[0] @ w13[:, :i].double().transpose(1, 2)) * qs[0]
+    s13[:, :i] = (torch.linspace(hi, lo, i, device="cuda", dtype=torch.float64) / mean).float()
+    return x, w13, s13
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,lo,hi", [("gelu", -8.0, -3.0), ("gelu", -12.5, -6.0), ("gelu", -2.0, -0.01)])
+@pytest.mark.parametrize("t,i", [(3, 64), (70, 136)])
+def test_moe_hidden_rows_of_negative_gates(ops, act, lo, hi, t, i):
+    """A hidden row goes by its own largest value, so that it needs small activations to be right relative to themselves.
+
+    A gate is D * (q_scale * w_scale) with D below 2^24: the scale, two products, 3 * 2^-24.  What that is in the activation's value is its condition
+    number, below 1 + g^2 for g Phi(g) (g phi(g) / Phi(g) is below 1 + g^2 for negative g) and below 1 + |g| for g sigmoid(g).  The activation adds
+    2^-20 (of an erfc 2^-21, of an exponential and a reciprocal 2^-23 each, and a few roundings of 2^-24), up and its product 4 * 2^-24."""
+    gen = torch.Generator(device="cuda").manual_seed(t + i)
+    x, w13, s13 = rows_of_gates(act, lo, hi, t, i, gen)
+    w2, s2 = weights(2 * 96, i, gen)
+    w2, s2 = w2.unflatten(0, (2, 96)), s2.view(2, 96)
+    s2 *= 1e3 / max(1e-30, float(torch.sigmoid(torch.tensor(hi, dtype=torch.float64))))   # (results of ordinary size)
+    ids = (torch.arange(t, device="cuda") % 2).to(torch.int32)[:, None].contiguous()
+    y = ops.int8_fused_moe(x, w13, s13, w2, s2, torch.ones(t, 1, device="cuda"), ids, act)
+    q, qs = codes_of(x)
+    for e in range(2):
+        s = ids[:, 0] == e
+        both = (q[s] @ w13[e].double().T) * qs[s][:, None] * s13[e].double()
+        g, up = both[:, :i], both[:, i:]
+        assert bool((g < 0.9 * hi).all()) and bool((g > 1.1 * lo).all())
+        h = (g * torch.sigmoid(g) if act == "silu" else g * torch.special.ndtr(g)) * up
+        rel = (1 + (g * g if act == "gelu" else g.abs())) * 3 * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22
+        a, top = h.abs().max(1, keepdim=True)
+        unit = h * 127 / a
+        close = ((unit - torch.floor(unit) - 0.5).abs() < unit.abs() * (rel + rel.gather(1, top)) + 2.0 ** -30).double()
+        f = (a / 127) * s2[e].double()
+        want = (torch.round(unit) @ w2[e].double().T) * f
+        room = (close @ w2[e].double().abs().T) * f + want.abs() * (rel.gather(1, top) + 8 * 2.0 ** -24)
+        off = (y[s].double() - want).abs()
+        assert bool((off <= room).all()), (float((off / want.abs().amax()).max()), float((room / want.abs().amax()).max()))
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 

@@ -152,7 +152,13 @@ __device__ __forceinline__ float i8_silu(float g) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
   return g * r;
 }
-__device__ __forceinline__ float i8_gelu(float g) { return 0.5f * g * (1.f + erff(g * 0.70710678f)); }
+// g Phi(g) = g / 2 erfc(-g / sqrt 2): relative to itself to 2^-20 for gates of both signs (1 + erf would cancel: nothing is left of it at -6).  What
+// -g / sqrt 2 lost is put back by the derivative, erfc(x + d) = erfc(x) (1 - 2 x d) for x > 0 up to a few 2^-24: at -8 it would be 64 roundings.
+__device__ __forceinline__ float i8_gelu(float g) {
+  constexpr float HI = 0.70710678f, LO = 1.2101617e-8f;   // 1 / sqrt 2 in two parts
+  const float x = -g * HI, lost = fmaf(-g, LO, fmaf(-g, HI, -x)), y = 0.5f * g * erfcf(x);
+  return x > 0.f ? fmaf(y * -2.f * x, lost, y) : y;
+}
 __device__ __forceinline__ float i8_bias(const I8Params& p, int n) {
   if (!p.bias) return 0.f;
   return p.dtype == DT_F32 ? static_cast<const float*>(p.bias)[n]
