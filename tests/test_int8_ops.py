@@ -428,6 +428,38 @@ def test_moe_hidden_rows_of_negative_gates(ops, act, lo, hi, t, i):
         assert bool((off <= room).all()), (float((off / want.abs().amax()).max()), float((room / want.abs().amax()).max()))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,sign,size", [("silu", -1, 2.0 ** -13), ("silu", -1, 2.0 ** -16), ("silu", 1, 2.0 ** -14), ("gelu", -1, 2.0 ** -16), ("gelu", 1, 2.0 ** -16)])
+def test_moe_activation_of_exact_gates(ops, act, sign, size):
+    """Scales that are powers of two and sums below 2^24: gates (of a size up to 75, 10 or 38) and up halves reach the activation without a rounding.
+    What is left is the activation's 2^-21 (silu: an exponential and a reciprocal to 2^-23 each, three roundings of 2^-24) or 2^-20 (gelu), up's product, the
+    row's scale a / 127, and four roundings of the down product, 2^-24 each."""
+    gen = torch.Generator(device="cuda").manual_seed(int(1 / size) + sign)
+    t, h, i = 40, 96, 72
+    x = torch.randint(60, 128, (t, h), device="cuda", generator=gen).float()
+    x[:, 5] = 127                                              # (codes are the values, the scale is 1)
+    buf = torch.randint(-127, 128, (1, 2 * i, h), device="cuda", generator=gen)
+    big = 30 + torch.arange(i, device="cuda")[:, None] // 2    # (gate rows of different sizes)
+    buf[0, :i] = sign * (big - torch.randint(0, 10, (i, h), device="cuda", generator=gen))
+    w13, s13 = buf.to(torch.int8), torch.full((1, 2 * i), size, device="cuda")
+    w2 = torch.randint(-127, 128, (1, 64 + 32, 80), device="cuda", generator=gen).to(torch.int8)[:, :, :i]
+    s2 = torch.full((1, h), 2.0 ** 20, device="cuda")
+    y = ops.int8_fused_moe(x, w13, s13, w2, s2, torch.ones(t, 1, device="cuda"), torch.zeros(t, 1, dtype=torch.int32, device="cuda"), act)
+    both = (x.double() @ w13[0].double().T) * size
+    g, up = both[:, :i], both[:, i:]
+    assert float(g.abs().max()) < 76 and bool((g.abs() > 0.1).all())
+    hidden = (g * torch.sigmoid(g) if act == "silu" else g * torch.special.ndtr(g)) * up
+    rel = 2.0 ** (-21 if act == "silu" else -20) + 2.0 ** -24
+    a = hidden.abs().amax(1, keepdim=True)
+    unit = hidden * 127 / a
+    close = ((unit - torch.floor(unit) - 0.5).abs() < 127 * 2 * rel).double()
+    f = a / 127 * 2.0 ** 20
+    want = (torch.round(unit) @ w2[0].double().T) * f
+    room = (close @ w2[0].double().abs().T) * f + want.abs() * (rel + 5 * 2.0 ** -24)
+    off = (y.double() - want).abs()
+    assert bool((off <= room).all()), (float((off / want.abs().amax()).max()), float((room / want.abs().amax()).max()))
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 
