@@ -140,6 +140,31 @@ def test_route_runs_of_equals(ops, scoring, with_bias, e, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [1, 4, 7])
+def test_route_experts_far_below_the_best(ops, scoring, k):
+    """A bias that keeps the row's best experts out: what is chosen lies 20 to 200 below them, and its weights still add up to one."""
+    e = 32
+    rows = []
+    for top, drop, step in ((0.0, 20.0, 1.0), (0.0, 69.0, 1.0), (0.0, 80.0, 1.0), (5.0, 95.0, 0.5), (0.0, 110.0, 3.0), (-70.0, 20.0, 0.25), (-100.0, 90.0, 1.0), (0.0, 200.0, 10.0)):
+        row = top - drop - step * torch.arange(e, dtype=torch.float32)
+        row[0] = top
+        rows += [row, row.flip(0), torch.where(torch.arange(e) % 5 == 4, -INF, row)]
+    logits = torch.stack(rows)
+    for value in (-INF, -2.0):
+        bias = torch.zeros(e)
+        bias[0] = bias[e - 1] = value
+        for groups, topk_group in ((1, 1), (4, 2)):
+            if groups > 1:
+                bias[:8] -= 3.0                               # (the best expert's group is out)
+            kw = dict(scoring=scoring, n_group=groups, topk_group=topk_group)
+            got = ops.moe_route(logits.cuda(), k, bias=bias.cuda(), **kw)
+            check(got, route(logits, k, bias=bias, **kw))
+            assert bool(((got[0].double().sum(1) - 1).abs() < 2.0 ** -20).all())
+            check(ops.moe_route(logits.cuda(), k, bias=bias.cuda(), renormalize=False, **kw), route(logits, k, bias=bias, renormalize=False, **kw), scoring == "softmax")
+
+
+@pytest.mark.gpu
 def test_route_strides_streams_and_empty(ops):
     gen = torch.Generator(device="cuda").manual_seed(8)
     big = torch.randn(30, 201, device="cuda", generator=gen)

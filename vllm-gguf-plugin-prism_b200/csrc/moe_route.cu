@@ -329,10 +329,10 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
     }
     if (p.renormalize) {
       const float sum = warp_sum(w);
-      if (sum >= 1e-30f) {
+      if (sum >= 0x1p-20f) {
         w = w / sum;
-      } else {   // (sigmoids of logits around -70 and less)
-        const double d = id >= 0 && p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : 0.0, all = warp_sum(d);
+      } else {   // (sigmoids of logits around -14 and less; a softmax with a bias that chose experts so far below the row's largest: scores may leave fp32's range)
+        const double d = id < 0 ? 0.0 : p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)high), all = warp_sum(d);
         w = all > 0.0 ? (float)(d / all) : 0.f;
       }
     }
