@@ -165,6 +165,23 @@ def test_route_experts_far_below_the_best(ops, scoring, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups,topk_group", [(64, 8, 4), (256, 8, 3), (60, 4, 1), (512, 32, 7)])
+@pytest.mark.parametrize("size", [1.0, 100.0, 1e5])
+def test_route_groups_of_choices_that_cancel(ops, scoring, e, groups, topk_group, size):
+    """A bias of both signs: a group's two best choices are large and their sum is small, so that what they were rounded by is more than what is between groups."""
+    gen = torch.Generator().manual_seed(e + groups)
+    logits = torch.randn(200, e, generator=gen) * torch.tensor([1.0, 0.1, 0.01, 0.001]).repeat(50)[:, None]
+    per = e // groups
+    bias = torch.full((e,), -size)
+    bias[1::per] = size
+    bias[per // 2:2 * per:per] -= size / 2                    # (groups that are plainly out, or in)
+    bias[3 * per:4 * per] -= 1e9 if size == 1.0 else 0.0
+    kw = dict(scoring=scoring, n_group=groups, topk_group=topk_group)
+    check(ops.moe_route(logits.cuda(), 4, bias=bias.cuda(), **kw), route(logits, 4, bias=bias, **kw))
+
+
+@pytest.mark.gpu
 def test_route_strides_streams_and_empty(ops):
     gen = torch.Generator(device="cuda").manual_seed(8)
     big = torch.randn(30, 201, device="cuda", generator=gen)

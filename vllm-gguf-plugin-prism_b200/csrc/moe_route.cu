@@ -71,24 +71,27 @@ __device__ __forceinline__ float route_rcp(float x) {
 // Whether a choice `a` is above another, `b`, for certain.  off: what two scores can be off by together.  e^x above is off by (|x| + 2) 2^-23 of
 // itself; a sigmoid by s (1 - s) times that, at most 2^-23, and 2^-24 + 2^-23 for the sum and the reciprocal: two of them by less than 2^-20.
 // A softmax' sum of up to 512 terms adds 21 roundings of 2^-24: two by less than 2^-18.  The sum with the bias is rounded by 2^-24 of
-// itself, and a key leaves out less than V 2^-23 of it; a sum of two choices is off by twice all that.  (NaN: not certain.)
-template <int V> __device__ __forceinline__ bool route_above(float a, float b, float off) {
-  return a - b > off * (1.f + (float)(V + 1) * 0x1p-3f * (fabsf(a) + fabsf(b)));   // ((V + 1) 2^-23 (|a| + |b|), off being 2^-20 at least)
+// itself, and a key leaves out less than V 2^-23 of it.  size: what has been rounded so, |a| + |b|.  (NaN: not certain.)
+template <int V> __device__ __forceinline__ bool route_above(float a, float b, float off, float size) {
+  return a - b > off * (1.f + (float)(V + 1) * 0x1p-3f * size);   // ((V + 1) 2^-23 size, off being 2^-20 at least)
 }
+template <int V> __device__ __forceinline__ bool route_above(float a, float b, float off) { return route_above<V>(a, b, off, fabsf(a) + fabsf(b)); }
 
 // The groups that remain, a bit each.  sure: false where the order of two groups that decides is not certain.
 template <typename Key, int V, bool SCORES>
 __device__ __forceinline__ uint32_t route_groups(const RouteParams& p, const Key (&key)[V], int lane, float off, bool& sure) {
-  Key mine = 0;   // lane g: score of group g
+  Key first = 0, second = 0;   // lane g: the two best choices of group g
   auto close = [&](int g, Key a, Key b) {   // a, b: this lane's two best of group g
     const Key best = warp_max(a);
-    Key score = best;
+    Key next = 0;
     if constexpr (SCORES) {
       const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
-      const Key second = warp_max(lane == owner ? b : a);
-      if (!route_out(second)) score = route_key(route_value(best) + route_value(second));
+      next = warp_max(lane == owner ? b : a);
     }
-    if (lane == g) mine = route_out(best) ? 0 : score;
+    if (lane == g) {
+      first = best;
+      second = next;
+    }
   };
   if (p.per % 32 == 0) {   // a group is whole registers
     const int n = p.per / 32;
@@ -118,6 +121,10 @@ __device__ __forceinline__ uint32_t route_groups(const RouteParams& p, const Key
       close(g, a, b);
     }
   }
+  // Lane g: score of group g, and what its error goes by, |best| + |second|, of which little may be left in their sum
+  const bool two = SCORES && !route_out(second);
+  Key mine = route_out(first) ? Key(0) : two ? route_key(route_value(first) + route_value(second)) : first;
+  const float size = fabsf((float)route_value(first)) + (two ? fabsf((float)route_value(second)) : 0.f);
   // (a group without an expert is picked when nothing else is left, which changes nothing)
   uint32_t taken = 0;
   Key last = 0;
@@ -128,9 +135,12 @@ __device__ __forceinline__ uint32_t route_groups(const RouteParams& p, const Key
     taken |= 1u << g;
     if (lane == g) mine = 0;
   }
-  if constexpr (sizeof(Key) == 4) {
+  if constexpr (sizeof(Key) == 4 && SCORES) {   // every group that is left against the last one taken, as if that were off by as much as the one of the largest size
+    const float most = __uint_as_float(warp_max(taken >> lane & 1u ? __float_as_uint(size) : 0u));
+    sure = __all_sync(0xffffffffu, mine == 0 || route_above<V>(route_value(last), route_value(mine), 2.f * off, most + size));
+  } else if constexpr (sizeof(Key) == 4) {
     const Key next = warp_max(mine);
-    sure = next == 0 || (SCORES ? route_above<V>(route_value(last), route_value(next), 2.f * off) : (last / V) > (next / V));   // (equal up to the index)
+    sure = next == 0 || (last / V) > (next / V);   // (equal up to the index)
   }
   return taken;
 }
