@@ -498,6 +498,38 @@ def test_c_abi_refuses_before_any_launch(native_libs):
     assert call(ws=room - 1) == -5 and call(top_k=257) == -7
 
 
+def test_c_abi_refuses_pointers_off_their_elements(native_libs):
+    """Every argument that a kernel reads or writes by its elements, one at a time, and a negative distance between rows."""
+    from gguf_b200 import capi
+
+    lib = capi.lib()
+    p, off1, off2 = ctypes.c_void_p(4096), ctypes.c_void_p(4097), ctypes.c_void_p(4098)
+    q = lib.gguf_b200_int8_quantize
+    assert q(p, 1, 64, p, 64, off2, 1, 64, None) == -4
+
+    def mul_mat(w_scales=p, bias=p, dtype=1, m=1, ldx=64):
+        return lib.gguf_b200_int8_mul_mat(p, 64, w_scales, p, ldx, bias, p, p, 1 << 20, 0, dtype, m, 8, 64, None)
+
+    def prepared(w_scales=p, q_scales=p, bias=p, dtype=1):
+        return lib.gguf_b200_int8_mul_mat_prepared(p, 64, w_scales, p, 64, q_scales, bias, p, 0, dtype, 1, 8, 64, None)
+
+    for m in (1, 40):
+        assert mul_mat(w_scales=off2, m=m) == -4 and mul_mat(bias=off1, m=m) == -4 and mul_mat(bias=off1, dtype=2, m=m) == -4 and mul_mat(bias=off2, dtype=0, m=m) == -4
+        assert mul_mat(ldx=-64, m=m) == -3
+    assert prepared(w_scales=off2) == -4 and prepared(q_scales=off2) == -4 and prepared(bias=off1) == -4 and prepared(bias=off2, dtype=0) == -4
+    room = lib.gguf_b200_int8_moe_workspace_bytes(4, 2, 8, 64, 64)
+
+    def moe(ldx=64, s13=p, s2=p, ids=p, weights=p):
+        return lib.gguf_b200_int8_fused_moe(p, ldx, p, 64, s13, p, 64, s2, p, ids, weights, p, room, 1, 1, 4, 2, 8, 64, 64, None)
+
+    assert moe(ldx=-1) == -3 and moe(s13=off2) == -4 and moe(s2=off2) == -4 and moe(ids=off2) == -4 and moe(weights=off2) == -4
+
+    def route(bias=None, weights=p, ids=p):
+        return lib.gguf_b200_moe_route(p, 1, 64, bias, weights, ids, 4, 64, 8, 1, 1, 1, 1, 1.0, None)
+
+    assert route(bias=off2) == -4 and route(weights=off2) == -4 and route(ids=off2) == -4
+
+
 def test_shapes_under_tracing(ops):
     from torch._subclasses.fake_tensor import FakeTensorMode
 

@@ -800,6 +800,7 @@ int64_t i8_ld(int64_t k) { return round_up(k, 16); }
 // rows of a matrix of 8-bit integers: where the tensor core's copies can start
 bool i8_rows_ok(const void* p, int64_t ld, int64_t k) { return p && aligned16(p) && ld >= k && ld % 16 == 0; }
 bool element_aligned(const void* p, int dtype) { return p && reinterpret_cast<uintptr_t>(p) % (dtype == DT_F32 ? 4 : 2) == 0; }
+bool word_aligned(const void* p) { return p && reinterpret_cast<uintptr_t>(p) % 4 == 0; }   // of float, int32_t
 int i8_check(int dtype, int64_t M, int64_t N, int64_t K) {
   if (!dtype_ok(dtype)) return E_BAD_DTYPE;
   if (M < 0 || N < 0 || K <= 0) return E_BAD_SHAPE;
@@ -835,7 +836,7 @@ int gguf_b200_int8_quantize(const void* X, int dtype, int64_t ldx, void* Q, int6
   if (M < 0 || K <= 0 || ldx < 0) return E_BAD_SHAPE;
   if (M >= (int64_t)1 << 31 || K >= (int64_t)1 << 31) return E_TOO_LARGE;
   if (M == 0) return E_OK;
-  if (!element_aligned(X, dtype) || !scales || !i8_rows_ok(Q, ldq, K)) return E_BAD_POINTER;
+  if (!element_aligned(X, dtype) || !word_aligned(scales) || !i8_rows_ok(Q, ldq, K)) return E_BAD_POINTER;
   I8Quantize a{};
   a.x = X; a.dtype = dtype; a.ldx = ldx;
   a.q = static_cast<int8_t*>(Q); a.ldq = ldq; a.scale = scales;
@@ -849,7 +850,8 @@ int gguf_b200_int8_mul_mat_prepared(const void* W, int64_t ldw, const float* w_s
                                     void* Y, int flags, int dtype, int64_t M, int64_t N, int64_t K, void* stream) {
   const int rc = i8_check(dtype, M, N, K);
   if (rc || M == 0 || N == 0) return rc;
-  if (!i8_rows_ok(W, ldw, K) || !i8_rows_ok(Q, ldq, K) || !w_scales || !q_scales || !element_aligned(Y, dtype)) return E_BAD_POINTER;
+  if (!i8_rows_ok(W, ldw, K) || !i8_rows_ok(Q, ldq, K) || !word_aligned(w_scales) || !word_aligned(q_scales) || !element_aligned(Y, dtype)) return E_BAD_POINTER;
+  if (bias && !element_aligned(bias, dtype)) return E_BAD_POINTER;
   int* st = status_ptr();
   if (!st) return E_CUDA;
   I8Product a{};
@@ -868,7 +870,8 @@ int gguf_b200_int8_mul_mat(const void* W, int64_t ldw, const float* w_scales, co
   int rc = i8_check(dtype, M, N, K);
   if (rc || M == 0 || N == 0) return rc;
   if (ldx < 0) return E_BAD_SHAPE;
-  if (!element_aligned(X, dtype) || !element_aligned(Y, dtype) || !i8_rows_ok(W, ldw, K) || !w_scales || !ws || !aligned16(ws)) return E_BAD_POINTER;
+  if (!element_aligned(X, dtype) || !element_aligned(Y, dtype) || !i8_rows_ok(W, ldw, K) || !word_aligned(w_scales) || !ws || !aligned16(ws)) return E_BAD_POINTER;
+  if (bias && !element_aligned(bias, dtype)) return E_BAD_POINTER;
   if (ws_bytes < gguf_b200_int8_scratch_bytes(M, K)) return E_WORKSPACE;
   if (i8_few(X, dtype, ldx, M, N, K)) {
     int* st = status_ptr();
@@ -897,14 +900,14 @@ int64_t gguf_b200_int8_moe_workspace_bytes(int64_t tokens, int64_t top_k, int64_
 int gguf_b200_int8_fused_moe(const void* X, int64_t ldx, const void* W13, int64_t ld13, const float* w13_scales, const void* W2, int64_t ld2,
                              const float* w2_scales, void* Y, const int32_t* topk_ids, const float* topk_weights, void* ws, int64_t ws_bytes, int dtype,
                              int act, int64_t tokens, int64_t top_k, int64_t n_experts, int64_t H, int64_t I, void* stream) {
-  if (top_k <= 0 || n_experts <= 0 || I <= 0 || H <= 0 || H % 8 != 0 || I % 8 != 0 || (act != 1 && act != 2)) return E_BAD_SHAPE;
+  if (ldx < 0 || top_k <= 0 || n_experts <= 0 || I <= 0 || H <= 0 || H % 8 != 0 || I % 8 != 0 || (act != 1 && act != 2)) return E_BAD_SHAPE;
   if (n_experts > 256 || top_k > 256 || H > I8_MAX_K || I > I8_MAX_K || tokens > 1 << 24 || tokens * top_k > 1 << 24 || tokens * (H / 8) >= (int64_t)1 << 31)
     return E_TOO_LARGE;
   int rc = i8_check(dtype, tokens, n_experts * 2 * I, H);
   if (!rc) rc = i8_check(dtype, tokens, n_experts * H, I);
   if (rc || tokens == 0) return rc;
-  if (!element_aligned(X, dtype) || !Y || !aligned16(Y) || !i8_rows_ok(W13, ld13, H) || !i8_rows_ok(W2, ld2, I) || !w13_scales || !w2_scales || !topk_ids || !topk_weights || !ws ||
-      !aligned16(ws))
+  if (!element_aligned(X, dtype) || !Y || !aligned16(Y) || !i8_rows_ok(W13, ld13, H) || !i8_rows_ok(W2, ld2, I) || !word_aligned(w13_scales) || !word_aligned(w2_scales) ||
+      !word_aligned(topk_ids) || !word_aligned(topk_weights) || !ws || !aligned16(ws))
     return E_BAD_POINTER;
   const I8MoeLayout L = i8_moe_layout(tokens, top_k, n_experts, H, I);
   if (ws_bytes < L.total) return E_WORKSPACE;
@@ -973,7 +976,7 @@ int gguf_b200_moe_route(const void* logits, int dtype, int64_t ld, const float* 
   if (n_experts > ROUTE_MAX_EXPERTS || top_k > ROUTE_MAX_TOP_K || n_group > 32 || tokens >= (int64_t)1 << 31) return E_TOO_LARGE;
   if (n_experts % n_group != 0 || topk_group > n_group || top_k > topk_group * (n_experts / n_group)) return E_BAD_SHAPE;
   if (tokens == 0) return E_OK;
-  if (!element_aligned(logits, dtype) || !weights || !ids) return E_BAD_POINTER;
+  if (!element_aligned(logits, dtype) || !word_aligned(weights) || !word_aligned(ids) || (bias && !word_aligned(bias))) return E_BAD_POINTER;
   return launch_moe_route(logits, dtype, ld, bias, weights, ids, tokens, (int)n_experts, (int)top_k, (int)n_group, (int)topk_group, scoring == 2, renormalize,
                           scale, static_cast<cudaStream_t>(stream));
 }
