@@ -149,6 +149,25 @@ def test_route_reads_the_layer(monkeypatch, native_libs):
     assert (seen["n_group"], seen["topk_group"]) == (8, 4)
 
 
+@pytest.mark.parametrize("name,value", [("custom_routing_function", lambda *a: None), ("enable_eplb", True)])
+def test_route_refuses_a_layer_that_routes_otherwise(monkeypatch, native_libs, name, value):
+    from vllm_gguf_plugin import ops
+    from vllm_gguf_plugin.quantization import GGUFMoEMethod
+
+    calls = []
+    monkeypatch.setattr(ops, "moe_route", lambda logits, top_k, **kw: calls.append(kw))
+    layer = torch.nn.Module()
+    layer.top_k = 3
+    setattr(layer, name, value)
+    for call in (lambda: GGUFMoEMethod.route(layer, None), lambda: GGUFMoEMethod(None).apply_logits(layer, None, None)):
+        with pytest.raises(NotImplementedError, match=name):
+            call()
+    assert not calls
+    setattr(layer, name, None if name == "custom_routing_function" else False)
+    GGUFMoEMethod.route(layer, None)
+    assert len(calls) == 1
+
+
 def test_rows_of_an_unknown_type_are_refused(native_libs):
     from vllm_gguf_plugin.quantization import int8_rows
 

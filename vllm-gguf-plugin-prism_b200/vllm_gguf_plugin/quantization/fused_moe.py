@@ -225,7 +225,11 @@ class GGUFMoEMethod(FusedMoEMethodBase):
     def route(layer, router_logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(topk_weights, topk_ids) of the router's logits ``[tokens, experts]``, by what vLLM's MoE layers say about it: ``top_k``,
         ``renormalize``, ``scoring_func``, ``e_score_correction_bias``, ``use_grouped_topk`` with ``num_expert_group`` and ``topk_group``,
-        ``routed_scaling_factor``.  (The serving engine does this for the reference's method.)"""
+        ``routed_scaling_factor``.  (The serving engine does this for the reference's method.)  A layer that routes by a function of its own, or
+        whose experts are moved about while it serves, is refused."""
+        for name in ("custom_routing_function", "enable_eplb"):
+            if getattr(layer, name, None):
+                raise NotImplementedError(f"{name} is not supported by the router of the GGUF MoE methods.")
         grouped = getattr(layer, "use_grouped_topk", False)
         return ops.moe_route(router_logits, layer.top_k, scoring=getattr(layer, "scoring_func", "softmax"),
                              bias=getattr(layer, "e_score_correction_bias", None),
