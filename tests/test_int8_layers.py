@@ -131,6 +131,54 @@ def test_moe_layer_from_its_logits(native_libs, tokens):
         int8.apply(layer8, x, weights_, ids)
 
 
+@pytest.mark.gpu
+def test_moe_layer_loaded_again_in_part(native_libs):
+    """What arrives after the first loading takes the place of what it is, and of nothing else: one projection, one half of one, one expert."""
+    from vllm_gguf_plugin.quantization import Int8MoEMethod, int8_rows
+
+    e, h, i, t = 4, 96, 64, 8
+    method = Int8MoEMethod(None)
+    layer = moe_layer(method, t, t, e, h, i)
+    method.process_weights_after_loading(layer)
+    ids, weights_ = torch.tensor([[0, 1], [2, 3], [3, 0]], dtype=torch.int32, device=DEV), torch.full((3, 2), 0.5, device=DEV)
+    x = torch.randn(3, h, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).half()
+
+    def state():
+        return [layer.w13_int8.clone(), layer.w13_scales.clone(), layer.w2_int8.clone(), layer.w2_scales.clone()]
+
+    def load(name, sid, w, expert=0):
+        param = getattr(layer, name + "_weight")
+        param.weight_loader(param, w, "experts", shard_id=sid, expert_id=expert)
+
+    def rows(w):
+        codes, scales = int8_rows(w.reshape(-1, w.shape[-1]), t)
+        return codes.unflatten(0, w.shape[:-1]), scales.view(w.shape[:-1])
+
+    want, n = state(), 0
+    for name, sid, at, lead, r0, k in (("w2", "w2", 2, (e, h), 0, i), ("w13", "w3", 0, (e, i), i, h), ("w13", "w1", 0, (i,), 0, h), ("w2", "w2", 2, (h,), 0, i)):
+        n += 1
+        w = blocks(t, int(np.prod(lead)), k, seed=1000 + n).unflatten(0, lead)
+        load(name, sid, w, expert=3)
+        method.process_weights_after_loading(layer)
+        part = slice(None) if len(lead) == 2 else 3
+        want[at][part, r0:r0 + lead[-1]], want[at + 1][part, r0:r0 + lead[-1]] = rows(w)
+        assert all(torch.equal(a, b) for a, b in zip(state(), want)), (name, sid)
+        y = method.apply(layer, x, weights_, ids)
+        fresh = torch.nn.Module()
+        fresh.w13_int8, fresh.w13_scales, fresh.w2_int8, fresh.w2_scales = layer.w13_int8, want[1], layer.w2_int8, want[3]
+        assert torch.equal(y, method.apply(fresh, x, weights_, ids))
+    # all of it again, an expert at a time
+    for j in range(e):
+        for name, sid, r, k in (("w13", "w1", i, h), ("w13", "w3", i, h), ("w2", "w2", h, i)):
+            load(name, sid, blocks(t, r, k, seed=50 * j + r + len(sid)), expert=j)
+    whole = {n_: getattr(layer, n_ + "_weight").data.clone() for n_ in ("w13", "w2")}
+    method.process_weights_after_loading(layer)
+    got = state()
+    for at, n_ in ((0, "w13"), (2, "w2")):
+        codes, scales = rows(whole[n_])
+        assert torch.equal(got[at], codes) and torch.equal(got[at + 1], scales)
+
+
 def test_route_reads_the_layer(monkeypatch, native_libs):
     from vllm_gguf_plugin import ops
     from vllm_gguf_plugin.quantization import GGUFMoEMethod

@@ -82,16 +82,37 @@ class Int8MoEMethod(GGUFMoEMethod):
     """MoE method that loads like ``GGUFMoEMethod`` and multiplies 8-bit integers.  After loading a layer holds ``w13_int8 [E, 2I, H]``,
     ``w13_scales [E, 2I]``, ``w2_int8 [E, H, I]`` and ``w2_scales [E, H]``; the blocks are given back."""
 
+    @staticmethod
+    def _load_weight(param, loaded_weight, weight_name=None, shard_id=None, expert_id=None, return_success=False):
+        """As the blocks' loader, which puts zeros in place of what has not arrived; notes what has: (expert, or None for all; first row, rows)."""
+        rows = loaded_weight.shape[-2]
+        out = GGUFMoEMethod._load_weight(param, loaded_weight, weight_name, shard_id, expert_id, return_success)
+        if shard_id in ("w1", "w3"):   # (of this tensor-parallel rank)
+            rows = param.data.shape[1] // 2
+        param.arrived = getattr(param, "arrived", []) + [(None if loaded_weight.dim() == 3 else int(expert_id), rows if shard_id == "w3" else 0, rows)]
+        return out
+
     def process_weights_after_loading(self, layer: torch.nn.Module):
-        if layer.w13_weight.numel() == 0:
-            return
+        """What has arrived since the last call becomes 8-bit integers; rows that have not keep those they have."""
         for name in ("w13", "w2"):
             param, kind = getattr(layer, name + "_weight"), getattr(layer, name + "_weight_type").weight_type
+            if param.numel() == 0:
+                continue
             experts, rows, width = param.shape
-            codes, scales = int8_rows(param.data.reshape(experts * rows, width), kind)
-            _set(layer, name + "_int8", codes.unflatten(0, (experts, rows)))
-            _set(layer, name + "_scales", scales.view(experts, rows))
-            param.data = torch.empty(0, dtype=torch.uint8, device=codes.device)
+            per, size = quant_sizes(kind)
+            had = layer._parameters.get(name + "_int8")
+            if had is None or had.shape != (experts, rows, width // size * per):
+                codes, scales = int8_rows(param.data.reshape(experts * rows, width), kind)
+                _set(layer, name + "_int8", codes.unflatten(0, (experts, rows)))
+                _set(layer, name + "_scales", scales.view(experts, rows))
+            else:
+                for expert, first, count in getattr(param, "arrived", None) or [(None, 0, rows)]:
+                    part = slice(None) if expert is None else slice(expert, expert + 1)
+                    blocks = param.data[part, first:first + count]
+                    codes, scales = int8_rows(blocks.reshape(-1, width), kind)
+                    had.data[part, first:first + count] = codes.unflatten(0, blocks.shape[:2])
+                    getattr(layer, name + "_scales").data[part, first:first + count] = scales.view(blocks.shape[:2])
+            param.data, param.arrived = torch.empty(0, dtype=torch.uint8, device=param.device), []
 
     def apply(self, layer, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
               shared_experts=None, shared_experts_input: torch.Tensor | None = None) -> torch.Tensor:
