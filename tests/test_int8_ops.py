@@ -460,6 +460,80 @@ def test_moe_activation_of_exact_gates(ops, act, sign, size):
     assert bool((off <= room).all()), (float((off / want.abs().amax()).max()), float((room / want.abs().amax()).max()))
 
 
+class Guarded:
+    """A buffer between two stretches of a pattern that have to be found again; `skew` elements behind a multiple of 256 bytes."""
+
+    def __init__(self, n, dtype, skew=0):
+        size = torch.empty(0, dtype=dtype).element_size()
+        self.front, self.bytes = 1024 + skew * size, n * size
+        self.all = torch.full((self.front + self.bytes + 8192,), 0xA5, dtype=torch.uint8, device="cuda")
+        self.p = ctypes.c_void_p(self.all.data_ptr() + self.front)
+        self.view = self.all[self.front:self.front + self.bytes].view(dtype)
+
+    def check(self, what):
+        clean = bool((self.all[:self.front] == 0xA5).all()) and bool((self.all[self.front + self.bytes:] == 0xA5).all())
+        assert clean, f"{what}: written beside"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 131, 96), (1, 4096, 2048), (5, 2050, 1000), (8, 1, 40), (3, 2050, 9000), (20, 2100, 14000), (33, 127, 300), (257, 130, 640),
+                                   (520, 4225, 1030), (450, 9000, 528), (1000, 333, 144)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_is_written_beside_results(native_libs, m, n, k, dtype):
+    from gguf_b200 import capi
+
+    lib, code, stream = capi.lib(), DTYPES.index(dtype), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    w, ws = weights(n, k, gen)
+    x = torch.randn(m, k, device="cuda", generator=gen).to(dtype)
+    qwant, swant = codes_of(x)
+    pitch = (k + 15) // 16 * 16
+    q, qs = Guarded(m * pitch, torch.int8), Guarded(m, torch.float32, 1)
+    assert lib.gguf_b200_int8_quantize(x.data_ptr(), code, k, q.p, pitch, qs.p, m, k, stream) == 0
+    q.check("codes")
+    qs.check("scales")
+    assert torch.equal(q.view.view(m, pitch)[:, :k].double(), qwant)
+    assert bool((q.view.view(m, pitch)[:, k:] == torch.tensor(0xA5, dtype=torch.uint8).view(torch.int8)).all())   # (nor behind the values of a row)
+    room = lib.gguf_b200_int8_scratch_bytes(m, k)
+    for skew in (0, 1):       # (rows that 16-byte stores can be made to, and others)
+        y, scratch = Guarded(m * n, dtype, skew), Guarded(room, torch.uint8)
+        assert lib.gguf_b200_int8_mul_mat(w.data_ptr(), w.stride(0), ws.data_ptr(), x.data_ptr(), k, None, y.p, scratch.p, room, 0, code, m, n, k, stream) == 0
+        y.check("product")
+        scratch.check("workspace")
+        check_product(y.view.view(m, n), qwant, swant, w, ws, None, dtype)
+        z = Guarded(m * n, dtype, skew)
+        assert lib.gguf_b200_int8_mul_mat_prepared(w.data_ptr(), w.stride(0), ws.data_ptr(), q.p, pitch, qs.p, None, z.p, 0, code, m, n, k, stream) == 0
+        z.check("prepared")
+        assert torch.equal(z.view, y.view)
+    assert capi.last_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,i", [(1, 5, 3, 72, 40), (33, 16, 4, 264, 392), (1025, 65, 1, 64, 32), (2049, 64, 4, 64, 32), (300, 8, 2, 1160, 136)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_is_written_beside_the_results_of_experts(native_libs, t, e, k, h, i, dtype):
+    from gguf_b200 import capi
+
+    lib, code, stream = capi.lib(), DTYPES.index(dtype), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    gen = torch.Generator(device="cuda").manual_seed(t + h)
+    w13, s13, w2, s2 = experts(e, h, i, gen)
+    x = torch.randn(t, h, device="cuda", generator=gen).to(dtype)
+    logits = torch.randn(t, e, device="cuda", generator=gen)
+    rw, ids = Guarded(t * k, torch.float32, 1), Guarded(t * k, torch.int32, 3)
+    assert lib.gguf_b200_moe_route(logits.data_ptr(), 0, e, None, rw.p, ids.p, t, e, k, 1, 1, 1, 1, 1.0, stream) == 0
+    rw.check("weights")
+    ids.check("ids")
+    ids.view[::7] = -1
+    room = lib.gguf_b200_int8_moe_workspace_bytes(t, k, e, h, i)
+    y, scratch = Guarded(t * h, dtype), Guarded(room, torch.uint8)
+    assert lib.gguf_b200_int8_fused_moe(x.data_ptr(), h, w13.data_ptr(), w13.stride(1), s13.data_ptr(), w2.data_ptr(), w2.stride(1), s2.data_ptr(), y.p, ids.p, rw.p,
+                                        scratch.p, room, code, 1, t, k, e, h, i, stream) == 0
+    y.check("result")
+    scratch.check("workspace")
+    assert torch.equal(y.view.view(t, h), capi.int8_fused_moe(x, w13, s13, w2, s2, rw.view.clone().view(t, k), ids.view.clone().view(t, k)))
+    assert capi.last_status() == 0
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 
