@@ -228,3 +228,60 @@ def test_traced_layer_is_one_operator(native_libs, types):
             if dtype == torch.float16 or 23 not in types:
                 assert calls == ["_C_gguf.linear_runs.default"], calls
             assert method.apply(layer, x).shape == (3, 32)
+
+
+@pytest.mark.parametrize("tokens,experts", [(5, 300), (70, 12)])
+def test_unfused_moe_leaves_out_slots_without_an_expert(native_libs, monkeypatch, tokens, experts):
+    """Ids of -1, as the router gives them for places without an expert: no product writes their rows, which are whatever the memory held, here NaN, and a
+    routing weight of 0 would not take that away.  (Steps of more than 256 experts, and all of them with VLLM_GGUF_FUSED_MOE=0, go this way.)"""
+    from vllm_gguf_plugin import ops
+    from vllm_gguf_plugin.quantization import fused_moe as fm
+
+    monkeypatch.setenv("VLLM_GGUF_FUSED_MOE", "0")
+    h, i, k = 8, 4, 3
+    gen = torch.Generator().manual_seed(tokens)
+    w1, w2 = torch.randn(experts, 2 * i, h, generator=gen), torch.randn(experts, h, i, generator=gen)
+    aligned = []
+
+    def vec(x, w, ids, top_k, weight_type, n, t):
+        assert ids.dtype == torch.int32 and ids.is_contiguous()
+        out = torch.full((ids.numel(), n), float("nan"))
+        for s, e in enumerate(ids.flatten().tolist()):
+            if 0 <= e < experts:
+                out[s] = w[e] @ x[s // top_k]
+        return out
+
+    def align(ids, block, n):
+        assert int(ids.min()) >= 0 and int(ids.max()) < n
+        aligned.append(ids)
+        return fm.moe_align_block_size_torch(ids, block, n)
+
+    def grouped(x, w, sorted_ids, expert_ids, post, weight_type, n, top_k, t):
+        out = torch.full((t * top_k if top_k > 1 else x.shape[0], n), float("nan"))
+        for b, e in enumerate(expert_ids.tolist()):
+            for s in sorted_ids[4 * b:4 * b + 4].tolist():
+                if s < out.shape[0] and 4 * b < int(post):
+                    out[s] = w[e] @ x[s // top_k]
+        return out
+
+    monkeypatch.setattr(ops, "ggml_moe_a8_vec", vec)
+    monkeypatch.setattr(ops, "ggml_moe_a8", grouped)
+    monkeypatch.setattr(ops, "ggml_moe_get_block_size", lambda t: 4)
+    monkeypatch.setattr(ops, "moe_sum", lambda x, out: out.copy_(x.sum(1)))
+    monkeypatch.setattr(fm, "_align", align)
+    monkeypatch.setattr(fm, "_act", lambda name, x: torch.nn.functional.silu(x[..., :i]) * x[..., i:])
+    x = torch.randn(tokens, h, generator=gen)
+    ids = torch.stack([torch.randperm(experts, generator=gen)[:k] for _ in range(tokens)]).to(torch.int32)
+    weights = torch.rand(tokens, k, generator=gen)
+    ids[0], ids[2, 1], ids[3, 2] = -1, -1, experts
+    weights[0], weights[2, 1], weights[3, 2] = 0, 0, 0
+    y = fm._fused_moe_gguf(x, w1, w2, weights, ids, 8, 8, "silu")
+    want = torch.zeros(tokens, h)
+    for t in range(tokens):
+        for j in range(k):
+            e = int(ids[t, j])
+            if 0 <= e < experts:
+                both = w1[e] @ x[t]
+                want[t] += weights[t, j] * (w2[e] @ (torch.nn.functional.silu(both[:i]) * both[i:]))
+    assert torch.allclose(y, want, rtol=1e-4, atol=1e-4) and not bool(y[0].any())
+    assert len(aligned) == (tokens > 64)

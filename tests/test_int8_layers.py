@@ -132,6 +132,31 @@ def test_moe_layer_from_its_logits(native_libs, tokens):
 
 
 @pytest.mark.gpu
+def test_layer_of_more_than_256_experts_behind_the_router(native_libs):
+    """Block formats, a padded row and a row with fewer experts than places: nothing comes from the places that are left."""
+    from vllm_gguf_plugin.quantization import GGUFMoEMethod
+
+    e, h, i = 260, 64, 32
+    method = GGUFMoEMethod(None)
+    layer = moe_layer(method, 8, 8, e, h, i)
+    layer.top_k = 4
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(6, h, device=DEV, generator=gen).half()
+    logits = torch.randn(6, e, device=DEV, generator=gen)
+    logits[2] = float("-inf")
+    logits[4] = float("-inf")
+    logits[4, 259] = 1.0
+    junk = torch.full((1 << 20,), float("nan"), device=DEV)   # (what the next buffers find)
+    del junk
+    y = method.apply_logits(layer, x, logits)
+    weights_, ids = method.route(layer, logits)
+    assert ids[2].tolist() == [-1] * 4 and ids[4].tolist() == [259, -1, -1, -1]
+    assert not bool(y[2].any()) and bool(torch.isfinite(y).all())
+    alone = method.apply(layer, x[4:5], torch.ones(1, 1, device=DEV), torch.full((1, 1), 259, dtype=torch.int32, device=DEV))
+    assert torch.equal(y[4:5], alone)
+
+
+@pytest.mark.gpu
 def test_moe_layer_loaded_again_in_part(native_libs):
     """What arrives after the first loading takes the place of what it is, and of nothing else: one projection, one half of one, one expert."""
     from vllm_gguf_plugin.quantization import Int8MoEMethod, int8_rows

@@ -107,10 +107,12 @@ def _fused_moe_gguf(
             and os.environ.get("VLLM_GGUF_FUSED_MOE", "1") == "1"):
         # one call: alignment, both expert products, activation, routing weights and top-k sum
         return ops.ggml_fused_moe(x, w1, w2, topk_weights, topk_ids, weight_type, weight_type2, activation)
+    # Slots without an expert (an id outside [0, E), as the router gives them where none is left): out of the result, whatever their rows hold.
+    without = (topk_ids < 0) | (topk_ids >= E)
     if weight_type2 in MMQ_QUANT_TYPES and weight_type in MMQ_QUANT_TYPES and x.shape[0] > 64:
         # the reference's sequence of separate ops (fused_moe.py:64-95)
         block_size = ops.ggml_moe_get_block_size(weight_type)
-        sorted_token_ids, expert_ids, num_tokens_post_padded = _align(topk_ids, block_size, E)
+        sorted_token_ids, expert_ids, num_tokens_post_padded = _align(topk_ids.masked_fill(without, 0), block_size, E)
         out = ops.ggml_moe_a8(x, w1, sorted_token_ids, expert_ids, num_tokens_post_padded, weight_type, N, top_k,
                               num_tokens)
         out = _act(activation, out)
@@ -125,6 +127,7 @@ def _fused_moe_gguf(
         raise NotImplementedError(
             f"no GGUF MoE kernel for quantization types ({int(weight_type)}, {int(weight_type2)})")
     out = out.reshape(num_tokens, top_k, w2.shape[1]).mul_(topk_weights.view(num_tokens, top_k, 1).to(out.dtype))
+    out.masked_fill_(without.view(num_tokens, top_k, 1), 0)
     out_hidden_states = torch.empty_like(x)
     ops.moe_sum(out, out_hidden_states)
     return out_hidden_states
