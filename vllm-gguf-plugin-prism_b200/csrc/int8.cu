@@ -154,9 +154,10 @@ __device__ __forceinline__ float i8_silu(float g) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + z));
   return (g < 0.f ? g * z : g) * r;
 }
-// g Phi(g) = g / 2 erfc(-g / sqrt 2): relative to itself to 2^-20 for gates of both signs (1 + erf would cancel: nothing is left of it at -6).  What
+// g Phi(g) = g / 2 erfc(-g / sqrt 2), relative to itself to 2^-20 for gates of both signs (1 + erf would cancel: nothing is left of it at -6).  What
 // -g / sqrt 2 lost is put back by the derivative, erfc(x + d) = erfc(x) (1 - 2 x d) for x > 0 up to a few 2^-24: at -8 it would be 64 roundings.
-__device__ __forceinline__ float i8_gelu(float g) {
+// (One copy: in line, eight times over, a step of 200 tokens over 32 experts took 41.3 us instead of 39.5, one of 2048 with SiLU 201 instead of 199.5.)
+static __device__ __noinline__ float i8_gelu(float g) {
   constexpr float HI = 0.70710678f, LO = 1.2101617e-8f;   // 1 / sqrt 2 in two parts
   const float x = -g * HI, lost = fmaf(-g, LO, fmaf(-g, HI, -x)), y = 0.5f * g * erfcf(x);
   return x > 0.f ? fmaf(y * -2.f * x, lost, y) : y;

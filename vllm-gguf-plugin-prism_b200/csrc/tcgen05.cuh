@@ -1,5 +1,5 @@
 // tcgen05 (5th-generation tensor core) instructions, tensor memory and matrix descriptors, as the tiled GEMM (mmq_kernel.cuh) and
-// the 8-bit integer product (int8_kernel.cuh) use them.
+// the 8-bit integer product (int8.cu) use them.
 #pragma once
 
 #include "common.cuh"
