@@ -4,14 +4,15 @@
 //                   takes up to 1024 slots; of more, a cluster of eight blocks takes equal runs, which learn of one another's counts
 //                   through shared memory.  A warp counts its share of the run and, once the sums over warps, blocks and experts are
 //                   there, places it, 32 slots at a time.
-//                   Latencies bound it: 16384 slots of 64 experts 8.4 us behind the kernel ahead, 64 slots 3.1 (10.6 with 16 blocks that
-//                   each counted all slots and summed over their warps for every 1024 of them, and 4.5 with divisions between the sums).
-//   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * weight, in fp32, rounded once.
+//                   Latencies bound it: 16384 slots of 64 experts 9 us behind the kernel ahead, 11 alone with cold caches; 64 slots 6.5 so.  (16 blocks
+//                   that each counted all slots and summed over their warps for every 1024 of them took 2 us more, divisions between the sums 1.4.)
+//   i8_sum_kernel   out[t] = sum over j of y[t * top_k + j] * weight, in fp32, rounded once.  Bound by memory: 2048 tokens of 2048 columns, eight
+//                   experts, 134 MB in 27 to 28 us (20.8 at the copy rate, beside what L2 still has to write of them).
 //
 // The experts' results travel from the down product to the sum in fp32, whatever the tokens' type: the step's largest buffer, 134 MB for 2048 tokens
-// of 2048 columns with eight experts each, written and read again.  (In fp16, with powers of two taken out, the same step took 200 us instead of
-// 224, but an fp16 result was off by 2.9e-4 instead of 2.0e-4, and rows of W2 whose scale is far below the expert's largest lost their bits.
-// The product and the sum in two halves of the columns, so that the buffer stays in L2: 226.)
+// of 2048 columns with eight experts each, written and read again.  (In fp16, with powers of two taken out, the same step took 196 us instead of
+// 221, but an fp16 result was off by 2.9e-4 instead of 2.0e-4, and rows of W2 whose scale is far below the expert's largest lost their bits.
+// The product and the sum in two halves of the columns, so that the buffer stays in L2: level.)
 #include <math.h>
 
 #include "common.cuh"

@@ -14,7 +14,7 @@
 // More than 32 candidates, an order of groups that is not settled and a softmax with a bias (which wants its sum in fp64) do the whole row again.
 //
 // Bound by the integer pipe, which runs at half the issue rate, and by the last row that is done again: 8192 tokens, 256 experts in eight
-// groups with a bias, 15.4 us (17.8 where a row is among them whose groups are not settled; 45 with 64-bit keys throughout, 24 with keys that
+// groups with a bias, 15.2 us (up to 19.3 where rows are among them whose groups are not settled; 45 with 64-bit keys throughout, 24 with keys that
 // kept 0 for "out", exact maxima for every row and fp64 in the weights, 19 to 20 with whole rows done again); fp32 logits with equals, no groups,
 // 11.1 (16.2 with whole rows, though 6.8 and not 6.6 for 64 experts without equals).  A token alone 2.5, of which the launch is most.
 #include "common.cuh"

@@ -312,7 +312,9 @@ def int8_mul_mat(W: torch.Tensor, w_scales: torch.Tensor, X: torch.Tensor, bias:
 
 def int8_mul_mat_prepared(W: torch.Tensor, w_scales: torch.Tensor, Q: torch.Tensor, q_scales: torch.Tensor, dtype: torch.dtype,
                           bias: torch.Tensor | None = None) -> torch.Tensor:
-    """``int8_mul_mat`` on what ``int8_quantize`` made of the activations, for several products of the same ones."""
+    """``int8_mul_mat`` on what ``int8_quantize`` made of the activations, for several products of the same ones.  It goes through the dispatcher and takes
+    the weights as ones that may still be written.  For q/k/v of 4096 values (rows 4096, 1024, 1024) against three ``int8_mul_mat``: in a CUDA graph one
+    token 19.4 us (16.8), eight 19.2 (22.9), 512 32.9 (36.6); in eager calls 49 (24), 33 (30), 49 (38), and less from some 2000 tokens on, 58 (68)."""
     return torch.ops._C_gguf.int8_mul_mat_prepared(W, w_scales, Q, q_scales, bias, dtype)
 
 
